@@ -1,9 +1,12 @@
-"""What is measured of two operators of a diffusion transformer's block, next to its attention:
+"""What is measured of three operators of a diffusion transformer's block, next to its sparse attention:
 
 * ``rope``: rotary positions with several axes (frame, row, column) of the queries and keys, and its gradient
   (the inverse rotation);
 * ``lora``: the low-rank adapters of many requests beside a shared projection, out = y + scale (x A^T) B^T with each
-  request's own A and B on its own rows; ``lora_step`` is the same with its backward pass, as a training step takes it.
+  request's own A and B on its own rows; ``lora_step`` is the same with its backward pass, as a training step takes it;
+* ``kv8``: attention over keys and values held in 8 bits, in pages of 64 tokens with a power-of-two scale for each
+  page and head, and the write of new tokens into them: the text of a prompt, kept over all denoising steps, or the
+  frames so far of a video that is made chunk by chunk.
 
 ``run`` computes them in elementary torch operations, or with ``own`` set through this package's entry points.
 """
@@ -24,11 +27,10 @@ def listed():
     return [
         # Wan2.1-14B at 720p, one denoising step's self-attention: 21 x 45 x 80 latent patches, head-major
         rope_case("rope_wan14b_720p", heads=40, kv_heads=40, grid=[21, 45, 80], axes=[44, 42, 42]),
-        # one latent frame of Wan2.1-1.3B at 480p (an image): latency and L2
-        rope_case("rope_wan1b_frame", heads=12, kv_heads=12, grid=[1, 30, 52], axes=[44, 42, 42], origin=[7, 0, 0]),
-        # HunyuanVideo at 720p: the video part of a sequence whose last 256 tokens are text
-        rope_case("rope_hunyuan_720p", heads=24, kv_heads=24, grid=[33, 45, 80], axes=[16, 56, 56], theta=256.0,
-                  tail=256),
+        # one latent frame with HunyuanVideo's heads at 480p, the video part of a sequence whose last 256 tokens are
+        # text: latency and L2
+        rope_case("rope_hunyuan_frame", heads=24, kv_heads=24, grid=[1, 30, 52], axes=[16, 56, 56], theta=256.0,
+                  origin=[7, 0, 0], tail=256),
         # gradients in fp32 of a packed batch with a position for every token, token-major, grouped keys
         rope_case("rope_grad_tokens_f32", batch=2, heads=16, kv_heads=4, dim=80, tokens=4111, axes=[16, 24, 24],
                   dtype="f32", token_major=True, inverse=True),
@@ -37,8 +39,6 @@ def listed():
                   far=1 << 20),
         # one style adapter on a square projection of Wan2.1-14B at 720p
         lora_case("lora_wan14b_720p", lengths=[75600], k=5120, n=5120, rank=32, adapters=1),
-        # the two halves of a guided step of Wan2.1-1.3B at 480p, each with its own adapter, on the FFN's first product
-        lora_case("lora_wan1b_ffn", lengths=[32760, 32760], k=1536, n=8960, rank=64, adapters=2),
         # prompts of ragged lengths into the cross-attention's keys; some without an adapter, a padded tail
         lora_case("lora_text_ragged", lengths=[512, 77, 1, 0, 300, 509, 64, 33, 128, 512, 255, 400, 17, 226, 512, 441],
                   k=5120, n=5120, rank=16, adapters=8, pad=109, without=3),
@@ -49,8 +49,13 @@ def listed():
         # training three adapters at once on ragged rows, the widest rank
         lora_case("lora_step_ragged", op="lora_step", lengths=[1560, 3000, 77, 4000, 1], k=1536, n=8960, rank=128,
                   adapters=3, pad=47, without=5),
-        # training on a handful of rows: latency
-        lora_case("lora_step_small", op="lora_step", lengths=[100, 30], k=1536, n=1536, rank=8, adapters=2),
+        # cross-attention of a guided step of Wan2.1-14B at 480p: the prompt's and the negative prompt's text
+        kv8_case("kv8_text_wan14b", heads=40, kv_heads=40, queries=32760, lengths=[512, 77]),
+        # the next three latent frames of a video at 480p with the heads of Wan2.1-1.3B join nine before them
+        kv8_case("kv8_chunk_wan1b", heads=12, kv_heads=12, queries=4680, lengths=[14040], append=True),
+        # one new token of each of eight requests, grouped keys, long caches
+        kv8_case("kv8_one_token", heads=40, kv_heads=8, queries=1, append=True,
+                 lengths=[32767, 20000, 32000, 777, 15000, 31001, 130, 24576]),
     ]
 
 
@@ -73,6 +78,14 @@ def lora_case(name=None, *, op="lora", lengths, k, n, rank, adapters, pad=0, wit
     return {"name": name, **case} if name else case
 
 
+def kv8_case(name=None, *, heads, kv_heads, dim=128, queries, lengths, append=False):
+    """``lengths``: tokens that each request has in the cache; ``append``: the queries' own keys and values are
+    written behind them first."""
+    case = {"op": "kv8", "heads": heads, "kv_heads": kv_heads, "dim": dim, "queries": queries,
+            "lengths": text(lengths), "append": append}
+    return {"name": name, **case} if name else case
+
+
 def text(values):
     return " ".join(map(str, values))
 
@@ -86,8 +99,8 @@ def log_uniform(rng, lo, hi):
 
 
 def draw(rng):
-    op = rng.choice(["rope", "lora", "lora_step"])
-    return draw_rope(rng) if op == "rope" else draw_lora(rng, op)
+    op = rng.choice(["rope", "lora", "lora_step", "kv8"])
+    return draw_rope(rng) if op == "rope" else draw_kv8(rng) if op == "kv8" else draw_lora(rng, op)
 
 
 def draw_rope(rng):
@@ -127,6 +140,17 @@ def draw_lora(rng, op):
                      without=rng.choice([0, 0, 3]))
 
 
+def draw_kv8(rng):
+    kv_heads = rng.choice([1, 4, 8, 12, 24, 40])
+    heads = kv_heads * rng.choice([1] if kv_heads > 8 else [1, 2, 5, 8])
+    batch = rng.choice([1, 1, 2, 5, 16])
+    queries = log_uniform(rng, 1, min(33000, 2 * 10 ** 6 // (batch * heads)))
+    most = max(1, min(40000, 10 ** 9 // (heads * batch * queries)))  # scores of the plain form
+    lengths = [rng.choice([0, 1, 64, 1000]) if rng.random() < 0.2 else log_uniform(rng, 1, most) for _ in range(batch)]
+    return kv8_case(heads=heads, kv_heads=kv_heads, dim=rng.choice([64, 128, 128]), queries=queries,
+                    lengths=[min(n, most) for n in lengths], append=queries <= most and rng.random() < 0.5)
+
+
 # ---------------------------------------------------------------------------
 # inputs
 # ---------------------------------------------------------------------------
@@ -137,7 +161,7 @@ def unpacked(case):
 def prepare(case, seed):
     case = unpacked(case)
     g = torch.Generator(device=DEVICE).manual_seed(seed)
-    return prepare_rope(case, g) if case["op"] == "rope" else prepare_lora(case, g)
+    return {"rope": prepare_rope, "kv8": prepare_kv8}.get(case["op"], prepare_lora)(case, g)
 
 
 def prepare_rope(case, g):
@@ -181,13 +205,50 @@ def prepare_lora(case, g):
     return state
 
 
+PAGE = 64
+
+
+def prepare_kv8(case, g):
+    """Token-major queries (a projection's output) and a cache whose pages lie in no order, filled from unit keys and
+    values; the pages' rows behind a request's last token hold what an earlier owner left."""
+    batch, dim, heads = len(case["lengths"]), case["dim"], case["kv_heads"]
+    added = case["queries"] if case["append"] else 0
+    need = [-(-(n + added) // PAGE) for n in case["lengths"]]
+    pages = sum(need) + 3
+    order = torch.randperm(pages, generator=g, device=DEVICE).int()
+    table = torch.full((batch, max(1, max(need))), -1, device=DEVICE, dtype=torch.int32)
+    first = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[first:first + n]
+        first += n
+    randn = lambda *shape: torch.randn(shape, generator=g, device=DEVICE, dtype=torch.bfloat16)  # noqa: E731
+    cache = []
+    for _ in range(2):
+        values = randn(pages, heads, PAGE, dim)
+        scale = page_scale(values.abs().amax(dim=(2, 3)).float())
+        cache += [(values / scale[..., None, None]).to(torch.float8_e4m3fn), scale]
+    state = {"case": case, "q": randn(batch, case["queries"], case["heads"], dim).transpose(1, 2),
+             "cache": (cache[0], cache[2], cache[1], cache[3]), "table": table,
+             "starts": torch.tensor(case["lengths"], device=DEVICE, dtype=torch.int32),
+             "lengths": torch.tensor([n + added for n in case["lengths"]], device=DEVICE, dtype=torch.int32)}
+    if added:
+        state["k"], state["v"] = (randn(batch, added, heads, dim).transpose(1, 2) for _ in range(2))
+    return state
+
+
+def page_scale(amax):
+    """The smallest power of two (2^-100 at least) that brings amax to 448, e4m3's largest value, or below."""
+    fraction, exponent = torch.frexp(amax)
+    exponent = torch.where(fraction <= 0.875, exponent - 9, exponent - 8)
+    return torch.ldexp(torch.ones_like(amax), torch.where(amax > 0, exponent, -100).clamp_min(-100))
+
+
 # ---------------------------------------------------------------------------
 # one pass
 # ---------------------------------------------------------------------------
 def run(state):
-    if state["case"]["op"] == "rope":
-        return run_rope(state)
-    return run_lora(state) if state["case"]["op"] == "lora" else run_lora_step(state)
+    op = state["case"]["op"]
+    return {"rope": run_rope, "lora": run_lora, "lora_step": run_lora_step, "kv8": run_kv8}[op](state)
 
 
 def run_rope(s):
@@ -265,6 +326,59 @@ def run_lora_step(s):
     return out, dx, da, db
 
 
+def run_kv8(s):
+    """The attention's output, after an append the cache too."""
+    case = s["case"]
+    if own:
+        from pasa_b200 import ops
+        if case["append"]:
+            ops.kv8_write(s["cache"], s["k"], s["v"], s["table"], s["starts"])
+        out = ops.kv8_attention(s["q"], s["cache"], s["table"], s["lengths"])
+        return (out, *s["cache"]) if case["append"] else out
+    k, v, k_scale, v_scale = s["cache"]
+    if case["append"]:
+        append(k, k_scale, s["k"], s["table"], s["starts"])
+        append(v, v_scale, s["v"], s["table"], s["starts"])
+    table, lengths = s["table"].clamp_min(0).long(), s["lengths"]
+    keys, values = ((c[table].float() * scale[table][..., None, None]).transpose(1, 2).flatten(2, 3)
+                    for c, scale in ((k, k_scale), (v, v_scale)))  # [B, kv heads, tokens, D]
+    inside = torch.arange(keys.shape[2], device=DEVICE) < lengths[:, None, None, None]
+    q = s["q"].float().unflatten(1, (case["kv_heads"], -1)).flatten(2, 3)  # a group's queries share their keys
+    score = (q @ keys.transpose(2, 3)) * case["dim"] ** -0.5
+    score.masked_fill_(~inside, -math.inf)
+    top = score.amax(dim=3, keepdim=True)
+    p = score.sub_(torch.where(top > -math.inf, top, 0.0)).exp_()  # a request without tokens: all zero
+    total = p.sum(dim=3, keepdim=True)
+    out = (p @ values) / torch.where(total > 0, total, 1.0)
+    out = out.to(s["q"].dtype).unflatten(2, (-1, case["queries"])).flatten(1, 2)
+    return (out, *s["cache"]) if case["append"] else out
+
+
+def append(cache, scales, new, table, starts):
+    """Writes new [B, H, L, D] behind ``starts`` tokens.  A page's scale is its new tokens'; where it has earlier
+    tokens it is the larger of theirs and that, and they are rounded to it."""
+    batch, heads, count, dim = new.shape
+    token = starts[:, None].long() + torch.arange(count, device=DEVICE)  # [B, L]
+    block = token // PAGE - (starts[:, None] // PAGE)
+    blocks = (PAGE - 1 + count + PAGE - 1) // PAGE
+    amax = torch.zeros((batch, heads, blocks), device=DEVICE).scatter_reduce(
+        2, block[:, None].expand(-1, heads, -1), new.abs().amax(dim=3).float(), "amax")
+    scale = page_scale(amax)
+    first, held = table.long().gather(1, (starts[:, None] // PAGE).long().clamp_max(table.shape[1] - 1)), starts % PAGE
+    first = first[:, 0].clamp_min(0)
+    old = scales[first]  # [B, H]
+    scale[:, :, 0] = torch.where(held[:, None] > 0, torch.maximum(old, scale[:, :, 0]), scale[:, :, 0])
+    earlier = cache[first].float() * (old / scale[:, :, 0])[..., None, None]
+    keep = (torch.arange(PAGE, device=DEVICE) < held[:, None])[:, None, :, None]
+    cache[first] = torch.where(keep, earlier, cache[first].float()).to(cache.dtype)
+    page = table.long().gather(1, token // PAGE)
+    mine = scale.gather(2, block[:, None].expand(-1, heads, -1))  # [B, H, L]
+    head = torch.arange(heads, device=DEVICE)[None, :, None]
+    cache.view(torch.uint8)[page[:, None], head, (token % PAGE)[:, None]] = \
+        (new.float() / mine[..., None]).to(cache.dtype).view(torch.uint8)
+    scales[page[:, None], head] = mine
+
+
 # ---------------------------------------------------------------------------
 # what a pass cannot do without, and the results in 64 bits
 # ---------------------------------------------------------------------------
@@ -275,6 +389,15 @@ def work(case):
         size = 4 if case["dtype"] == "f32" else 2
         where = 0 if case["grid"] else case["batch"] * case["tokens"] * len(case["axes"]) * 4
         return {"bytes": 2 * values * size + where, "flops": 3 * values}
+    if case["op"] == "kv8":
+        added = case["queries"] if case["append"] else 0
+        kv = 2 * case["kv_heads"] * case["dim"]  # values of one token's key and value
+        q = len(case["lengths"]) * case["queries"] * case["heads"] * case["dim"]
+        tokens = [n + added for n in case["lengths"]]
+        # q and its result; each cached token once, a page's scales; a new one read in 16 bits and written in 8
+        moved = 4 * q + kv * sum(case["lengths"]) + 8 * case["kv_heads"] * sum(-(-n // PAGE) for n in tokens)
+        return {"bytes": moved + 3 * kv * added * len(tokens),
+                "flops": 4 * case["heads"] * case["dim"] * case["queries"] * sum(tokens)}
     k, n, rank, adapters = (case[name] for name in ("k", "n", "rank", "adapters"))
     with_adapter = [i for i, length in enumerate(case["lengths"])
                     if length and not (case["without"] and (i + 1) % case["without"] == 0)]
@@ -291,7 +414,7 @@ def work(case):
 def exact(case, seed):
     state = prepare(case, seed)
     case = state["case"]
-    return exact_rope(case, state) if case["op"] == "rope" else exact_lora(case, state)
+    return {"rope": exact_rope, "kv8": exact_kv8}.get(case["op"], exact_lora)(case, state)
 
 
 def exact_rope(case, s):
@@ -350,3 +473,39 @@ def exact_lora(case, s):
             da[slot] += scale * g.T.matmul(x)
             db[slot] += scale * dy.T.matmul(h)
     return out if dx is None else (out, dx, da, db)
+
+
+def exact_kv8(case, s):
+    """Request by request and head by head.  What is rounded to 8 bits has no value in 64."""
+    k, v, k_scale, v_scale = s["cache"]
+    out = torch.zeros(s["q"].shape, device=DEVICE, dtype=torch.float64)
+    group = case["heads"] // case["kv_heads"]
+    for i, count in enumerate(case["lengths"]):
+        pages = s["table"][i].tolist()
+        for head in range(case["kv_heads"]):
+            rows = []
+            for source, scale, new in ((k, k_scale, s.get("k")), (v, v_scale, s.get("v"))):
+                used = pages[:-(-count // PAGE)]
+                row = (source[used, head].double() * scale[used, head].double()[:, None, None]).flatten(0, 1)[:count]
+                rows.append(row if new is None else held(row, scale[used, head], new[i, head], count))
+            keys, values = rows
+            for h in range(head * group, (head + 1) * group):
+                if len(keys):
+                    weights = torch.softmax(s["q"][i, h].double().matmul(keys.T) / math.sqrt(case["dim"]), dim=1)
+                    out[i, h] = weights.matmul(values)
+    return (out, None, None, None, None) if case["append"] else out
+
+
+def held(row, scale, new, count):
+    """The values that a head's pages hold after ``new`` has been written behind its ``count`` tokens."""
+    row, new = row.clone(), new.double()
+    first = count // PAGE * PAGE  # of the page that the new tokens begin in
+    parts = [row[:first]]
+    for at in range(first, count + len(new), PAGE):
+        mine = new[max(0, at - count):at + PAGE - count]
+        step = page_scale(mine.abs().max().float()).double()
+        kept = row[at:] if at < count else row[:0]
+        if len(kept):
+            step = torch.maximum(step, scale[-1].double())
+        parts += [(part / step).to(torch.float8_e4m3fn).double() * step for part in (kept.float(), mine.float())]
+    return torch.cat(parts)
