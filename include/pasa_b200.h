@@ -402,6 +402,49 @@ PASA_API int pasa_forward_scatter(void* stream, const void* q, const void* k, co
               const float* noise, void* workspace, size_t workspace_bytes,
               void* const* o_peer_table, int n_ranks, int64_t head0, int64_t heads_total, int kernel);
 
+/*
+ * Rotary positions with several axes, without a table.  Pair p of the first
+ * sum(axes) dimensions is turned by the angle pos[axis of p] * freqs[p]; the
+ * dimensions behind them are copied.  The axes' pairs follow one another:
+ * axes[0] / 2 pairs of axis 0, then those of axis 1, and so on.
+ *   tensors     host array of 1 or 2 tensors (queries, keys), each
+ *               [batch, heads, tokens, dim] with unit stride in dim and any
+ *               strides before it; out may be x itself (the same strides) and
+ *               must not overlap it otherwise
+ *   positions   [tokens, n_axes] (pos_batch_stride 0) or [batch, tokens,
+ *               n_axes], device; or NULL: token t is point t of the row-major
+ *               grid (host, n_axes sizes, product = tokens), counted from
+ *               origin (host, or NULL for zeros)
+ *   axes, freqs host: even dimensions of each axis (sum <= dim, <= 256), and
+ *               sum / 2 frequencies in radians
+ *   inverse     turn by the negative angles; also the gradient of the forward
+ * Nothing to do (0 tokens, heads or batch entries) is PASA_OK.
+ */
+typedef enum pasa_pos_type {
+  PASA_POS_I32 = 0,
+  PASA_POS_I64 = 1,
+  PASA_POS_F32 = 2,
+  PASA_POS_F64 = 3
+} pasa_pos_type;
+
+typedef enum pasa_pairing {
+  PASA_PAIRS_INTERLEAVED = 0, /* pair p is dimensions 2p, 2p + 1      */
+  PASA_PAIRS_HALVES = 1       /* pair p is dimensions p, p + sum / 2  */
+} pasa_pairing;
+
+typedef struct pasa_rope_tensor {
+  const void* x;
+  void* out;
+  int64_t heads;
+  int64_t x_stride[3];   /* batch, head, token, in elements */
+  int64_t out_stride[3];
+} pasa_rope_tensor;
+
+PASA_API int pasa_rope_axes(void* stream, const pasa_rope_tensor* tensors, int n_tensors, int dtype,
+              int64_t batch, int64_t tokens, int dim, const void* positions, int pos_type,
+              int64_t pos_batch_stride, const int64_t* grid, const int64_t* origin, int n_axes,
+              const int* axes, const double* freqs, int pairing, int inverse);
+
 #ifdef __cplusplus
 }
 #endif

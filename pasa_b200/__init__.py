@@ -3,7 +3,8 @@
 Drop-in for ZHANGWENTAI/PASA's ``pisa_pg_attention``
 (svg/kernels/triton/group_pisa_attention.py) and the HunyuanVideo token
 placement (svg/models/hyvideo/placement.py), running hand-written CUDA
-through the C ABI in ``include/pasa_b200.h``.
+through the C ABI in ``include/pasa_b200.h``; and the operators around it
+that have no counterpart there (rotary positions with several axes).
 """
 from .ops import (  # noqa: F401
     dense_attention,
@@ -13,6 +14,7 @@ from .ops import (  # noqa: F401
     pisa_pg_attention,
     pisa_pg_attention_host,
     pisa_pg_attention_range,
+    rope_axes,
 )
 
 __all__ = [
@@ -23,4 +25,5 @@ __all__ = [
     "piecewise_sparse_attention",
     "hunyuan_sparse_head_placement",
     "hunyuan_hidden_states_placement",
+    "rope_axes",
 ]

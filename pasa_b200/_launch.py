@@ -1,0 +1,52 @@
+"""What the operators with modules of their own share: argument checks, the launch on the tensors' device and its
+current stream, and the rule for gradients under stream capture."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+
+def check_cuda(name: str, t: torch.Tensor, dims: Optional[int] = None, dtypes=None,
+               device: Optional[torch.device] = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (pasa_b200 has no CPU path)")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+
+
+def launch(fn: str, device: torch.device, *args) -> None:
+    """Calls a C entry point on ``device``'s current stream and maps its status to an exception."""
+    entry = getattr(_lib.load(), fn)
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = entry(torch.cuda.current_stream(index).cuda_stream, *args)
+    else:
+        with torch.cuda.device(index):
+            code = entry(torch.cuda.current_stream(index).cuda_stream, *args)
+    if code:
+        _lib.check(fn, code)
+
+
+def wants_grad(fn: str, *tensors) -> bool:
+    """Whether autograd has to see this call.  While a stream is captured that is refused: the engine may run leaves'
+    accumulation on the stream of an eager graph of the same leaves, which a capture cannot contain."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{fn}: autograd is not recorded into a CUDA graph; capture the explicit forward and "
+                           "gradient calls under torch.no_grad()")
+    return True
+
+
+def overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements share memory, for the strides that views have (a broadcast dimension)."""
+    return any(size > 1 and stride == 0 for size, stride in zip(t.shape, t.stride()))

@@ -41,6 +41,9 @@ MODEL_WAN = 1
 
 PEER_HANDLE_BYTES = 64
 
+POS_I32, POS_I64, POS_F32, POS_F64 = 0, 1, 2, 3
+PAIRS_INTERLEAVED, PAIRS_HALVES = 0, 1
+
 EXPORTS = (
     "pasa_abi_version", "pasa_status_string", "pasa_derive", "pasa_workspace_size", "pasa_prep",
     "pasa_select", "pasa_attn", "pasa_forward", "pasa_forward_noalloc", "pasa_place",
@@ -48,10 +51,16 @@ EXPORTS = (
     "pasa_dit_row_norm", "pasa_dit_qkv_rope", "pasa_forward_ex", "pasa_peer_alloc", "pasa_peer_free",
     "pasa_peer_open", "pasa_peer_close", "pasa_dit_qkv_rope_scatter", "pasa_forward_scatter",
     "pasa_sample_mse_workspace_size", "pasa_sample_mse", "pasa_forward_range_workspace_size",
-    "pasa_forward_range",
+    "pasa_forward_range", "pasa_rope_axes",
 )
 
 _lib = None
+
+
+class RopeTensor(ctypes.Structure):
+    """pasa_rope_tensor"""
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("heads", c_int64), ("x_stride", c_int64 * 3),
+                ("out_stride", c_int64 * 3)]
 
 
 def load() -> ctypes.CDLL:
@@ -106,6 +115,9 @@ def load() -> ctypes.CDLL:
         "pasa_dit_row_norm": (c_int, [P, P, P, P, P, P, P, P, P, c_int64, c_int64, c_int, c_float, c_int, P]),
         "pasa_dit_qkv_rope": (c_int, [P, P, P, P, P, P, P, P, c_int64, c_int64, c_int, c_int, c_float, c_int,
                                       P, P, P]),
+        "pasa_rope_axes": (c_int, [P, POINTER(RopeTensor), c_int, c_int, c_int64, c_int64, c_int, P, c_int, c_int64,
+                                   POINTER(c_int64), POINTER(c_int64), c_int, POINTER(c_int), POINTER(c_double), c_int,
+                                   c_int]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

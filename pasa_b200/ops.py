@@ -441,3 +441,7 @@ def hunyuan_hidden_states_placement(hidden_states, hidden_states_out, best_mask_
     """Token-major -> frame-major for temporal heads (placement.py:360-387)."""
     _place(hidden_states, hidden_states_out, best_mask_idx, context_length, num_frame, frame_size, inverse=1)
     return hidden_states_out
+
+
+# operators with modules of their own
+from .rope import rope_axes  # noqa: E402,F401
