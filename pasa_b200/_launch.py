@@ -27,11 +27,11 @@ def launch(fn: str, device: torch.device, *args) -> None:
     """Calls a C entry point on ``device``'s current stream and maps its status to an exception."""
     entry = getattr(_lib.load(), fn)
     index = device.index
-    if index == torch.cuda.current_device():
-        code = entry(torch.cuda.current_stream(index).cuda_stream, *args)
+    if index == torch._C._cuda_getDevice():
+        code = entry(torch._C._cuda_getCurrentRawStream(index), *args)
     else:
         with torch.cuda.device(index):
-            code = entry(torch.cuda.current_stream(index).cuda_stream, *args)
+            code = entry(torch._C._cuda_getCurrentRawStream(index), *args)
     if code:
         _lib.check(fn, code)
 
@@ -39,7 +39,12 @@ def launch(fn: str, device: torch.device, *args) -> None:
 def wants_grad(fn: str, *tensors) -> bool:
     """Whether autograd has to see this call.  While a stream is captured that is refused: the engine may run leaves'
     accumulation on the stream of an eager graph of the same leaves, which a capture cannot contain."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            break
+    else:
         return False
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{fn}: autograd is not recorded into a CUDA graph; capture the explicit forward and "

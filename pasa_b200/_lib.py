@@ -57,12 +57,6 @@ EXPORTS = (
 _lib = None
 
 
-class RopeTensor(ctypes.Structure):
-    """pasa_rope_tensor"""
-    _fields_ = [("x", c_void_p), ("out", c_void_p), ("heads", c_int64), ("x_stride", c_int64 * 3),
-                ("out_stride", c_int64 * 3)]
-
-
 def load() -> ctypes.CDLL:
     global _lib
     if _lib is not None:
@@ -115,7 +109,7 @@ def load() -> ctypes.CDLL:
         "pasa_dit_row_norm": (c_int, [P, P, P, P, P, P, P, P, P, c_int64, c_int64, c_int, c_float, c_int, P]),
         "pasa_dit_qkv_rope": (c_int, [P, P, P, P, P, P, P, P, c_int64, c_int64, c_int, c_int, c_float, c_int,
                                       P, P, P]),
-        "pasa_rope_axes": (c_int, [P, POINTER(RopeTensor), c_int, c_int, c_int64, c_int64, c_int, P, c_int, c_int64,
+        "pasa_rope_axes": (c_int, [P, P, c_int, c_int, c_int64, c_int64, c_int, P, c_int, c_int64,
                                    POINTER(c_int64), POINTER(c_int64), c_int, POINTER(c_int), POINTER(c_double), c_int,
                                    c_int]),
     }

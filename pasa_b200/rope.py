@@ -3,7 +3,9 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Optional, Sequence, Tuple, Union
+import math
+import struct
+from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -16,74 +18,89 @@ _POS_TYPES = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float3
 _PAIRS = {"interleaved": _lib.PAIRS_INTERLEAVED, "halves": _lib.PAIRS_HALVES}
 
 
-@functools.lru_cache(maxsize=64)
-def _axes(axes: Tuple[int, ...], theta: Tuple[float, ...]):
-    """The axes' dimensions and their pairs' frequencies theta^(-2i/d) as C arrays."""
+class _Plan(NamedTuple):
+    """What a call's arguments other than its tensors come to, checked once for each set of them."""
+    axes: tuple
+    turned: int            # dimensions
+    points: Optional[int]  # of the grid
+    where: tuple           # C arguments of the grid
+    tail: tuple            # C arguments behind the positions, without the direction
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(axes, theta, pairs, grid, origin) -> _Plan:
+    axes = tuple(int(d) for d in axes)
+    theta = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(axes)
     if not 1 <= len(axes) <= 4 or any(d < 0 or d % 2 for d in axes) or not 2 <= sum(axes) <= 256:
         raise ValueError(f"axes are 1 to 4 even numbers of dimensions, 2 to 256 together, got {axes}")
-    if len(theta) != len(axes) or any(not t > 0 for t in theta):
+    if len(theta) != len(axes) or any(not 0 < t < math.inf for t in theta):
         raise ValueError("theta is one positive number, or one for each axis")
+    if pairs not in _PAIRS:
+        raise ValueError("pairs is 'interleaved' or 'halves'")
     freqs = [t ** (-2 * i / d) for d, t in zip(axes, theta) for i in range(d // 2)]
-    return (ctypes.c_int * len(axes))(*axes), (ctypes.c_double * len(freqs))(*freqs)
-
-
-def _check(name, t, like=None):
-    check_cuda(name, t, 4, _DTYPES)
-    if like is not None:
-        if t.device != like.device or t.dtype != like.dtype:
-            raise ValueError("q and k must share one dtype and device")
-        if (t.shape[0], t.shape[2], t.shape[3]) != (like.shape[0], like.shape[2], like.shape[3]):
-            raise ValueError(f"q and k may differ in heads only, got {tuple(like.shape)} and {tuple(t.shape)}")
+    where = points = None
+    if grid is not None:
+        grid = tuple(int(n) for n in grid)
+        origin = (0,) * len(axes) if origin is None else tuple(int(n) for n in origin)
+        if len(grid) != len(axes) or len(origin) != len(axes) or min(grid) < 0:
+            raise ValueError(f"grid {grid} and origin {origin} need one number for each of {len(axes)} axes")
+        points = math.prod(grid)
+        where = (None, 0, 0, (ctypes.c_int64 * len(grid))(*grid), (ctypes.c_int64 * len(grid))(*origin))
+    elif origin is not None:
+        raise ValueError("origin goes with grid")
+    tail = (len(axes), (ctypes.c_int * len(axes))(*axes), (ctypes.c_double * len(freqs))(*freqs), _PAIRS[pairs])
+    return _Plan(axes, sum(axes), points, where, tail)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.shape[3] == 1 or t.stride(3) == 1 else t.contiguous()
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
-def _apply(tensors, outs, positions, cfg):
-    axes, theta, grid, origin, pairs, inverse = cfg
-    c_axes, c_freqs = _axes(axes, theta)
+# pasa_rope_tensor, once or twice
+_TENSORS = {n: struct.Struct("=" + n * "QQ7q") for n in (1, 2)}
+
+
+def _apply(tensors, outs, positions, plan, inverse):
     first = tensors[0]
     batch, _, tokens, dim = first.shape
-    args = (_lib.RopeTensor * len(tensors))()
-    for a, x, out in zip(args, tensors, outs):
-        a.x, a.out, a.heads = x.data_ptr(), out.data_ptr(), x.shape[1]
-        a.x_stride[:] = x.stride()[:3]
-        a.out_stride[:] = out.stride()[:3]
-    if grid is not None:
-        where = (None, 0, 0, (ctypes.c_int64 * len(grid))(*grid), (ctypes.c_int64 * len(grid))(*origin))
+    fields = []
+    for x, out in zip(tensors, outs):
+        xs, os = x.stride(), out.stride()
+        fields += (x.data_ptr(), out.data_ptr(), x.shape[1], xs[0], xs[1], xs[2], os[0], os[1], os[2])
+    if positions is None:
+        where = plan.where
     else:
         where = (positions.data_ptr(), _POS_TYPES[positions.dtype],
                  positions.stride(0) if positions.dim() == 3 and batch > 1 else 0, None, None)
-    launch("pasa_rope_axes", first.device, args, len(tensors), _DTYPES[first.dtype], batch, tokens, dim, *where,
-           len(axes), c_axes, c_freqs, pairs, int(inverse))
+    launch("pasa_rope_axes", first.device, _TENSORS[len(tensors)].pack(*fields), len(tensors), _DTYPES[first.dtype],
+           batch, tokens, dim, *where, *plan.tail, inverse)
     return outs
 
 
 class _RopeAxes(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, cfg, positions, *tensors):
-        ctx.cfg = cfg
+    def forward(ctx, plan, inverse, positions, *tensors):
+        ctx.plan, ctx.inverse = plan, inverse
         ctx.save_for_backward(positions)
-        return _new(tensors, positions, cfg)
+        return _new(tensors, positions, plan, inverse)
 
     @staticmethod
     def backward(ctx, *grads):
-        cfg = ctx.cfg[:-1] + (not ctx.cfg[-1],)  # a rotation's transpose is its inverse
         given = [g for g in grads if g is not None]
-        turned = iter(_turn(given, ctx.saved_tensors[0], cfg) if given else ())
-        return (None, None, *(None if g is None else next(turned) for g in grads))
+        # a rotation's transpose is its inverse
+        turned = iter(_turn(given, ctx.saved_tensors[0], ctx.plan, not ctx.inverse) if given else ())
+        return (None, None, None, *(None if g is None else next(turned) for g in grads))
 
 
-def _new(tensors, positions, cfg):
+def _new(tensors, positions, plan, inverse):
     rows = [_rows(t) for t in tensors]
-    return tuple(_apply(rows, [torch.empty_like(t) for t in rows], positions, cfg))
+    return tuple(_apply(rows, [torch.empty_like(t) for t in rows], positions, plan, inverse))
 
 
-def _turn(tensors, positions, cfg):
+def _turn(tensors, positions, plan, inverse):
     if wants_grad("rope_axes", *tensors):
-        return _RopeAxes.apply(cfg, positions, *tensors)
-    return _new(tensors, positions, cfg)
+        return _RopeAxes.apply(plan, inverse, positions, *tensors)
+    return _new(tensors, positions, plan, inverse)
 
 
 def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, axes: Sequence[int],
@@ -105,39 +122,30 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, axes: Sequen
     Angles are formed in fp64, the rotation in fp32, and rounded once.  Returns new tensors like q and k (one tensor
     without k), or q and k themselves with ``inplace``.  Differentiable in q and k, except under stream capture.
     """
-    _check("q", q)
-    tensors = [q]
-    if k is not None:
-        _check("k", k, q)
-        tensors.append(k)
-    axes = tuple(int(d) for d in axes)
-    theta = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(axes)
-    _axes(axes, theta)
+    check_cuda("q", q, 4, _DTYPES)
+    tensors = (q,)
     batch, _, tokens, dim = q.shape
-    if sum(axes) > dim:
-        raise ValueError(f"axes {axes} take more than the {dim} dimensions of a head")
-    if pairs not in _PAIRS:
-        raise ValueError("pairs is 'interleaved' or 'halves'")
+    if k is not None:
+        check_cuda("k", k, 4, _DTYPES, q.device)
+        if k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (batch, tokens, dim):
+            raise ValueError(f"q and k may differ in heads only, got {q.dtype} {tuple(q.shape)} and {k.dtype} "
+                             f"{tuple(k.shape)}")
+        tensors = (q, k)
     if (positions is None) == (grid is None):
         raise ValueError("give either positions or grid")
+    plan = _plan(tuple(axes), tuple(theta) if isinstance(theta, (tuple, list)) else theta, pairs,
+                 None if grid is None else tuple(grid), None if origin is None else tuple(origin))
+    if plan.turned > dim:
+        raise ValueError(f"axes {plan.axes} take more than the {dim} dimensions of a head")
+    if grid is not None and plan.points != tokens:
+        raise ValueError(f"grid {tuple(grid)} has {plan.points} points for {tokens} tokens")
     if positions is not None:
-        if origin is not None:
-            raise ValueError("origin goes with grid")
         check_cuda("positions", positions, None, _POS_TYPES, q.device)
-        if tuple(positions.shape) not in ((tokens, len(axes)), (batch, tokens, len(axes))):
-            raise ValueError(f"positions must be [{tokens}, {len(axes)}] or [{batch}, {tokens}, {len(axes)}], "
-                             f"got {tuple(positions.shape)}")
+        if tuple(positions.shape) not in ((tokens, len(plan.axes)), (batch, tokens, len(plan.axes))):
+            raise ValueError(f"positions must be [{tokens}, {len(plan.axes)}] or [{batch}, {tokens}, "
+                             f"{len(plan.axes)}], got {tuple(positions.shape)}")
         positions = positions.contiguous()
-    else:
-        grid = tuple(int(n) for n in grid)
-        origin = (0,) * len(axes) if origin is None else tuple(int(n) for n in origin)
-        points = 1
-        for n in grid:
-            points *= n
-        if len(grid) != len(axes) or len(origin) != len(axes) or min(grid) < 0 or points != tokens:
-            raise ValueError(f"grid {grid} and origin {origin} need one number for each of {len(axes)} axes, and "
-                             f"{tokens} points")
-    cfg = (axes, theta, grid, origin, _PAIRS[pairs], bool(inverse))
+    inverse = bool(inverse)
     if inplace:
         if wants_grad("rope_axes", *tensors):
             raise ValueError("inplace is not differentiable")
@@ -147,7 +155,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, axes: Sequen
                                  "turned in place")
         if k is not None and k.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("q and k are the same memory: it would be turned twice")
-        _apply(tensors, tensors, positions, cfg)
+        _apply(tensors, tensors, positions, plan, inverse)
     else:
-        tensors = _turn(tensors, positions, cfg)
-    return tensors[0] if k is None else tuple(tensors)
+        tensors = _turn(tensors, positions, plan, inverse)
+    return tensors[0] if k is None else tensors

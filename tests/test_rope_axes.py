@@ -1,5 +1,6 @@
 """pasa_rope_axes on the host: what it refuses before touching the device, and calls with nothing to do."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -9,10 +10,8 @@ from pasa_b200 import _lib, ops
 
 def call(*, x=4096, out=4096, heads=2, n_tensors=1, dtype=_lib.BF16, batch=1, tokens=6, dim=16, positions=4096,
          pos_type=_lib.POS_I32, grid=None, axes=(4, 6), freqs=True, pairing=0, n_axes=None):
-    t = (_lib.RopeTensor * 2)()
-    for i in range(2):
-        t[i].x, t[i].out, t[i].heads = x, out, heads
-        t[i].x_stride[:] = t[i].out_stride[:] = (heads * tokens * dim, tokens * dim, dim)
+    strides = (heads * tokens * dim, tokens * dim, dim)
+    t = struct.pack("=QQ7q", x or 0, out or 0, heads, *strides, *strides) * 2
     n = len(axes) if n_axes is None else n_axes
     return _lib.load().pasa_rope_axes(
         None, t, n_tensors, dtype, batch, tokens, dim, positions, pos_type, 0,
