@@ -445,6 +445,56 @@ PASA_API int pasa_rope_axes(void* stream, const pasa_rope_tensor* tensors, int n
               int64_t pos_batch_stride, const int64_t* grid, const int64_t* origin, int n_axes,
               const int* axes, const double* freqs, int pairing, int inverse);
 
+/*
+ * Errors of the operators below on the current device: the bits that their
+ * kernels' bounded waits have set since the last call (PASA_DEVERR_*), written
+ * to the host word `flags` and cleared.  Synchronises the stream.
+ */
+PASA_API int pasa_operator_errors(void* stream, uint32_t* flags);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection.  Request q
+ * owns rows [rows[q], rows[q+1]) of x, y and out and the adapter slots[q] (no
+ * adapter if that is outside [0, adapters)):
+ *     h = scale[slot] * x A^T,   out = y + h B^T
+ * on its rows; out = y on rows without an adapter, those before rows[0] and
+ * behind rows[requests] among them.
+ *   x    [m, k] bf16, row stride ldx      a  [adapters, rank, k] bf16
+ *   y    [m, n] bf16, row stride ldy      b  [adapters, n, rank] bf16
+ *   out  [m, n] bf16, row stride ldo; may be y (in place), no other overlap
+ *   rows, slots  device int32 [requests + 1], [requests]; rows must not
+ *        decrease (then some rows of out are not written; nothing outside of
+ *        the tensors is read or written in any case)
+ *   scale device fp32 [adapters], or NULL for 1
+ *   h    scratch of pasa_lora_h_size bytes; what pasa_lora_update_backward
+ *        takes as h
+ * k, n and rank are multiples of 8, rank at most 128, pointers 16-byte
+ * aligned, row strides multiples of 8.  Sums are fp32, h is kept to 2^-17.
+ */
+PASA_API int pasa_lora_h_size(int64_t m, int rank, size_t* bytes);
+PASA_API int pasa_lora_update(void* stream, const void* x, int64_t ldx, const void* y, int64_t ldy,
+              const void* a, const void* b, const float* scale, int64_t m, int64_t k, int64_t n, int rank,
+              int64_t adapters, const int32_t* rows, const int32_t* slots, int64_t requests,
+              void* h, void* out, int64_t ldo);
+
+/*
+ * Its gradients from dy, the gradient of out (the gradient of y is dy):
+ *     g = scale[slot] * dy B,   dx = dx_base + g A,   da = g^T x,   db = dy^T h
+ * with the sums of da and db over all rows of each adapter, in a fixed order.
+ *   h        of the forward call (h_given 1), or scratch of the same size in
+ *            which it is computed again
+ *   dx_base  [m, k] bf16 or NULL (zero); may be dx
+ *   dx [m, k], da [adapters, rank, k], db [adapters, n, rank] bf16; each may
+ *            be NULL: not computed.  Adapters without rows get zeros.
+ */
+PASA_API int pasa_lora_backward_workspace_size(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters,
+              int64_t requests, size_t* bytes);
+PASA_API int pasa_lora_update_backward(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+              const void* a, const void* b, const float* scale, int64_t m, int64_t k, int64_t n, int rank,
+              int64_t adapters, const int32_t* rows, const int32_t* slots, int64_t requests, void* h, int h_given,
+              const void* dx_base, int64_t ldbase, void* dx, int64_t lddx, void* da, void* db,
+              void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

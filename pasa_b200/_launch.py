@@ -2,6 +2,7 @@
 current stream, and the rule for gradients under stream capture."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -34,6 +35,18 @@ def launch(fn: str, device: torch.device, *args) -> None:
             code = entry(torch._C._cuda_getCurrentRawStream(index), *args)
     if code:
         _lib.check(fn, code)
+
+
+def check_operator_errors(device=None) -> None:
+    """Raise if a kernel of ``lora_update`` or its gradient gave up a wait on ``device`` since the last call
+    (synchronises the current stream)."""
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    flags = ctypes.c_uint32(0)
+    with torch.cuda.device(index):
+        _lib.check("pasa_operator_errors", _lib.load().pasa_operator_errors(
+            torch.cuda.current_stream().cuda_stream, ctypes.byref(flags)))
+    if flags.value & _lib.DEVERR_WAIT_TIMEOUT:
+        raise RuntimeError(f"pasa_b200: a device-side barrier wait timed out (error word {flags.value:#x})")
 
 
 def wants_grad(fn: str, *tensors) -> bool:

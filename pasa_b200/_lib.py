@@ -51,7 +51,8 @@ EXPORTS = (
     "pasa_dit_row_norm", "pasa_dit_qkv_rope", "pasa_forward_ex", "pasa_peer_alloc", "pasa_peer_free",
     "pasa_peer_open", "pasa_peer_close", "pasa_dit_qkv_rope_scatter", "pasa_forward_scatter",
     "pasa_sample_mse_workspace_size", "pasa_sample_mse", "pasa_forward_range_workspace_size",
-    "pasa_forward_range", "pasa_rope_axes",
+    "pasa_forward_range", "pasa_rope_axes", "pasa_operator_errors", "pasa_lora_h_size", "pasa_lora_update",
+    "pasa_lora_backward_workspace_size", "pasa_lora_update_backward",
 )
 
 _lib = None
@@ -112,6 +113,15 @@ def load() -> ctypes.CDLL:
         "pasa_rope_axes": (c_int, [P, P, c_int, c_int, c_int64, c_int64, c_int, P, c_int, c_int64,
                                    POINTER(c_int64), POINTER(c_int64), c_int, POINTER(c_int), POINTER(c_double), c_int,
                                    c_int]),
+        "pasa_operator_errors": (c_int, [P, POINTER(c_uint32)]),
+        "pasa_lora_h_size": (c_int, [c_int64, c_int, POINTER(c_size_t)]),
+        "pasa_lora_update": (c_int, [P, P, c_int64, P, c_int64, P, P, P, c_int64, c_int64, c_int64, c_int, c_int64, P,
+                                     P, c_int64, P, P, c_int64]),
+        "pasa_lora_backward_workspace_size": (c_int, [c_int64, c_int64, c_int64, c_int, c_int64, c_int64,
+                                                      POINTER(c_size_t)]),
+        "pasa_lora_update_backward": (c_int, [P, P, c_int64, P, c_int64, P, P, P, c_int64, c_int64, c_int64, c_int,
+                                              c_int64, P, P, c_int64, P, c_int, P, c_int64, P, c_int64, P, P, P,
+                                              c_size_t]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

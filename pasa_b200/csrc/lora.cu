@@ -1,0 +1,984 @@
+// Low-rank adapters of many requests beside a shared projection.  Request q
+// owns the rows [rows[q], rows[q+1]) and the adapter slots[q] (none if outside
+// [0, adapters)); with that adapter's A [R, K], B [N, R] and scale s
+//     h = s x A^T            (down)      out = y + h B^T          (up)
+// and backwards, from dy,
+//     g = s dy B             (down)      dx  = base + g A         (up)
+//     dA = g^T x,  dB = dy^T h           (grad), summed over the adapter's rows.
+//
+// Bound: HBM.  R is at most 128, so a row of x costs 2 R operations for every
+// 2 bytes: a quarter of the tensor cores' balance at most.  The tensor cores
+// (tcgen05) are still needed: at R = 64 a step at Wan2.1-14B's size is 0.2
+// TFLOP.  The products run as three kernels, each reading its large operands
+// once: down reads x (or dy), up reads y and writes out (or dx), grad reads x
+// and dy.  h and g are R wide; passing them through memory costs R / K of the
+// traffic and lets each kernel split its own long axis: down splits K over a
+// cluster of up to 8 CTAs when there are few rows (the partial sums meet in
+// distributed shared memory, in rank order), up splits N.
+//
+// Rounding: h and g are products' operands again, and are kept as two bf16
+// terms, v = hi + lo to 2^-17 of v, each multiplied and accumulated in fp32:
+// one term would cost 2^-9.  The second term doubles the small products, which
+// are not what bounds the kernels.  Results are rounded once.
+//
+// Rows are worked on in spans: a span begins at every multiple of 128 rows and
+// at every request's first row, and ends at the next of either, so a span has
+// one adapter.  Every block finds its span from `rows` on the device (no host
+// copy; a captured graph follows new lengths).
+#include "umma.cuh"
+
+namespace pasa {
+namespace lora {
+
+constexpr int kRows = 128;          // rows of a span at most: the lanes of the accumulator
+constexpr int kThreads = 192;       // warp 0 TMA, warp 1 MMA + TMEM, warps 2-5 epilogue
+constexpr int kBox = 32;            // rows of a TMA box of x, y, out and h: a short span loads only what it has
+constexpr int kBoxBytes = kBox * 128;
+constexpr int kMaxStages = 8;
+constexpr int kMaxRank = 128;
+constexpr int kSmemTwo = 112 * 1024;  // shared memory of a block when two share an SM
+
+struct Rows {
+  const int32_t* rows;   // [requests + 1]
+  const int32_t* slots;  // [requests]
+  const float* scale;    // [adapters] or null
+  int requests, adapters;
+  int64_t m;
+};
+
+struct Span {
+  int64_t begin;
+  int count;  // 0: nothing to do
+  int slot;   // -1: no adapter
+};
+
+// Span t of aligned(m) + requests + 1: a multiple of kRows, then a request's
+// first row (and the row behind the last request).  All lanes of a warp call it.
+__device__ __forceinline__ Span find_span(const Rows& a, int64_t t, int lane) {
+  const int64_t aligned = (a.m + kRows - 1) / kRows;
+  Span s{0, 0, -1};
+  int64_t own = -1;
+  if (t < aligned) {
+    s.begin = t * kRows;
+  } else {
+    own = t - aligned;
+    s.begin = a.rows[own];
+    if (s.begin <= 0 || s.begin >= a.m || s.begin % kRows == 0) return s;
+  }
+  int before = 0;  // requests that begin at or before this row
+  for (int i = lane; i <= a.requests; i += 32) before += a.rows[i] <= s.begin ? 1 : 0;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
+  const int request = before - 1;               // -1: before the first; requests: behind the last
+  if (own >= 0 && own != request) return s;     // request `own` is empty; a later one begins here too
+  int64_t end = (s.begin / kRows + 1) * kRows;
+  if (end > a.m) end = a.m;
+  if (request < a.requests) {
+    const int64_t next = a.rows[request + 1];
+    if (next < end) end = next;
+  }
+  s.count = end > s.begin ? int(end - s.begin) : 0;
+  if (request >= 0 && request < a.requests) {
+    const int slot = a.slots[request];
+    if (slot >= 0 && slot < a.adapters) s.slot = slot;
+  }
+  return s;
+}
+
+// v = hi + lo in two bf16 terms; an infinity or NaN is hi alone.
+__device__ __forceinline__ void split2(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(v0, v1);
+  const float h0 = __uint_as_float(hi << 16), h1 = __uint_as_float(hi & 0xFFFF0000u);
+  lo = pack_bf16x2(isfinite(h0) ? v0 - h0 : 0.f, isfinite(h1) ? v1 - h1 : 0.f);
+}
+
+struct Ring {
+  int stages, stage_bytes;
+};
+
+// ---------------------------------------------------------------------------
+// down: h[rows, R] = scale * u[rows, C] w^T, w = A [R, C] (K-major) or B [C, R]
+// (MN-major, its ranks contiguous)
+// ---------------------------------------------------------------------------
+struct DownMaps {
+  CUtensorMap u, w;
+};
+struct DownArgs {
+  Rows rows;
+  Ring ring;
+  int rp;          // R rounded up to 16
+  int64_t steps;   // 64-wide steps of C
+  int split;       // CTAs of a cluster, each a share of the steps
+  __nv_bfloat16* h;  // [2][m][rp]
+  uint32_t* err;
+};
+
+__host__ __device__ constexpr int down_w_bytes(bool mn, int rp) { return mn ? ((rp + 63) / 64) * 8192 : rp * 128; }
+
+template <bool MN>
+__global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ DownMaps maps,
+                                                        const __grid_constant__ DownArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(blockIdx.x % unsigned(a.split));
+  const Span span = find_span(a.rows, blockIdx.x / unsigned(a.split), lane);
+  if (span.count == 0 || span.slot < 0) return;  // the same for the whole cluster
+
+  const uint32_t cols = a.rp <= 32 ? 32 : a.rp <= 64 ? 64 : 128;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(&done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(&tmem_slot, cols); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  dependents_may_start();  // they take TMEM too: not before this block has its own
+  const int first = int(a.steps * rank / a.split), last = int(a.steps * (rank + 1) / a.split);
+  const int w_bytes = down_w_bytes(MN, a.rp);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int boxes = (span.count + kBox - 1) / kBox;
+      int issued = 0;
+      for (int i = 0; first + i < last; ++i) {
+        const int s = i % a.ring.stages;
+        if (!mbar_wait_bounded(&empty[s], uint32_t((i / a.ring.stages) & 1) ^ 1u)) {
+          report_operator_timeout(a.err);
+          break;
+        }
+        unsigned char* st = sm + s * a.ring.stage_bytes;
+        const int32_t c0 = (first + i) * 64;
+        mbar_arrive_expect_tx(&full[s], uint32_t(boxes * kBoxBytes + w_bytes));
+        for (int b = 0; b < boxes; ++b)
+          tma_load_3d(st + b * kBoxBytes, &maps.u, &full[s], c0, int32_t(span.begin) + b * kBox, 0);
+        unsigned char* w = st + kRows * 128;
+        if (MN) {
+          for (int r = 0; r < a.rp; r += 64) tma_load_3d(w + r * 128, &maps.w, &full[s], r, c0, span.slot);
+        } else {
+          tma_load_3d(w, &maps.w, &full[s], c0, 0, span.slot);
+        }
+        issued = i + 1;
+      }
+      // the copies in flight land before the block can end
+      for (int i = issued > a.ring.stages ? issued - a.ring.stages : 0; i < issued; ++i)
+        mbar_wait_bounded(&full[i % a.ring.stages], uint32_t((i / a.ring.stages) & 1));
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_bf16(128, a.rp, false, MN);
+      for (int i = 0; first + i < last; ++i) {
+        const int s = i % a.ring.stages;
+        if (!mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1))) {
+          report_operator_timeout(a.err);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t st = smem_u32(sm + s * a.ring.stage_bytes);
+        const uint64_t ud = umma_desc_sw128(st, 16, 1024);
+        const uint64_t wd = umma_desc_sw128(st + kRows * 128, MN ? 8192 : 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ss(tmem, ud + uint64_t((kk * 32) >> 4), wd + uint64_t((kk * (MN ? 2048 : 32)) >> 4), idesc,
+                 i > 0 || kk > 0 ? 1u : 0u);
+        tc_commit(&empty[s]);
+      }
+      tc_commit(&done);
+    }
+  } else {
+    const int q = warp & 3, row = q * 32 + lane;
+    if (!mbar_wait_bounded(&done, 0)) report_operator_timeout(a.err);
+    tc_fence_after();
+    const bool live = row < span.count;
+    const float scale = a.rows.scale ? a.rows.scale[span.slot] : 1.f;
+    __nv_bfloat16* hi = a.h + (span.begin + row) * a.rp;
+    __nv_bfloat16* lo = hi + a.rows.m * a.rp;
+    float* part = reinterpret_cast<float*>(sm) + row * (a.rp + 4);  // the ring is free once `done`
+    for (int c = 0; c < a.rp; c += 16) {
+      uint32_t v[16];
+      __syncwarp();
+      tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t(c), v);
+      tmem_wait_ld();
+      if (a.split > 1) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<uint4*>(part + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      } else if (live) {
+        uint32_t h[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          split2(scale * __uint_as_float(v[2 * i]), scale * __uint_as_float(v[2 * i + 1]), h[i], l[i]);
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          *reinterpret_cast<uint4*>(hi + c + 2 * i) = make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+          *reinterpret_cast<uint4*>(lo + c + 2 * i) = make_uint4(l[i], l[i + 1], l[i + 2], l[i + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, cols);
+  if (a.split == 1) return;
+
+  // The cluster's partial sums, in rank order; each CTA sums a share of the rows.
+  __syncwarp();
+  cluster_sync_all();
+  const float scale = a.rows.scale ? a.rows.scale[span.slot] : 1.f;
+  const int quads = a.rp / 4;
+  for (int i = int(threadIdx.x) + rank * kThreads; i < span.count * quads; i += kThreads * a.split) {
+    const int row = i / quads, c = (i - row * quads) * 4;
+    const uint32_t at = smem_u32(sm) + uint32_t(row * (a.rp + 4) + c) * 4u;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < a.split; ++r) {
+      const float4 v = cluster_load4(cluster_map(at, uint32_t(r)));
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    uint32_t h[2], l[2];
+    split2(scale * sum.x, scale * sum.y, h[0], l[0]);
+    split2(scale * sum.z, scale * sum.w, h[1], l[1]);
+    __nv_bfloat16* hi = a.h + (span.begin + row) * a.rp + c;
+    *reinterpret_cast<uint2*>(hi) = make_uint2(h[0], h[1]);
+    *reinterpret_cast<uint2*>(hi + a.rows.m * a.rp) = make_uint2(l[0], l[1]);
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA ends while another reads its partial sums
+}
+
+// ---------------------------------------------------------------------------
+// up: out[rows, C] = base[rows, C] + h[rows, R] w, w^T = B [C, R] (K-major) or
+// w = A [R, C] (MN-major).  A block owns a span and a share of the 64-column
+// chunks.  The base's chunk lands in shared memory by TMA, is added to in
+// place and leaves by TMA from there (by plain stores where a box of 32 rows
+// reaches into another span).
+// ---------------------------------------------------------------------------
+constexpr int kChunk = 64;
+constexpr int kAcc = 4;  // accumulators in flight
+
+struct UpMaps {
+  CUtensorMap base, out, h, w;
+};
+struct UpArgs {
+  Rows rows;
+  Ring ring;
+  int rp;
+  int64_t chunks;  // of C
+  int split;       // blocks of a span
+  int64_t cols, ldo;
+  __nv_bfloat16* out;
+  int has_base;    // else the base is zero
+  int in_place;    // out is base: spans without an adapter are done
+  uint32_t* err;
+};
+
+__host__ __device__ constexpr int up_w_bytes(bool mn, int rp) { return mn ? rp * 128 : ((rp + 63) / 64) * 8192; }
+__host__ __device__ constexpr int up_h_bytes(int rp) { return 2 * ((rp + 63) / 64) * kRows * 128; }
+
+template <bool MN>
+__global__ void __launch_bounds__(kThreads) up_kernel(const __grid_constant__ UpMaps maps,
+                                                      const __grid_constant__ UpArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAcc], acc_empty[kAcc], h_full;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Span span = find_span(a.rows, blockIdx.x / unsigned(a.split), lane);
+  if (span.count == 0 || (span.slot < 0 && a.in_place)) return;
+  const int part = int(blockIdx.x % unsigned(a.split));
+  const int first = int(a.chunks * part / a.split), mine = int(a.chunks * (part + 1) / a.split) - first;
+  const bool adapts = span.slot >= 0;
+  const int boxes = (span.count + kBox - 1) / kBox;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
+    for (int b = 0; b < kAcc; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4); }
+    mbar_init(&h_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(&tmem_slot, kAcc * kChunk); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int atoms = (a.rp + 63) / 64;
+  unsigned char* hs = sm;                       // [hi, lo][atoms][128 rows][64]
+  unsigned char* ring = sm + up_h_bytes(a.rp);  // stage: base [128][64], then w
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int w_bytes = adapts ? up_w_bytes(MN, a.rp) : 0;
+      const int y_bytes = a.has_base ? boxes * kBoxBytes : 0;
+      auto issue = [&](int i) {
+        const int s = i % a.ring.stages;
+        unsigned char* st = ring + s * a.ring.stage_bytes;
+        const int32_t c0 = (first + i) * kChunk;
+        mbar_arrive_expect_tx(&full[s], uint32_t(y_bytes + w_bytes));
+        if (a.has_base)
+          for (int b = 0; b < boxes; ++b)
+            tma_load_3d(st + b * kBoxBytes, &maps.base, &full[s], c0, int32_t(span.begin) + b * kBox, 0);
+        if (adapts) {
+          unsigned char* w = st + kRows * 128;
+          if (MN) tma_load_3d(w, &maps.w, &full[s], c0, 0, span.slot);
+          else
+            for (int t = 0; t < atoms; ++t) tma_load_3d(w + t * 8192, &maps.w, &full[s], t * 64, c0, span.slot);
+        }
+      };
+      const int ahead = mine < a.ring.stages ? mine : a.ring.stages;
+      for (int i = 0; i < ahead; ++i) issue(i);  // these do not depend on the kernel before
+      wait_for_predecessor();
+      if (adapts) {
+        mbar_arrive_expect_tx(&h_full, uint32_t(2 * atoms * boxes * kBoxBytes));
+        for (int t = 0; t < 2; ++t)
+          for (int c = 0; c < atoms; ++c)
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d(hs + (t * atoms + c) * (kRows * 128) + b * kBoxBytes, &maps.h, &h_full, c * 64,
+                          int32_t(span.begin) + b * kBox, t);
+      }
+      int issued = ahead;
+      for (int i = ahead; i < mine; ++i) {
+        if (!mbar_wait_bounded(&empty[i % a.ring.stages], uint32_t((i / a.ring.stages) & 1) ^ 1u)) {
+          report_operator_timeout(a.err);
+          break;
+        }
+        issue(i);
+        issued = i + 1;
+      }
+      if (adapts) mbar_wait_bounded(&h_full, 0);
+      for (int i = issued > a.ring.stages ? issued - a.ring.stages : 0; i < issued; ++i)
+        mbar_wait_bounded(&full[i % a.ring.stages], uint32_t((i / a.ring.stages) & 1));
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && adapts) {
+      const uint32_t idesc = umma_idesc_bf16(128, kChunk, false, MN);
+      const uint64_t hd = umma_desc_sw128(smem_u32(hs), 16, 1024);
+      bool ok = mbar_wait_bounded(&h_full, 0);
+      for (int i = 0; i < mine && ok; ++i) {
+        const int s = i % a.ring.stages, b = i % kAcc;
+        if (!mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1)) ||
+            !mbar_wait_bounded(&acc_empty[b], uint32_t((i / kAcc) & 1) ^ 1u)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t wd =
+            umma_desc_sw128(smem_u32(ring + s * a.ring.stage_bytes + kRows * 128), MN ? 8192 : 16, 1024);
+        for (int t = 0; t < 2; ++t)
+          for (int kk = 0; kk < a.rp / 16; ++kk) {
+            const int h_off = (t * atoms + kk / 4) * (kRows * 128) + (kk % 4) * 32;
+            const int w_off = MN ? kk * 2048 : (kk / 4) * 8192 + (kk % 4) * 32;
+            mma_ss(tmem + uint32_t(b * kChunk), hd + uint64_t(h_off >> 4), wd + uint64_t(w_off >> 4), idesc,
+                   t > 0 || kk > 0 ? 1u : 0u);
+          }
+        tc_commit(&acc_full[b]);
+      }
+      if (!ok) report_operator_timeout(a.err);
+    }
+  } else {
+    const int q = warp & 3;
+    const int live = min(max(span.count - q * kBox, 0), kBox);  // this warp's rows of the span
+    wait_for_predecessor();
+    bool ok = true;
+    for (int i = 0; i < mine; ++i) {
+      const int s = i % a.ring.stages, b = i % kAcc;
+      unsigned char* box = ring + s * a.ring.stage_bytes + q * kBoxBytes;
+      if (ok) {
+        ok = mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1)) &&
+             (!adapts || mbar_wait_bounded(&acc_full[b], uint32_t((i / kAcc) & 1)));
+        if (!ok) report_operator_timeout(a.err);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (live > 0 && ok) {
+        uint32_t d[2][32];
+        if (adapts) {
+          tc_fence_after();
+          const uint32_t t = tmem + (uint32_t(q * 32) << 16) + uint32_t(b * kChunk);
+          tmem_ld32(t, d[0]);
+          tmem_ld32(t + 32, d[1]);
+          tmem_wait_ld();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0 && adapts) mbar_arrive(&acc_empty[b]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {  // the row's eight 16-byte vectors, swizzled
+          uint4* at = reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4));
+          uint4 y = a.has_base ? *at : make_uint4(0u, 0u, 0u, 0u);
+          if (adapts) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int x = (c & 3) * 8 + 2 * e;
+              w[e] = pack_bf16x2(__uint_as_float(w[e] << 16) + __uint_as_float(d[c >> 2][x]),
+                                 __uint_as_float(w[e] & 0xFFFF0000u) + __uint_as_float(d[c >> 2][x + 1]));
+            }
+          }
+          *at = y;
+        }
+        const int64_t c0 = int64_t(first + i) * kChunk, r0 = span.begin + q * kBox;
+        fence_proxy_async();  // the stage's next reader or writer is TMA
+        __syncwarp();
+        if (live == kBox) {
+          if (lane == 0) {
+            tma_store_3d(&maps.out, box, int32_t(c0), int32_t(r0), 0);
+            bulk_commit();
+          }
+        } else {  // the box's other rows are another span's
+          for (int r = lane >> 3; r < live; r += 4) {
+            const int64_t col = c0 + (lane & 7) * 8;
+            if (col < a.cols)
+              *reinterpret_cast<uint4*>(a.out + (r0 + r) * a.ldo + col) =
+                  *reinterpret_cast<uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          }
+        }
+      } else if (lane == 0 && adapts) {
+        mbar_arrive(&acc_empty[b]);
+      }
+      // free the stage whose store has left shared memory: the one before
+      __syncwarp();
+      if (lane == 0) {
+        bulk_wait_read<1>();
+        if (i > 0) mbar_arrive(&empty[(i - 1) % a.ring.stages]);
+      }
+    }
+    if (lane == 0) bulk_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kAcc * kChunk);
+}
+
+// ---------------------------------------------------------------------------
+// grad: for each adapter, d[C, R] = sum over its rows of u[row, C]^T h[row, R]:
+// dA = (x, g) and dB = (dy, h) in one launch.  A block owns 256 columns of one
+// of the two, an adapter and a share of the adapter's 64-row stages; a stage's
+// rows behind the request's last are zeroed in shared memory (they hold
+// another request's values, which may be NaN).  hi and lo sit side by side as
+// the columns of one operand, so a stage is 8 MMAs of M = 128, N = 128 (N = 256
+// above rank 64); the two halves are added at the end.  Shares of one adapter
+// are summed in order by a second kernel.
+// ---------------------------------------------------------------------------
+constexpr int kGradRows = 64;
+constexpr int kGradCols = 256;
+constexpr int kGradU = kGradRows * kGradCols * 2;
+
+struct GradMaps {
+  CUtensorMap u[2], h[2];
+};
+struct GradArgs {
+  Rows rows;
+  Ring ring;
+  int rank, atoms;
+  int problem0;           // the first problem computed (0: dA, 1: dB)
+  int64_t cols[2], blocks[2];  // columns and column blocks
+  int parts;              // shares of an adapter's rows
+  float* partial;         // [parts][adapters][rank * cols] for each problem, if parts > 1
+  __nv_bfloat16* out[2];  // [adapters][rank][cols], [adapters][cols][rank]
+  uint32_t* err;
+};
+
+__device__ __forceinline__ int request_stages(const Rows& a, int q, int slot, int64_t& begin, int64_t& end) {
+  if (q >= a.requests || a.slots[q] != slot) return 0;
+  begin = a.rows[q];
+  end = a.rows[q + 1];
+  if (begin < 0) begin = 0;
+  if (end > a.m) end = a.m;
+  return end > begin ? int((end - begin + kGradRows - 1) / kGradRows) : 0;
+}
+
+__global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ GradMaps maps,
+                                                        const __grid_constant__ GradArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int valid[kMaxStages];  // rows of a stage that are the request's
+  __shared__ int stages_total;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t id = blockIdx.x;
+  int problem = a.problem0;
+  const int64_t each = int64_t(a.parts) * a.rows.adapters;
+  if (problem == 0 && id >= a.blocks[0] * each) { id -= a.blocks[0] * each; problem = 1; }
+  const int64_t col0 = (id % a.blocks[problem]) * kGradCols;
+  id /= a.blocks[problem];
+  const int part = int(id % a.parts), slot = int(id / a.parts);
+  const int n = 128 * a.atoms;                // accumulator columns of 128 matrix columns: hi, then lo
+  const uint32_t cols = uint32_t(2 * n);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(&done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(&tmem_slot, cols); tmem_relinquish(); }
+  if (warp == 0) {
+    int total = 0;
+    int64_t begin, end;
+    for (int q = lane; q < a.rows.requests; q += 32) total += request_stages(a.rows, q, slot, begin, end);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (lane == 0) stages_total = total;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int first = int(int64_t(stages_total) * part / a.parts);
+  const int mine = int(int64_t(stages_total) * (part + 1) / a.parts) - first;
+
+  if (warp == 0) {
+    // all lanes look for the adapter's requests, lane 0 issues
+    int i = 0, base = 0;
+    bool ok = true;
+    for (int q0 = 0; q0 < a.rows.requests && i < mine && ok; q0 += 32) {
+      int64_t begin = 0, end = 0;
+      const int own = request_stages(a.rows, q0 + lane, slot, begin, end);
+      int upto = own;  // inclusive prefix sum
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += v;
+      }
+      const uint32_t some = __ballot_sync(0xffffffffu, own > 0);
+      for (uint32_t left = some; left != 0 && i < mine && ok; left &= left - 1) {
+        const int src = __ffs(int(left)) - 1;
+        const int count = __shfl_sync(0xffffffffu, own, src);
+        const int before = base + __shfl_sync(0xffffffffu, upto, src) - count;
+        const int64_t r0 = __shfl_sync(0xffffffffu, begin, src), r1 = __shfl_sync(0xffffffffu, end, src);
+        for (int t = max(0, first + i - before); t < count && i < mine && ok; ++t, ++i) {
+          const int s = i % a.ring.stages;
+          ok = mbar_wait_bounded(&empty[s], uint32_t((i / a.ring.stages) & 1) ^ 1u);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) {
+            const int64_t row = r0 + int64_t(t) * kGradRows;
+            unsigned char* st = sm + s * a.ring.stage_bytes;
+            valid[s] = int(r1 - row < kGradRows ? r1 - row : kGradRows);
+            mbar_arrive_expect_tx(&full[s], uint32_t(a.ring.stage_bytes));
+            for (int c = 0; c < kGradCols; c += 64)
+              tma_load_3d(st + c * 128, &maps.u[problem], &full[s], int32_t(col0) + c, int32_t(row), 0);
+            for (int c = 0; c < 2 * a.atoms; ++c)
+              tma_load_3d(st + kGradU + c * 8192, &maps.h[problem], &full[s], (c % a.atoms) * 64, int32_t(row),
+                          c / a.atoms);
+          }
+          __syncwarp();
+        }
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (!ok && lane == 0) report_operator_timeout(a.err);
+    for (int j = i > a.ring.stages ? i - a.ring.stages : 0; j < i; ++j)
+      mbar_wait_bounded(&full[j % a.ring.stages], uint32_t((j / a.ring.stages) & 1));
+  } else if (warp == 1) {
+    const uint32_t idesc = umma_idesc_bf16(128, n, true, true);
+    bool ok = true;
+    for (int i = 0; i < mine; ++i) {
+      const int s = i % a.ring.stages;
+      ok = mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      unsigned char* st = sm + s * a.ring.stage_bytes;
+      const int rows = valid[s];
+      if (rows < kGradRows) {  // zero the other rows of every [64 rows][64] box
+        const int per_box = (kGradRows - rows) * 8, boxes = a.ring.stage_bytes / 8192;
+        for (int j = lane; j < boxes * per_box; j += 32)
+          *reinterpret_cast<uint4*>(st + (j / per_box) * 8192 + rows * 128 + (j % per_box) * 16) =
+              make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
+        __syncwarp();
+      }
+      if (lane == 0) {
+        tc_fence_after();
+        const uint64_t ud = umma_desc_sw128(smem_u32(st), 8192, 1024);
+        const uint64_t hd = umma_desc_sw128(smem_u32(st) + kGradU, 8192, 1024);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int kk = 0; kk < kGradRows / 16; ++kk)
+            mma_ss(tmem + uint32_t(c * n), ud + uint64_t((c * 16384 + kk * 2048) >> 4),
+                   hd + uint64_t((kk * 2048) >> 4), idesc, i > 0 || kk > 0 ? 1u : 0u);
+        tc_commit(&empty[s]);
+      }
+      __syncwarp();
+    }
+    if (lane == 0) {
+      if (!ok) report_operator_timeout(a.err);
+      tc_commit(&done);
+    }
+  } else {
+    const int q = warp & 3;
+    if (!mbar_wait_bounded(&done, 0)) report_operator_timeout(a.err);
+    tc_fence_after();
+    const int64_t size = int64_t(a.rank) * a.cols[problem];
+    float* partial = a.partial + (problem == 1 && a.problem0 == 0 ? each * a.rank * a.cols[0] : 0) +
+                     (int64_t(part) * a.rows.adapters + slot) * size;
+    __nv_bfloat16* out = a.out[problem] + int64_t(slot) * size;
+    for (int c = 0; c < 2; ++c) {
+      const int64_t col = col0 + c * 128 + q * 32 + lane;
+      for (int r0 = 0; r0 < a.rank; r0 += 16) {
+        uint32_t hi[16], lo[16];
+        __syncwarp();
+        const uint32_t t = tmem + (uint32_t(q * 32) << 16) + uint32_t(c * n + r0);
+        tmem_ld16(t, hi);
+        tmem_ld16(t + uint32_t(n / 2), lo);
+        tmem_wait_ld();
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = mine > 0 ? __uint_as_float(hi[i]) + __uint_as_float(lo[i]) : 0.f;
+        if (col < a.cols[problem]) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+            if (r0 + i >= a.rank) continue;  // a multiple of 8
+            if (problem == 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int64_t at = int64_t(r0 + i + e) * a.cols[0] + col;
+                if (a.parts > 1) partial[at] = v[i + e];
+                else out[at] = __float2bfloat16_rn(v[i + e]);
+              }
+            } else {
+              const int64_t at = col * a.rank + r0 + i;
+              if (a.parts > 1) {
+                *reinterpret_cast<float4*>(partial + at) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                *reinterpret_cast<float4*>(partial + at + 4) = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
+              } else {
+                *reinterpret_cast<uint4*>(out + at) =
+                    make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
+                               pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, cols);
+}
+
+// out = bf16(sum over the parts, in order), 8 values a thread; dA's values, then dB's.
+__global__ void __launch_bounds__(256) grad_sum_kernel(const float* __restrict__ partial, int parts, int64_t size0,
+                                                       int64_t size1, __nv_bfloat16* out0, __nv_bfloat16* out1) {
+  int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
+  int64_t size = size0;
+  __nv_bfloat16* out = out0;
+  if (i >= size0) {
+    i -= size0;
+    partial += size0 * parts;
+    size = size1;
+    out = out1;
+    if (i >= size1) return;
+  }
+  float v[8] = {};
+  for (int p = 0; p < parts; ++p) {
+    const float4* src = reinterpret_cast<const float4*>(partial + p * size + i);
+    const float4 x = src[0], y = src[1];
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+    v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+  }
+  *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                  pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+// bf16 [batch][rows][cols], row stride ld; a box of 64 x box_rows, 128-byte swizzle.
+bool make_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t batch, int64_t ld,
+              int box_rows) {
+  const auto fn = tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(batch)};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(rows) * cuuint64_t(ld) * 2};
+  const cuuint32_t box[3] = {64u, cuuint32_t(box_rows), 1u};
+  const cuuint32_t step[3] = {1u, 1u, 1u};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+Ring ring_of(int stage_bytes, int room) {
+  int stages = room / stage_bytes;
+  if (stages > kMaxStages) stages = kMaxStages;
+  return Ring{stages, stage_bytes};
+}
+
+template <typename F>
+cudaError_t allow_smem(F kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+int64_t span_count(const Rows& r) { return cdiv(r.m, kRows) + r.requests + 1; }
+// spans that have rows, about: every request ends one, at most one a row
+int64_t busy_spans(const Rows& r) {
+  const int64_t most = cdiv(r.m, kRows) + (r.requests > 0 ? r.requests - 1 : 0);
+  return most < r.m ? most : r.m;
+}
+
+struct Matrix {
+  const void* p;
+  int64_t ld;
+};
+
+template <bool MN>
+cudaError_t down(cudaStream_t st, const Rows& r, Matrix u, int64_t c, const void* w, int rank, __nv_bfloat16* h,
+                 int sms, uint32_t* err) {
+  DownMaps maps;
+  DownArgs a{};
+  a.rp = int(cdiv(rank, 16)) * 16;
+  if (!make_map(&maps.u, u.p, c, r.m, 1, u.ld, kBox)) return cudaErrorInvalidValue;
+  if (!(MN ? make_map(&maps.w, w, rank, c, r.adapters, rank, 64)
+           : make_map(&maps.w, w, c, rank, r.adapters, c, a.rp)))
+    return cudaErrorInvalidValue;
+  a.rows = r;
+  a.ring = ring_of(kRows * 128 + down_w_bytes(MN, a.rp), kSmemTwo - 2048);
+  a.steps = cdiv(c, 64);
+  a.h = h;
+  a.err = err;
+  // few rows: K is split while that still adds blocks that find an SM free
+  a.split = 1;
+  while (a.split < 8 && busy_spans(r) * a.split * 2 <= 2 * sms && a.steps >= a.split * 4) a.split *= 2;
+  const int smem = a.ring.stages * a.ring.stage_bytes + 1024;
+  cudaError_t e = allow_smem(down_kernel<MN>, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(span_count(r) * a.split));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(a.split);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, down_kernel<MN>, maps, a);
+}
+
+template <bool MN>
+cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const void* w, int rank, int64_t c,
+               Matrix base, Matrix out, int sms, uint32_t* err) {
+  UpMaps maps;
+  UpArgs a{};
+  a.rp = int(cdiv(rank, 16)) * 16;
+  if (!make_map(&maps.out, out.p, c, r.m, 1, out.ld, kBox) || !make_map(&maps.h, h, a.rp, r.m, 2, a.rp, kBox))
+    return cudaErrorInvalidValue;
+  if (base.p == nullptr) maps.base = maps.out;
+  else if (!make_map(&maps.base, base.p, c, r.m, 1, base.ld, kBox)) return cudaErrorInvalidValue;
+  if (!(MN ? make_map(&maps.w, w, c, rank, r.adapters, c, a.rp)
+           : make_map(&maps.w, w, rank, c, r.adapters, rank, kChunk)))
+    return cudaErrorInvalidValue;
+  a.rows = r;
+  // up to rank 64 two blocks share an SM; above, h alone takes 64 KB and one block takes all
+  const int room = (a.rp <= 64 ? kSmemTwo : 2 * kSmemTwo) - up_h_bytes(a.rp) - 2048;
+  a.ring = ring_of(kRows * 128 + up_w_bytes(MN, a.rp), room);
+  a.chunks = cdiv(c, kChunk);
+  a.cols = c;
+  a.ldo = out.ld;
+  a.out = static_cast<__nv_bfloat16*>(const_cast<void*>(out.p));
+  a.has_base = base.p != nullptr;
+  a.in_place = base.p == out.p;
+  a.err = err;
+  // few rows: N is split until the blocks fill the SMs, two chunks a block at least
+  int64_t split = cdiv(2 * sms, busy_spans(r));
+  if (split > a.chunks / 2) split = a.chunks / 2;
+  a.split = split < 1 ? 1 : int(split);
+  const int smem = up_h_bytes(a.rp) + a.ring.stages * a.ring.stage_bytes + 1024;
+  cudaError_t e = allow_smem(up_kernel<MN>, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(span_count(r) * a.split));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, up_kernel<MN>, maps, a);
+}
+
+// Shares of an adapter's rows: enough blocks for every SM if the adapters' rows are alike.
+int grad_parts(const Rows& r, int64_t blocks, int sms) {
+  const int64_t adapters = r.adapters < r.requests ? r.adapters : r.requests;
+  int64_t parts = cdiv(2 * sms, blocks * adapters);
+  const int64_t most = cdiv(r.m, 4 * kGradRows * adapters);
+  if (parts > most) parts = most;
+  return parts < 1 ? 1 : int(parts);
+}
+
+int64_t grad_blocks(int64_t c) { return cdiv(c, kGradCols); }
+
+cudaError_t grad(cudaStream_t st, const Rows& r, int rank, Matrix x, int64_t k, Matrix dy, int64_t n,
+                 const __nv_bfloat16* g, const __nv_bfloat16* h, void* da, void* db, void* workspace, int sms,
+                 uint32_t* err) {
+  GradMaps maps;
+  GradArgs a{};
+  const int rp = int(cdiv(rank, 16)) * 16;
+  if (!make_map(&maps.u[0], x.p, k, r.m, 1, x.ld, kGradRows) || !make_map(&maps.u[1], dy.p, n, r.m, 1, dy.ld, kGradRows) ||
+      !make_map(&maps.h[0], g, rp, r.m, 2, rp, kGradRows) || !make_map(&maps.h[1], h, rp, r.m, 2, rp, kGradRows))
+    return cudaErrorInvalidValue;
+  a.rows = r;
+  a.rank = rank;
+  a.atoms = rp <= 64 ? 1 : 2;
+  a.ring = ring_of(kGradU + 2 * a.atoms * 8192, 2 * kSmemTwo - 4096);
+  a.problem0 = da ? 0 : 1;
+  a.cols[0] = k;
+  a.cols[1] = n;
+  a.blocks[0] = grad_blocks(k);
+  a.blocks[1] = grad_blocks(n);
+  const int64_t blocks = (da ? a.blocks[0] : 0) + (db ? a.blocks[1] : 0);
+  a.parts = grad_parts(r, grad_blocks(k) + grad_blocks(n), sms);
+  a.partial = static_cast<float*>(workspace);
+  a.out[0] = static_cast<__nv_bfloat16*>(da);
+  a.out[1] = static_cast<__nv_bfloat16*>(db);
+  a.err = err;
+  const int smem = a.ring.stages * a.ring.stage_bytes + 1024;
+  cudaError_t e = allow_smem(grad_kernel, smem);
+  if (e != cudaSuccess) return e;
+  grad_kernel<<<unsigned(blocks * a.parts * r.adapters), kThreads, smem, st>>>(maps, a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || a.parts == 1) return e;
+  const int64_t size0 = da ? r.adapters * rank * k : 0, size1 = db ? r.adapters * rank * n : 0;
+  grad_sum_kernel<<<unsigned(cdiv((size0 + size1) / 8, 256)), 256, 0, st>>>(a.partial, a.parts, size0, size1,
+                                                                          a.out[0], a.out[1]);
+  return cudaGetLastError();
+}
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+int check(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int64_t requests) {
+  if (m < 0 || k < 1 || n < 1 || adapters < 1 || requests < 0) return PASA_ERR_SHAPE;
+  if (k % 8 || n % 8 || rank < 8 || rank > kMaxRank || rank % 8) return PASA_ERR_SHAPE;
+  if (m > (int64_t(1) << 30) || k > (1 << 24) || n > (1 << 24) || adapters > (1 << 20) || requests > (1 << 20))
+    return PASA_ERR_SHAPE;
+  return PASA_OK;
+}
+
+int check_matrix(const void* p, int64_t ld, int64_t cols) {
+  if (!p) return PASA_ERR_NULL;
+  if (misaligned(p)) return PASA_ERR_ALIGN;
+  return ld < cols || ld % 8 || ld > (int64_t(1) << 32) ? PASA_ERR_SHAPE : PASA_OK;
+}
+
+int device_sms(int* sms) {
+  int dev = 0, major = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return PASA_ERR_CUDA;
+  return major == 10 ? PASA_OK : PASA_ERR_DEVICE;
+}
+
+}  // namespace lora
+}  // namespace pasa
+
+using namespace pasa;
+
+extern "C" {
+
+int pasa_lora_h_size(int64_t m, int rank, size_t* bytes) {
+  if (!bytes) return PASA_ERR_NULL;
+  const int st = lora::check(m, 8, 8, rank, 1, 0);
+  if (st) return st;
+  *bytes = size_t(2 * m) * size_t(cdiv(rank, 16) * 16) * 2;
+  return PASA_OK;
+}
+
+int pasa_lora_update(void* stream, const void* x, int64_t ldx, const void* y, int64_t ldy, const void* a,
+                     const void* b, const float* scale, int64_t m, int64_t k, int64_t n, int rank, int64_t adapters,
+                     const int32_t* rows, const int32_t* slots, int64_t requests, void* h, void* out, int64_t ldo) {
+  using namespace pasa::lora;
+  int st = check(m, k, n, rank, adapters, requests);
+  if (st || m == 0) return st;
+  if ((st = check_matrix(x, ldx, k)) || (st = check_matrix(y, ldy, n)) || (st = check_matrix(out, ldo, n))) return st;
+  if (!a || !b || !rows || !h || (requests && !slots)) return PASA_ERR_NULL;
+  if (misaligned(a) || misaligned(b) || misaligned(h)) return PASA_ERR_ALIGN;
+  if (out == y && ldo != ldy) return PASA_ERR_SHAPE;
+  int sms = 0;
+  if ((st = device_sms(&sms))) return st;
+  uint32_t* err = operator_error_word();
+  if (!err) return PASA_ERR_CUDA;
+  const Rows r{rows, slots, scale, int(requests), int(adapters), m};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  __nv_bfloat16* hh = static_cast<__nv_bfloat16*>(h);
+  cudaError_t e = down<false>(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
+  if (e == cudaSuccess) e = up<false>(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo}, sms, err);
+  return e == cudaSuccess ? PASA_OK : PASA_ERR_CUDA;
+}
+
+int pasa_lora_backward_workspace_size(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int64_t requests,
+                                      size_t* bytes) {
+  using namespace pasa::lora;
+  if (!bytes) return PASA_ERR_NULL;
+  int st = check(m, k, n, rank, adapters, requests);
+  if (st) return st;
+  int sms = 0;
+  if ((st = device_sms(&sms))) return st;
+  size_t h = 0;
+  pasa_lora_h_size(m, rank, &h);
+  const Rows r{nullptr, nullptr, nullptr, int(requests), int(adapters), m};
+  const int parts = m && requests ? grad_parts(r, grad_blocks(k) + grad_blocks(n), sms) : 1;
+  const size_t partial = parts > 1 ? size_t(parts) * size_t(adapters) * size_t(rank) * size_t(k + n) * 4 : 0;
+  *bytes = align256(h) + partial;
+  return PASA_OK;
+}
+
+int pasa_lora_update_backward(void* stream, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* a,
+                              const void* b, const float* scale, int64_t m, int64_t k, int64_t n, int rank,
+                              int64_t adapters, const int32_t* rows, const int32_t* slots, int64_t requests, void* h,
+                              int h_given, const void* dx_base, int64_t ldbase, void* dx, int64_t lddx, void* da,
+                              void* db, void* workspace, size_t workspace_bytes) {
+  using namespace pasa::lora;
+  int st = check(m, k, n, rank, adapters, requests);
+  if (st) return st;
+  if (m && ((st = check_matrix(dy, lddy, n)) || (st = check_matrix(x, ldx, k)) ||
+            (dx && (st = check_matrix(dx, lddx, k))) || (dx && dx_base && (st = check_matrix(dx_base, ldbase, k)))))
+    return st;
+  if (!a || !b || !rows || (requests && !slots) || (m && db && !h)) return PASA_ERR_NULL;
+  if (misaligned(a) || misaligned(b) || misaligned(h) || misaligned(da) || misaligned(db)) return PASA_ERR_ALIGN;
+  if (dx && dx == dx_base && lddx != ldbase) return PASA_ERR_SHAPE;
+  size_t need = 0;
+  if ((st = pasa_lora_backward_workspace_size(m, k, n, rank, adapters, requests, &need))) return st;
+  if (need && (!workspace || workspace_bytes < need)) return PASA_ERR_WORKSPACE;
+  if (misaligned(workspace)) return PASA_ERR_ALIGN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (m == 0 || requests == 0) {  // no row has an adapter
+    const size_t grad_bytes = size_t(adapters) * size_t(rank) * 2;
+    if (da && cudaMemsetAsync(da, 0, grad_bytes * size_t(k), s) != cudaSuccess) return PASA_ERR_CUDA;
+    if (db && cudaMemsetAsync(db, 0, grad_bytes * size_t(n), s) != cudaSuccess) return PASA_ERR_CUDA;
+    if (m == 0 || !dx) return PASA_OK;
+  }
+  int sms = 0;
+  if ((st = device_sms(&sms))) return st;
+  uint32_t* err = operator_error_word();
+  if (!err) return PASA_ERR_CUDA;
+  const Rows r{rows, slots, scale, int(requests), int(adapters), m};
+  __nv_bfloat16* g = static_cast<__nv_bfloat16*>(workspace);
+  __nv_bfloat16* hh = static_cast<__nv_bfloat16*>(h);
+  size_t h_bytes = 0;
+  pasa_lora_h_size(m, rank, &h_bytes);
+  cudaError_t e = cudaSuccess;
+  if (db && !h_given && requests) e = down<false>(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
+  if (e == cudaSuccess && (dx || da)) e = down<true>(s, r, Matrix{dy, lddy}, n, b, rank, g, sms, err);
+  if (e == cudaSuccess && dx)
+    e = up<true>(s, r, g, a, rank, k, Matrix{dx_base, ldbase}, Matrix{dx, lddx}, sms, err);
+  if (e == cudaSuccess && (da || db) && requests)
+    e = grad(s, r, rank, Matrix{x, ldx}, k, Matrix{dy, lddy}, n, g, hh, da, db,
+             static_cast<unsigned char*>(workspace) + align256(h_bytes), sms, err);
+  return e == cudaSuccess ? PASA_OK : PASA_ERR_CUDA;
+}
+
+}  // extern "C"
