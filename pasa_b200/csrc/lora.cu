@@ -52,35 +52,46 @@ struct Span {
   int slot;   // -1: no adapter
 };
 
-// Span t of aligned(m) + requests + 1: a multiple of kRows, then a request's
-// first row (and the row behind the last request).  All lanes of a warp call it.
+// Span t, in the order of the rows; count 0 behind the last one.  Segment 0 is
+// the rows before the first request, then the requests, then the rows behind
+// the last; each lane of the warp takes a segment's bounds and a prefix sum over
+// their spans finds the one with span t.  All lanes of a warp call it.
 __device__ __forceinline__ Span find_span(const Rows& a, int64_t t, int lane) {
-  const int64_t aligned = (a.m + kRows - 1) / kRows;
   Span s{0, 0, -1};
-  int64_t own = -1;
-  if (t < aligned) {
-    s.begin = t * kRows;
-  } else {
-    own = t - aligned;
-    s.begin = a.rows[own];
-    if (s.begin <= 0 || s.begin >= a.m || s.begin % kRows == 0) return s;
-  }
-  int before = 0;  // requests that begin at or before this row
-  for (int i = lane; i <= a.requests; i += 32) before += a.rows[i] <= s.begin ? 1 : 0;
+  for (int first = 0; first <= a.requests + 1; first += 32) {
+    const int segment = first + lane;
+    int64_t begin = 0, end = 0;
+    if (segment <= a.requests + 1) {
+      begin = segment == 0 ? 0 : a.rows[segment - 1];
+      end = segment <= a.requests ? a.rows[segment] : a.m;
+      if (begin < 0) begin = 0;
+      if (end > a.m) end = a.m;
+    }
+    const int64_t own = end > begin ? (end - 1) / kRows - begin / kRows + 1 : 0;
+    int64_t upto = own;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
-  const int request = before - 1;               // -1: before the first; requests: behind the last
-  if (own >= 0 && own != request) return s;     // request `own` is empty; a later one begins here too
-  int64_t end = (s.begin / kRows + 1) * kRows;
-  if (end > a.m) end = a.m;
-  if (request < a.requests) {
-    const int64_t next = a.rows[request + 1];
-    if (next < end) end = next;
-  }
-  s.count = end > s.begin ? int(end - s.begin) : 0;
-  if (request >= 0 && request < a.requests) {
-    const int slot = a.slots[request];
-    if (slot >= 0 && slot < a.adapters) s.slot = slot;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += v;
+    }
+    const uint32_t reached = __ballot_sync(0xffffffffu, upto > t);
+    if (reached == 0) {
+      t -= __shfl_sync(0xffffffffu, upto, 31);
+      continue;
+    }
+    const int src = __ffs(int(reached)) - 1;
+    t -= __shfl_sync(0xffffffffu, upto - own, src);
+    begin = __shfl_sync(0xffffffffu, begin, src);
+    end = __shfl_sync(0xffffffffu, end, src);
+    s.begin = t == 0 ? begin : (begin / kRows + t) * kRows;
+    const int64_t next = (s.begin / kRows + 1) * kRows;
+    s.count = int((next < end ? next : end) - s.begin);
+    const int request = first + src - 1;
+    if (request >= 0 && request < a.requests) {
+      const int slot = a.slots[request];
+      if (slot >= 0 && slot < a.adapters) s.slot = slot;
+    }
+    return s;
   }
   return s;
 }
@@ -92,9 +103,16 @@ __device__ __forceinline__ void split2(float v0, float v1, uint32_t& hi, uint32_
   lo = pack_bf16x2(isfinite(h0) ? v0 - h0 : 0.f, isfinite(h1) ? v1 - h1 : 0.f);
 }
 
+// Shared memory is carved up by the block itself: a short span needs fewer
+// bytes a stage and gets more stages, which is what a span of few rows, bound
+// by the latency of reading weights, needs.
 struct Ring {
   int stages, stage_bytes;
 };
+__device__ __forceinline__ Ring ring_in(int room, int stage_bytes) {
+  const int stages = room / stage_bytes;
+  return Ring{stages < kMaxStages ? stages : kMaxStages, stage_bytes};
+}
 
 // ---------------------------------------------------------------------------
 // down: h[rows, R] = scale * u[rows, C] w^T, w = A [R, C] (K-major) or B [C, R]
@@ -105,7 +123,7 @@ struct DownMaps {
 };
 struct DownArgs {
   Rows rows;
-  Ring ring;
+  int room;        // bytes of shared memory for the ring
   int rp;          // R rounded up to 16
   int64_t steps;   // 64-wide steps of C
   int split;       // CTAs of a cluster, each a share of the steps
@@ -129,8 +147,14 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
   if (span.count == 0 || span.slot < 0) return;  // the same for the whole cluster
 
   const uint32_t cols = a.rp <= 32 ? 32 : a.rp <= 64 ? 64 : 128;
+  const int boxes = (span.count + kBox - 1) / kBox;
+  const int w_bytes = down_w_bytes(MN, a.rp), u_bytes = boxes * kBoxBytes;
+  // (every MMA reads 128 rows: where a span has fewer boxes the others' rows
+  // are the weights and stages behind them, and only make rows that are not kept;
+  // the last stage is followed by the rest of a full tile)
+  const Ring ring = ring_in(a.room - (kRows * 128 - u_bytes), u_bytes + w_bytes);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(&done, 1);
     fence_barrier_init();
   }
@@ -141,24 +165,22 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
   const uint32_t tmem = tmem_slot;
   dependents_may_start();  // they take TMEM too: not before this block has its own
   const int first = int(a.steps * rank / a.split), last = int(a.steps * (rank + 1) / a.split);
-  const int w_bytes = down_w_bytes(MN, a.rp);
 
   if (warp == 0) {
     if (lane == 0) {
-      const int boxes = (span.count + kBox - 1) / kBox;
       int issued = 0;
       for (int i = 0; first + i < last; ++i) {
-        const int s = i % a.ring.stages;
-        if (!mbar_wait_bounded(&empty[s], uint32_t((i / a.ring.stages) & 1) ^ 1u)) {
+        const int s = i % ring.stages;
+        if (!mbar_wait_bounded(&empty[s], uint32_t((i / ring.stages) & 1) ^ 1u)) {
           report_operator_timeout(a.err);
           break;
         }
-        unsigned char* st = sm + s * a.ring.stage_bytes;
+        unsigned char* st = sm + s * ring.stage_bytes;
         const int32_t c0 = (first + i) * 64;
-        mbar_arrive_expect_tx(&full[s], uint32_t(boxes * kBoxBytes + w_bytes));
+        mbar_arrive_expect_tx(&full[s], uint32_t(u_bytes + w_bytes));
         for (int b = 0; b < boxes; ++b)
           tma_load_3d(st + b * kBoxBytes, &maps.u, &full[s], c0, int32_t(span.begin) + b * kBox, 0);
-        unsigned char* w = st + kRows * 128;
+        unsigned char* w = st + u_bytes;
         if (MN) {
           for (int r = 0; r < a.rp; r += 64) tma_load_3d(w + r * 128, &maps.w, &full[s], r, c0, span.slot);
         } else {
@@ -167,22 +189,22 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
         issued = i + 1;
       }
       // the copies in flight land before the block can end
-      for (int i = issued > a.ring.stages ? issued - a.ring.stages : 0; i < issued; ++i)
-        mbar_wait_bounded(&full[i % a.ring.stages], uint32_t((i / a.ring.stages) & 1));
+      for (int i = issued > ring.stages ? issued - ring.stages : 0; i < issued; ++i)
+        mbar_wait_bounded(&full[i % ring.stages], uint32_t((i / ring.stages) & 1));
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = umma_idesc_bf16(128, a.rp, false, MN);
       for (int i = 0; first + i < last; ++i) {
-        const int s = i % a.ring.stages;
-        if (!mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1))) {
+        const int s = i % ring.stages;
+        if (!mbar_wait_bounded(&full[s], uint32_t((i / ring.stages) & 1))) {
           report_operator_timeout(a.err);
           break;
         }
         tc_fence_after();
-        const uint32_t st = smem_u32(sm + s * a.ring.stage_bytes);
+        const uint32_t st = smem_u32(sm + s * ring.stage_bytes);
         const uint64_t ud = umma_desc_sw128(st, 16, 1024);
-        const uint64_t wd = umma_desc_sw128(st + kRows * 128, MN ? 8192 : 16, 1024);
+        const uint64_t wd = umma_desc_sw128(st + u_bytes, MN ? 8192 : 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           mma_ss(tmem, ud + uint64_t((kk * 32) >> 4), wd + uint64_t((kk * (MN ? 2048 : 32)) >> 4), idesc,
@@ -254,24 +276,36 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
 
 // ---------------------------------------------------------------------------
 // up: out[rows, C] = base[rows, C] + h[rows, R] w, w^T = B [C, R] (K-major) or
-// w = A [R, C] (MN-major).  A block owns a span and a share of the 64-column
-// chunks.  The base's chunk lands in shared memory by TMA, is added to in
-// place and leaves by TMA from there (by plain stores where a box of 32 rows
-// reaches into another span).
+// w = A [R, C] (MN-major).  A unit of work is a span and a share of its
+// 64-column chunks; two blocks an SM go through their units, and their loads
+// run ahead into the next unit.  h (hi and lo) lies in TMEM as the products'
+// first operand.  The base's chunk lands in shared memory by TMA, is added to
+// in place and leaves by TMA from there (by plain stores where a box of 32 rows
+// reaches into another span); each of the four epilogue warps owns a box of 32
+// rows and waits for no other.  The base and the weights have rings of their
+// own: the weights' is freed by the product, the base's only when its store has
+// left.  A chunk's way from TMEM through shared memory is 1000 to 2000 clocks
+// of latency; the SM's second block fills them.  (One block an SM with two sets
+// of epilogue warps in turn needs both sets to see every phase of both rings,
+// and was slower: 61 against 51 us for 24 single rows.)
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 64;
-constexpr int kAcc = 4;  // accumulators in flight
+constexpr int kMaxAcc = 3;          // accumulators in flight
+constexpr int kUpThreads = 224;     // warp 0 base, 1 MMA + TMEM, 2 weights, 3-6 epilogue
+constexpr int kUpEpi = 4;
+constexpr uint32_t kUpTmem = 256;   // accumulators from column 0; h (hi, then lo, rp / 2 each) at the end
 
 struct UpMaps {
-  CUtensorMap base, out, h, w;
+  CUtensorMap base, out, w;
 };
 struct UpArgs {
   Rows rows;
-  Ring ring;
+  int room;        // bytes of shared memory for the rings
   int rp;
   int64_t chunks;  // of C
-  int split;       // blocks of a span
+  int split;       // units of a span
   int64_t cols, ldo;
+  const __nv_bfloat16* h;  // [2][m][rp]
   __nv_bfloat16* out;
   int has_base;    // else the base is zero
   int in_place;    // out is base: spans without an adapter are done
@@ -279,173 +313,256 @@ struct UpArgs {
 };
 
 __host__ __device__ constexpr int up_w_bytes(bool mn, int rp) { return mn ? rp * 128 : ((rp + 63) / 64) * 8192; }
-__host__ __device__ constexpr int up_h_bytes(int rp) { return 2 * ((rp + 63) / 64) * kRows * 128; }
+
+struct Unit {
+  Span span;
+  int first, chunks;
+  bool adapts;
+  int live_boxes;
+};
+
+__device__ __forceinline__ Unit find_unit(const UpArgs& a, int64_t id, int lane) {
+  Unit u;
+  u.span = find_span(a.rows, id / a.split, lane);
+  const int part = int(id % a.split);
+  u.first = int(a.chunks * part / a.split);
+  u.chunks = int(a.chunks * (part + 1) / a.split) - u.first;
+  u.adapts = u.span.slot >= 0;
+  u.live_boxes = (u.span.count + kBox - 1) / kBox;
+  if (!u.adapts && a.in_place) u.chunks = 0;
+  return u;
+}
+
+// A place in a ring and the parity of the phase that comes next there.
+struct Cursor {
+  int at;
+  uint32_t parity;
+  __device__ __forceinline__ void next(int slots) {
+    if (++at == slots) { at = 0; parity ^= 1u; }
+  }
+};
 
 template <bool MN>
-__global__ void __launch_bounds__(kThreads) up_kernel(const __grid_constant__ UpMaps maps,
-                                                      const __grid_constant__ UpArgs a) {
+__global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant__ UpMaps maps,
+                                                           const __grid_constant__ UpArgs a) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAcc], acc_empty[kAcc], h_full;
+  __shared__ uint64_t y_full[kMaxStages], y_empty[kMaxStages], w_full[kMaxStages], w_empty[kMaxStages];
+  __shared__ uint64_t acc_full[kMaxAcc], acc_empty[kMaxAcc], h_full;
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Span span = find_span(a.rows, blockIdx.x / unsigned(a.split), lane);
-  if (span.count == 0 || (span.slot < 0 && a.in_place)) return;
-  const int part = int(blockIdx.x % unsigned(a.split));
-  const int first = int(a.chunks * part / a.split), mine = int(a.chunks * (part + 1) / a.split) - first;
-  const bool adapts = span.slot >= 0;
-  const int boxes = (span.count + kBox - 1) / kBox;
+  // a slot of the base's ring holds a full span's chunk: boxes of 32 rows
+  const int box_rows = a.rows.m >= kRows ? kRows / kBox : int((a.rows.m + kBox - 1) / kBox);
+  const int y_bytes = box_rows * kBoxBytes, w_bytes = up_w_bytes(MN, a.rp);
+  // three base chunks to two of the weights' at the most
+  const int n_w = min(kMaxStages, a.room / (w_bytes + y_bytes + y_bytes / 2));
+  const int n_y = min(kMaxStages, (a.room - n_w * w_bytes) / y_bytes);
+  const int n_acc = a.rp <= 64 ? 3 : 2;
+  unsigned char* ys = sm + n_w * w_bytes;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
-    for (int b = 0; b < kAcc; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4); }
-    mbar_init(&h_full, 1);
+    for (int s = 0; s < n_y; ++s) { mbar_init(&y_full[s], 1); mbar_init(&y_empty[s], kUpEpi); }
+    for (int s = 0; s < n_w; ++s) { mbar_init(&w_full[s], 1); mbar_init(&w_empty[s], 1); }
+    for (int b = 0; b < n_acc; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], kUpEpi); }
+    mbar_init(&h_full, kUpEpi);
     fence_barrier_init();
   }
-  if (warp == 1) { tmem_alloc(&tmem_slot, kAcc * kChunk); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc(&tmem_slot, kUpTmem); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  const int atoms = (a.rp + 63) / 64;
-  unsigned char* hs = sm;                       // [hi, lo][atoms][128 rows][64]
-  unsigned char* ring = sm + up_h_bytes(a.rp);  // stage: base [128][64], then w
+  const uint32_t tmem = tmem_slot, h_tmem = tmem + kUpTmem - uint32_t(a.rp);
 
-  if (warp == 0) {
-    if (lane == 0) {
-      const int w_bytes = adapts ? up_w_bytes(MN, a.rp) : 0;
-      const int y_bytes = a.has_base ? boxes * kBoxBytes : 0;
-      auto issue = [&](int i) {
-        const int s = i % a.ring.stages;
-        unsigned char* st = ring + s * a.ring.stage_bytes;
-        const int32_t c0 = (first + i) * kChunk;
-        mbar_arrive_expect_tx(&full[s], uint32_t(y_bytes + w_bytes));
-        if (a.has_base)
-          for (int b = 0; b < boxes; ++b)
-            tma_load_3d(st + b * kBoxBytes, &maps.base, &full[s], c0, int32_t(span.begin) + b * kBox, 0);
-        if (adapts) {
-          unsigned char* w = st + kRows * 128;
-          if (MN) tma_load_3d(w, &maps.w, &full[s], c0, 0, span.slot);
-          else
-            for (int t = 0; t < atoms; ++t) tma_load_3d(w + t * 8192, &maps.w, &full[s], t * 64, c0, span.slot);
-        }
-      };
-      const int ahead = mine < a.ring.stages ? mine : a.ring.stages;
-      for (int i = 0; i < ahead; ++i) issue(i);  // these do not depend on the kernel before
-      wait_for_predecessor();
-      if (adapts) {
-        mbar_arrive_expect_tx(&h_full, uint32_t(2 * atoms * boxes * kBoxBytes));
-        for (int t = 0; t < 2; ++t)
-          for (int c = 0; c < atoms; ++c)
-            for (int b = 0; b < boxes; ++b)
-              tma_load_3d(hs + (t * atoms + c) * (kRows * 128) + b * kBoxBytes, &maps.h, &h_full, c * 64,
-                          int32_t(span.begin) + b * kBox, t);
-      }
-      int issued = ahead;
-      for (int i = ahead; i < mine; ++i) {
-        if (!mbar_wait_bounded(&empty[i % a.ring.stages], uint32_t((i / a.ring.stages) & 1) ^ 1u)) {
-          report_operator_timeout(a.err);
-          break;
-        }
-        issue(i);
-        issued = i + 1;
-      }
-      if (adapts) mbar_wait_bounded(&h_full, 0);
-      for (int i = issued > a.ring.stages ? issued - a.ring.stages : 0; i < issued; ++i)
-        mbar_wait_bounded(&full[i % a.ring.stages], uint32_t((i / a.ring.stages) & 1));
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && adapts) {
-      const uint32_t idesc = umma_idesc_bf16(128, kChunk, false, MN);
-      const uint64_t hd = umma_desc_sw128(smem_u32(hs), 16, 1024);
-      bool ok = mbar_wait_bounded(&h_full, 0);
-      for (int i = 0; i < mine && ok; ++i) {
-        const int s = i % a.ring.stages, b = i % kAcc;
-        if (!mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1)) ||
-            !mbar_wait_bounded(&acc_empty[b], uint32_t((i / kAcc) & 1) ^ 1u)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint64_t wd =
-            umma_desc_sw128(smem_u32(ring + s * a.ring.stage_bytes + kRows * 128), MN ? 8192 : 16, 1024);
-        for (int t = 0; t < 2; ++t)
-          for (int kk = 0; kk < a.rp / 16; ++kk) {
-            const int h_off = (t * atoms + kk / 4) * (kRows * 128) + (kk % 4) * 32;
-            const int w_off = MN ? kk * 2048 : (kk / 4) * 8192 + (kk % 4) * 32;
-            mma_ss(tmem + uint32_t(b * kChunk), hd + uint64_t(h_off >> 4), wd + uint64_t(w_off >> 4), idesc,
-                   t > 0 || kk > 0 ? 1u : 0u);
+  if (warp == 0 || warp == 2) {
+    // the base and the weights do not depend on the kernel before
+    const bool weights = warp == 2;
+    uint64_t* full = weights ? w_full : y_full;
+    uint64_t* empty = weights ? w_empty : y_empty;
+    const int slots = weights ? n_w : n_y;
+    Cursor c{0, 1};
+    int64_t issued = 0;
+    bool ok = true;
+    for (int64_t id = blockIdx.x; ok; id += gridDim.x) {
+      const Unit u = find_unit(a, id, lane);
+      if (u.span.count == 0) break;
+      if (weights ? !u.adapts : !a.has_base) continue;
+      if (lane == 0) {
+        for (int i = 0; i < u.chunks; ++i) {
+          if (!mbar_wait_bounded(&empty[c.at], c.parity)) {
+            report_operator_timeout(a.err);
+            ok = false;
+            break;
           }
-        tc_commit(&acc_full[b]);
+          const int32_t c0 = (u.first + i) * kChunk;
+          if (weights) {
+            unsigned char* w = sm + c.at * w_bytes;
+            mbar_arrive_expect_tx(&full[c.at], uint32_t(w_bytes));
+            if (MN) {
+              tma_load_3d(w, &maps.w, &full[c.at], c0, 0, u.span.slot);
+            } else {
+              for (int r = 0; r < a.rp; r += 64) tma_load_3d(w + r * 128, &maps.w, &full[c.at], r, c0, u.span.slot);
+            }
+          } else {
+            mbar_arrive_expect_tx(&full[c.at], uint32_t(u.live_boxes * kBoxBytes));
+            for (int b = 0; b < u.live_boxes; ++b)
+              tma_load_3d(ys + c.at * y_bytes + b * kBoxBytes, &maps.base, &full[c.at], c0,
+                          int32_t(u.span.begin) + b * kBox, 0);
+          }
+          ++issued;
+          c.next(slots);
+        }
       }
-      if (!ok) report_operator_timeout(a.err);
+      ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+    }
+    if (lane == 0)  // the copies in flight land before the block can end
+      for (int64_t i = issued > slots ? issued - slots : 0; i < issued; ++i)
+        mbar_wait_bounded(&full[i % slots], uint32_t((i / slots) & 1));
+  } else if (warp == 1) {
+    const uint32_t idesc = umma_idesc_bf16(128, kChunk, false, MN);
+    Cursor w{0, 0}, c{0, 1};
+    uint32_t h_parity = 0;
+    bool ok = true;
+    for (int64_t id = blockIdx.x; ok; id += gridDim.x) {
+      const Unit u = find_unit(a, id, lane);
+      if (u.span.count == 0) break;
+      if (!u.adapts) continue;
+      if (elect_one()) {
+        ok = mbar_wait_bounded(&h_full, h_parity);
+        for (int i = 0; i < u.chunks && ok; ++i) {
+          if (!mbar_wait_bounded(&w_full[w.at], w.parity) || !mbar_wait_bounded(&acc_empty[c.at], c.parity)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t wd =
+              umma_desc_sw128(smem_u32(sm + w.at * w_bytes), MN ? 8192 : 16, 1024);
+          for (int t = 0; t < 2; ++t)
+            for (int kk = 0; kk < a.rp / 16; ++kk) {
+              const int w_off = MN ? kk * 2048 : (kk / 4) * 8192 + (kk % 4) * 32;
+              mma_ts(tmem + uint32_t(c.at * kChunk), h_tmem + uint32_t(t * (a.rp / 2) + kk * 8),
+                     wd + uint64_t(w_off >> 4), idesc, t > 0 || kk > 0 ? 1u : 0u);
+            }
+          tc_commit(&w_empty[w.at]);
+          tc_commit(&acc_full[c.at]);
+          w.next(n_w);
+          c.next(n_acc);
+        }
+        if (!ok) report_operator_timeout(a.err);
+      }
+      h_parity ^= 1u;
+      ok = __all_sync(0xffffffffu, ok);  // the elected lane's, the others' is true
     }
   } else {
     const int q = warp & 3;
-    const int live = min(max(span.count - q * kBox, 0), kBox);  // this warp's rows of the span
+    const uint32_t lanes = uint32_t(q * 32) << 16;
     wait_for_predecessor();
     bool ok = true;
-    for (int i = 0; i < mine; ++i) {
-      const int s = i % a.ring.stages, b = i % kAcc;
-      unsigned char* box = ring + s * a.ring.stage_bytes + q * kBoxBytes;
-      if (ok) {
-        ok = mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1)) &&
-             (!adapts || mbar_wait_bounded(&acc_full[b], uint32_t((i / kAcc) & 1)));
-        if (!ok) report_operator_timeout(a.err);
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (live > 0 && ok) {
-        uint32_t d[2][32];
-        if (adapts) {
-          tc_fence_after();
-          const uint32_t t = tmem + (uint32_t(q * 32) << 16) + uint32_t(b * kChunk);
-          tmem_ld32(t, d[0]);
-          tmem_ld32(t + 32, d[1]);
-          tmem_wait_ld();
-          tc_fence_before();
-        }
+    Cursor y{0, 0}, c{0, 0};
+    int before = -1;  // the slot whose store may still read it
+    for (int64_t id = blockIdx.x;; id += gridDim.x) {
+      const Unit u = find_unit(a, id, lane);
+      if (u.span.count == 0) break;
+      const int live = min(max(u.span.count - q * kBox, 0), kBox);  // this warp's rows of the span
+      if (u.adapts) {
+        // h of the warp's rows, rows behind the span zero.  (The products of the unit before have ended: this warp
+        // has waited for the last one's accumulator.)
+        const __nv_bfloat16* row = a.h + (u.span.begin + q * kBox + lane) * a.rp;
+        for (int t = 0; t < 2; ++t, row += a.rows.m * a.rp)
+          for (int r = 0; r < a.rp; r += 32) {  // 16 columns of two values; rp is a multiple of 16
+            uint32_t v[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 x = make_uint4(0u, 0u, 0u, 0u);
+              if (lane < live && r + 8 * i < a.rp) x = *reinterpret_cast<const uint4*>(row + r + 8 * i);
+              v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+            }
+            __syncwarp();
+            const uint32_t at = h_tmem + lanes + uint32_t(t * (a.rp / 2) + r / 2);
+            if (r + 32 <= a.rp) tmem_st16(at, v);
+            else tmem_st8(at, v);
+          }
+        tmem_wait_st();
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0 && adapts) mbar_arrive(&acc_empty[b]);
+        if (lane == 0) mbar_arrive(&h_full);
+      }
+      for (int i = 0; i < u.chunks; ++i) {
+        unsigned char* box = ys + y.at * y_bytes + q * kBoxBytes;
+        if (ok) {
+          ok = (!a.has_base || mbar_wait_bounded(&y_full[y.at], y.parity)) &&
+               (!u.adapts || mbar_wait_bounded(&acc_full[c.at], c.parity));
+          if (!ok) report_operator_timeout(a.err);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        const int64_t c0 = int64_t(u.first + i) * kChunk, r0 = u.span.begin + q * kBox;
+        const bool works = live > 0 && ok;
+        if (works) {
+          if (u.adapts || !a.has_base) {
+            unsigned char* mine = box + lane * 128;  // the row's eight 16-byte vectors, swizzled
+            uint32_t d[2][32];
+            if (u.adapts) {
+              tc_fence_after();
+              const uint32_t t = tmem + lanes + uint32_t(c.at * kChunk);
+              tmem_ld32(t, d[0]);
+              tmem_ld32(t + 32, d[1]);
+            } else {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {  // the row's eight 16-byte vectors, swizzled
-          uint4* at = reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4));
-          uint4 y = a.has_base ? *at : make_uint4(0u, 0u, 0u, 0u);
-          if (adapts) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+              for (int e = 0; e < 32; ++e) d[0][e] = d[1][e] = 0u;
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int x = (c & 3) * 8 + 2 * e;
-              w[e] = pack_bf16x2(__uint_as_float(w[e] << 16) + __uint_as_float(d[c >> 2][x]),
-                                 __uint_as_float(w[e] & 0xFFFF0000u) + __uint_as_float(d[c >> 2][x + 1]));
+            for (int e = 0; e < 2; ++e) {
+              uint4 x[4];
+#pragma unroll
+              for (int v = 0; v < 4; ++v)
+                x[v] = a.has_base ? *reinterpret_cast<uint4*>(mine + (((4 * e + v) ^ (lane & 7)) << 4))
+                                  : make_uint4(0u, 0u, 0u, 0u);
+              if (e == 0 && u.adapts) {
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[c.at]);
+              }
+#pragma unroll
+              for (int v = 0; v < 16; ++v) {
+                uint32_t& w = reinterpret_cast<uint32_t*>(&x[v / 4])[v & 3];
+                w = pack_bf16x2(__uint_as_float(w << 16) + __uint_as_float(d[e][2 * v]),
+                                __uint_as_float(w & 0xFFFF0000u) + __uint_as_float(d[e][2 * v + 1]));
+              }
+#pragma unroll
+              for (int v = 0; v < 4; ++v)
+                *reinterpret_cast<uint4*>(mine + (((4 * e + v) ^ (lane & 7)) << 4)) = x[v];
             }
           }
-          *at = y;
+          fence_proxy_async();  // the slot's next reader or writer is TMA
+          __syncwarp();
+          if (live == kBox) {
+            if (lane == 0) {
+              tma_store_3d(&maps.out, box, int32_t(c0), int32_t(r0), 0);
+              bulk_commit();
+            }
+          } else {  // the box's other rows are another span's
+            for (int r = lane >> 3; r < live; r += 4) {
+              const int64_t col = c0 + (lane & 7) * 8;
+              if (col < a.cols)
+                *reinterpret_cast<uint4*>(a.out + (r0 + r) * a.ldo + col) =
+                    *reinterpret_cast<uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            }
+            __syncwarp();
+          }
+        } else if (lane == 0 && u.adapts) {
+          mbar_arrive(&acc_empty[c.at]);
         }
-        const int64_t c0 = int64_t(first + i) * kChunk, r0 = span.begin + q * kBox;
-        fence_proxy_async();  // the stage's next reader or writer is TMA
+        // free the slot whose store has left shared memory: the one before
+        if (lane == 0) {
+          if (works && live == kBox) bulk_wait_read<1>();
+          else bulk_wait_read<0>();
+          if (before >= 0 && a.has_base) mbar_arrive(&y_empty[before]);
+        }
         __syncwarp();
-        if (live == kBox) {
-          if (lane == 0) {
-            tma_store_3d(&maps.out, box, int32_t(c0), int32_t(r0), 0);
-            bulk_commit();
-          }
-        } else {  // the box's other rows are another span's
-          for (int r = lane >> 3; r < live; r += 4) {
-            const int64_t col = c0 + (lane & 7) * 8;
-            if (col < a.cols)
-              *reinterpret_cast<uint4*>(a.out + (r0 + r) * a.ldo + col) =
-                  *reinterpret_cast<uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-          }
-        }
-      } else if (lane == 0 && adapts) {
-        mbar_arrive(&acc_empty[b]);
-      }
-      // free the stage whose store has left shared memory: the one before
-      __syncwarp();
-      if (lane == 0) {
-        bulk_wait_read<1>();
-        if (i > 0) mbar_arrive(&empty[(i - 1) % a.ring.stages]);
+        before = y.at;
+        y.next(n_y);
+        if (u.adapts) c.next(n_acc);
       }
     }
     if (lane == 0) bulk_wait<0>();
@@ -453,7 +570,7 @@ __global__ void __launch_bounds__(kThreads) up_kernel(const __grid_constant__ Up
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, kAcc * kChunk);
+  if (warp == 1) tmem_dealloc(tmem, kUpTmem);
 }
 
 // ---------------------------------------------------------------------------
@@ -596,7 +713,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
         fence_proxy_async();
         __syncwarp();
       }
-      if (lane == 0) {
+      if (elect_one()) {
         tc_fence_after();
         const uint64_t ud = umma_desc_sw128(smem_u32(st), 8192, 1024);
         const uint64_t hd = umma_desc_sw128(smem_u32(st) + kGradU, 8192, 1024);
@@ -610,7 +727,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
       }
       __syncwarp();
     }
-    if (lane == 0) {
+    if (elect_one()) {
       if (!ok) report_operator_timeout(a.err);
       tc_commit(&done);
     }
@@ -719,6 +836,7 @@ cudaError_t allow_smem(F kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+// at most: every segment ends one
 int64_t span_count(const Rows& r) { return cdiv(r.m, kRows) + r.requests + 1; }
 // spans that have rows, about: every request ends one, at most one a row
 int64_t busy_spans(const Rows& r) {
@@ -742,14 +860,14 @@ cudaError_t down(cudaStream_t st, const Rows& r, Matrix u, int64_t c, const void
            : make_map(&maps.w, w, c, rank, r.adapters, c, a.rp)))
     return cudaErrorInvalidValue;
   a.rows = r;
-  a.ring = ring_of(kRows * 128 + down_w_bytes(MN, a.rp), kSmemTwo - 2048);
+  a.room = kSmemTwo - 2048;
   a.steps = cdiv(c, 64);
   a.h = h;
   a.err = err;
   // few rows: K is split while that still adds blocks that find an SM free
   a.split = 1;
   while (a.split < 8 && busy_spans(r) * a.split * 2 <= 2 * sms && a.steps >= a.split * 4) a.split *= 2;
-  const int smem = a.ring.stages * a.ring.stage_bytes + 1024;
+  const int smem = a.room + 1024;
   cudaError_t e = allow_smem(down_kernel<MN>, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
@@ -772,17 +890,15 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   UpMaps maps;
   UpArgs a{};
   a.rp = int(cdiv(rank, 16)) * 16;
-  if (!make_map(&maps.out, out.p, c, r.m, 1, out.ld, kBox) || !make_map(&maps.h, h, a.rp, r.m, 2, a.rp, kBox))
-    return cudaErrorInvalidValue;
+  if (!make_map(&maps.out, out.p, c, r.m, 1, out.ld, kBox)) return cudaErrorInvalidValue;
   if (base.p == nullptr) maps.base = maps.out;
   else if (!make_map(&maps.base, base.p, c, r.m, 1, base.ld, kBox)) return cudaErrorInvalidValue;
   if (!(MN ? make_map(&maps.w, w, c, rank, r.adapters, c, a.rp)
-           : make_map(&maps.w, w, rank, c, r.adapters, rank, kChunk)))
+           : make_map(&maps.w, w, rank, c, r.adapters, rank, kChunk)))  // 64 ranks of 128 columns
     return cudaErrorInvalidValue;
   a.rows = r;
-  // up to rank 64 two blocks share an SM; above, h alone takes 64 KB and one block takes all
-  const int room = (a.rp <= 64 ? kSmemTwo : 2 * kSmemTwo) - up_h_bytes(a.rp) - 2048;
-  a.ring = ring_of(kRows * 128 + up_w_bytes(MN, a.rp), room);
+  a.room = kSmemTwo - 2048;
+  a.h = h;
   a.chunks = cdiv(c, kChunk);
   a.cols = c;
   a.ldo = out.ld;
@@ -790,16 +906,21 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   a.has_base = base.p != nullptr;
   a.in_place = base.p == out.p;
   a.err = err;
-  // few rows: N is split until the blocks fill the SMs, two chunks a block at least
-  int64_t split = cdiv(2 * sms, busy_spans(r));
-  if (split > a.chunks / 2) split = a.chunks / 2;
-  a.split = split < 1 ? 1 : int(split);
-  const int smem = up_h_bytes(a.rp) + a.ring.stages * a.ring.stage_bytes + 1024;
+  // Units of a span: those with which the block that has most to do is done
+  // first.  A unit costs its chunks and the time of about two more until its h
+  // is in TMEM.
+  double best = 0.0;
+  for (int64_t split = 1; split <= a.chunks; ++split) {
+    const double time = double(cdiv(busy_spans(r) * split, 2 * sms)) * (double(cdiv(a.chunks, split)) + 2.0);
+    if (split == 1 || time < best * 0.98) { best = time; a.split = int(split); }
+  }
+  const int64_t units = span_count(r) * a.split;
+  const int smem = a.room + 1024;
   cudaError_t e = allow_smem(up_kernel<MN>, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(span_count(r) * a.split));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(unsigned(units < 2 * sms ? units : 2 * sms));
+  cfg.blockDim = dim3(kUpThreads);
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -810,13 +931,20 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   return cudaLaunchKernelEx(&cfg, up_kernel<MN>, maps, a);
 }
 
-// Shares of an adapter's rows: enough blocks for every SM if the adapters' rows are alike.
+// Shares of an adapter's rows.  A block takes an SM for itself, so the shares
+// are those, of 1 to 3 waves, that leave the fewest SMs idle in the last one if
+// the adapters' rows are alike (at 40 column blocks 8 shares, a little more than
+// two waves, took 88 us where 7 take 64 us).
 int grad_parts(const Rows& r, int64_t blocks, int sms) {
   const int64_t adapters = r.adapters < r.requests ? r.adapters : r.requests;
-  int64_t parts = cdiv(2 * sms, blocks * adapters);
-  const int64_t most = cdiv(r.m, 4 * kGradRows * adapters);
-  if (parts > most) parts = most;
-  return parts < 1 ? 1 : int(parts);
+  const int64_t each = blocks * adapters, most = cdiv(r.m, 4 * kGradRows * adapters);
+  int64_t best = 1;
+  double best_use = 0.0;
+  for (int64_t parts = 1; parts <= most && (parts == 1 || each * parts <= 3 * sms); ++parts) {
+    const double use = double(each * parts) / double(cdiv(each * parts, sms) * sms);
+    if (use > best_use * 1.02) { best = parts; best_use = use; }
+  }
+  return int(best);
 }
 
 int64_t grad_blocks(int64_t c) { return cdiv(c, kGradCols); }

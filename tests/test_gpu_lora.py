@@ -193,6 +193,22 @@ def test_repeated_calls_agree(cuda_device):
         assert all(torch.equal(u, v) for u, v in zip(first, got))
 
 
+@pytest.mark.parametrize("n,rank", [(128, 16), (136, 72), (1024, 8), (5120, 16)])
+def test_spans_with_and_without_adapters_in_turn(cuda_device, n, rank):
+    """Blocks that go from a span with an adapter to one without and back, over and over: the same every time."""
+    lengths = [700, 90, 33, 1000, 5, 260, 128, 640, 300, 1500] * 4
+    p = Problem(lengths, k=64, n=n, rank=rank, adapters=3, slots=[(0, -1, 1, -1, -1, 2, 0)[i % 7] for i in range(40)],
+                tail=400)
+    first = ops.lora_update(p.y, *p.args)
+    p.check_out(first)
+    outs = [ops.lora_update(p.y, *p.args) for _ in range(40)]
+    assert all(torch.equal(first, out) for out in outs)
+    grads = [ops.lora_update_backward(p.dy, *p.args) for _ in range(10)]
+    p.check_grads(*grads[0])
+    assert all(torch.equal(u, v) for g in grads for u, v in zip(grads[0], g))
+    ops.check_operator_errors()
+
+
 def test_autograd(cuda_device):
     """The same gradients as the explicit call, through a projection, and the formula's against differences."""
     p = Problem(lengths=[40, 24], k=64, n=72, rank=8, adapters=2)
