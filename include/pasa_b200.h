@@ -468,8 +468,8 @@ PASA_API int pasa_operator_errors(void* stream, uint32_t* flags);
  *   scale device fp32 [adapters], or NULL for 1
  *   h    scratch of pasa_lora_h_size bytes; what pasa_lora_update_backward
  *        takes as h
- * k, n and rank are multiples of 8, rank at most 128, pointers 16-byte
- * aligned, row strides multiples of 8.  Sums are fp32, h is kept to 2^-17.
+ * k, n and rank are multiples of 8, rank at most 128, adapters at most 4096,
+ * pointers 16-byte aligned, row strides multiples of 8.  Sums are fp32, h is kept to 2^-17.
  */
 PASA_API int pasa_lora_h_size(int64_t m, int rank, size_t* bytes);
 PASA_API int pasa_lora_update(void* stream, const void* x, int64_t ldx, const void* y, int64_t ldy,

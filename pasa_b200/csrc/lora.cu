@@ -21,9 +21,9 @@
 // one term would cost 2^-9.  The second term doubles the small products, which
 // are not what bounds the kernels.  Results are rounded once.
 //
-// Rows are worked on in spans: a span begins at every multiple of 128 rows and
-// at every request's first row, and ends at the next of either, so a span has
-// one adapter.  Every block finds its span from `rows` on the device (no host
+// Rows are worked on in spans: a span begins at every multiple of 128 rows (4 in
+// the kernels for few rows) and at every request's first row, and ends at the
+// next of either, so a span has one adapter.  Every block finds its span from `rows` on the device (no host
 // copy; a captured graph follows new lengths).
 #include "umma.cuh"
 
@@ -56,6 +56,7 @@ struct Span {
 // the rows before the first request, then the requests, then the rows behind
 // the last; each lane of the warp takes a segment's bounds and a prefix sum over
 // their spans finds the one with span t.  All lanes of a warp call it.
+template <int ROWS>
 __device__ __forceinline__ Span find_span(const Rows& a, int64_t t, int lane) {
   Span s{0, 0, -1};
   for (int first = 0; first <= a.requests + 1; first += 32) {
@@ -67,7 +68,7 @@ __device__ __forceinline__ Span find_span(const Rows& a, int64_t t, int lane) {
       if (begin < 0) begin = 0;
       if (end > a.m) end = a.m;
     }
-    const int64_t own = end > begin ? (end - 1) / kRows - begin / kRows + 1 : 0;
+    const int64_t own = end > begin ? (end - 1) / ROWS - begin / ROWS + 1 : 0;
     int64_t upto = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -83,8 +84,8 @@ __device__ __forceinline__ Span find_span(const Rows& a, int64_t t, int lane) {
     t -= __shfl_sync(0xffffffffu, upto - own, src);
     begin = __shfl_sync(0xffffffffu, begin, src);
     end = __shfl_sync(0xffffffffu, end, src);
-    s.begin = t == 0 ? begin : (begin / kRows + t) * kRows;
-    const int64_t next = (s.begin / kRows + 1) * kRows;
+    s.begin = t == 0 ? begin : (begin / ROWS + t) * ROWS;
+    const int64_t next = (s.begin / ROWS + 1) * ROWS;
     s.count = int((next < end ? next : end) - s.begin);
     const int request = first + src - 1;
     if (request >= 0 && request < a.requests) {
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(blockIdx.x % unsigned(a.split));
-  const Span span = find_span(a.rows, blockIdx.x / unsigned(a.split), lane);
+  const Span span = find_span<kRows>(a.rows, blockIdx.x / unsigned(a.split), lane);
   if (span.count == 0 || span.slot < 0) return;  // the same for the whole cluster
 
   const uint32_t cols = a.rp <= 32 ? 32 : a.rp <= 64 ? 64 : 128;
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
   const int first = int(a.steps * rank / a.split), last = int(a.steps * (rank + 1) / a.split);
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int issued = 0;
       for (int i = 0; first + i < last; ++i) {
         const int s = i % ring.stages;
@@ -281,17 +282,17 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
 // run ahead into the next unit.  h (hi and lo) lies in TMEM as the products'
 // first operand.  The base's chunk lands in shared memory by TMA, is added to
 // in place and leaves by TMA from there (by plain stores where a box of 32 rows
-// reaches into another span); each of the four epilogue warps owns a box of 32
-// rows and waits for no other.  The base and the weights have rings of their
+// reaches into another span).  The base and the weights have rings of their
 // own: the weights' is freed by the product, the base's only when its store has
-// left.  A chunk's way from TMEM through shared memory is 1000 to 2000 clocks
-// of latency; the SM's second block fills them.  (One block an SM with two sets
-// of epilogue warps in turn needs both sets to see every phase of both rings,
-// and was slower: 61 against 51 us for 24 single rows.)
+// left.  The epilogue is a chain of latencies, 1200 clocks a chunk for its four
+// warps (waits 330, TMEM 320, sums and shared memory 510), which the SM's
+// second block fills; issuing the stores and waiting for them, 400 more, is a
+// warp of its own.  (One block an SM with two sets of epilogue warps in turn
+// needs both sets to see every phase of both rings, and was slower.)
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 64;
 constexpr int kMaxAcc = 3;          // accumulators in flight
-constexpr int kUpThreads = 224;     // warp 0 base, 1 MMA + TMEM, 2 weights, 3-6 epilogue
+constexpr int kUpThreads = 256;     // warp 0 base, 1 MMA + TMEM, 2 weights, 3-6 epilogue, 7 stores
 constexpr int kUpEpi = 4;
 constexpr uint32_t kUpTmem = 256;   // accumulators from column 0; h (hi, then lo, rp / 2 each) at the end
 
@@ -323,7 +324,7 @@ struct Unit {
 
 __device__ __forceinline__ Unit find_unit(const UpArgs& a, int64_t id, int lane) {
   Unit u;
-  u.span = find_span(a.rows, id / a.split, lane);
+  u.span = find_span<kRows>(a.rows, id / a.split, lane);
   const int part = int(id % a.split);
   u.first = int(a.chunks * part / a.split);
   u.chunks = int(a.chunks * (part + 1) / a.split) - u.first;
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t y_full[kMaxStages], y_empty[kMaxStages], w_full[kMaxStages], w_empty[kMaxStages];
+  __shared__ uint64_t y_full[kMaxStages], y_done[kMaxStages], y_empty[kMaxStages], w_full[kMaxStages], w_empty[kMaxStages];
   __shared__ uint64_t acc_full[kMaxAcc], acc_empty[kMaxAcc], h_full;
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
   unsigned char* ys = sm + n_w * w_bytes;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < n_y; ++s) { mbar_init(&y_full[s], 1); mbar_init(&y_empty[s], kUpEpi); }
+    for (int s = 0; s < n_y; ++s) { mbar_init(&y_full[s], 1); mbar_init(&y_done[s], kUpEpi); mbar_init(&y_empty[s], 1); }
     for (int s = 0; s < n_w; ++s) { mbar_init(&w_full[s], 1); mbar_init(&w_empty[s], 1); }
     for (int b = 0; b < n_acc; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], kUpEpi); }
     mbar_init(&h_full, kUpEpi);
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
       const Unit u = find_unit(a, id, lane);
       if (u.span.count == 0) break;
       if (weights ? !u.adapts : !a.has_base) continue;
-      if (lane == 0) {
+      if (elect_one()) {
         for (int i = 0; i < u.chunks; ++i) {
           if (!mbar_wait_bounded(&empty[c.at], c.parity)) {
             report_operator_timeout(a.err);
@@ -413,9 +414,9 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
           c.next(slots);
         }
       }
-      ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+      ok = __all_sync(0xffffffffu, ok);
     }
-    if (lane == 0)  // the copies in flight land before the block can end
+    if (elect_one())  // the copies in flight land before the block can end
       for (int64_t i = issued > slots ? issued - slots : 0; i < issued; ++i)
         mbar_wait_bounded(&full[i % slots], uint32_t((i / slots) & 1));
   } else if (warp == 1) {
@@ -453,13 +454,42 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
       h_parity ^= 1u;
       ok = __all_sync(0xffffffffu, ok);  // the elected lane's, the others' is true
     }
+  } else if (warp == 7) {
+    // full boxes leave by TMA; a slot is free when its boxes have left shared memory
+    wait_for_predecessor();
+    bool ok = true;
+    Cursor y{0, 0};
+    int before = -1;  // the slot whose stores may still read it
+    for (int64_t id = blockIdx.x; ok; id += gridDim.x) {
+      const Unit u = find_unit(a, id, lane);
+      if (u.span.count == 0) break;
+      if (elect_one()) {
+        for (int i = 0; i < u.chunks; ++i) {
+          if (!mbar_wait_bounded(&y_done[y.at], y.parity)) {
+            report_operator_timeout(a.err);
+            ok = false;
+            break;
+          }
+          for (int b = 0; (b + 1) * kBox <= u.span.count; ++b)
+            tma_store_3d(&maps.out, ys + y.at * y_bytes + b * kBoxBytes, (u.first + i) * kChunk,
+                         int32_t(u.span.begin) + b * kBox, 0);
+          bulk_commit();
+          bulk_wait_read<1>();
+          if (before >= 0) mbar_arrive(&y_empty[before]);
+          before = y.at;
+          y.next(n_y);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (elect_one()) bulk_wait<0>();
   } else {
     const int q = warp & 3;
     const uint32_t lanes = uint32_t(q * 32) << 16;
     wait_for_predecessor();
     bool ok = true;
-    Cursor y{0, 0}, c{0, 0};
-    int before = -1;  // the slot whose store may still read it
+    Cursor y{0, a.has_base ? 0u : 1u}, c{0, 0};  // of the base's arrivals, or of the slots that are free
+    uint64_t* ready = a.has_base ? y_full : y_empty;
     for (int64_t id = blockIdx.x;; id += gridDim.x) {
       const Unit u = find_unit(a, id, lane);
       if (u.span.count == 0) break;
@@ -490,7 +520,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
       for (int i = 0; i < u.chunks; ++i) {
         unsigned char* box = ys + y.at * y_bytes + q * kBoxBytes;
         if (ok) {
-          ok = (!a.has_base || mbar_wait_bounded(&y_full[y.at], y.parity)) &&
+          ok = mbar_wait_bounded(&ready[y.at], y.parity) &&
                (!u.adapts || mbar_wait_bounded(&acc_full[c.at], c.parity));
           if (!ok) report_operator_timeout(a.err);
         }
@@ -536,36 +566,22 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
           }
           fence_proxy_async();  // the slot's next reader or writer is TMA
           __syncwarp();
-          if (live == kBox) {
-            if (lane == 0) {
-              tma_store_3d(&maps.out, box, int32_t(c0), int32_t(r0), 0);
-              bulk_commit();
-            }
-          } else {  // the box's other rows are another span's
+          if (live < kBox)  // the box's other rows are another span's
             for (int r = lane >> 3; r < live; r += 4) {
               const int64_t col = c0 + (lane & 7) * 8;
               if (col < a.cols)
                 *reinterpret_cast<uint4*>(a.out + (r0 + r) * a.ldo + col) =
                     *reinterpret_cast<uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
             }
-            __syncwarp();
-          }
         } else if (lane == 0 && u.adapts) {
           mbar_arrive(&acc_empty[c.at]);
         }
-        // free the slot whose store has left shared memory: the one before
-        if (lane == 0) {
-          if (works && live == kBox) bulk_wait_read<1>();
-          else bulk_wait_read<0>();
-          if (before >= 0 && a.has_base) mbar_arrive(&y_empty[before]);
-        }
         __syncwarp();
-        before = y.at;
+        if (lane == 0) mbar_arrive(&y_done[y.at]);
         y.next(n_y);
         if (u.adapts) c.next(n_acc);
       }
     }
-    if (lane == 0) bulk_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -574,18 +590,175 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
 }
 
 // ---------------------------------------------------------------------------
-// grad: for each adapter, d[C, R] = sum over its rows of u[row, C]^T h[row, R]:
-// dA = (x, g) and dB = (dy, h) in one launch.  A block owns 256 columns of one
-// of the two, an adapter and a share of the adapter's 64-row stages; a stage's
-// rows behind the request's last are zeroed in shared memory (they hold
-// another request's values, which may be NaN).  hi and lo sit side by side as
-// the columns of one operand, so a stage is 8 MMAs of M = 128, N = 128 (N = 256
-// above rank 64); the two halves are added at the end.  Shares of one adapter
-// are summed in order by a second kernel.
+// Few rows (single tokens of many requests): both products read the requests'
+// weights once and do next to nothing with them, so what counts is how many
+// loads are in flight.  On the tensor cores a span of one row still takes 128
+// rows' epilogue, 1500 clocks for 8 KB of weights; here 24 single rows of
+// 5120 -> 30720 at rank 64 (76 MB) take 34 us where they took 57 us.
 // ---------------------------------------------------------------------------
-constexpr int kGradRows = 64;
-constexpr int kGradCols = 256;
-constexpr int kGradU = kGradRows * kGradCols * 2;
+constexpr int kFewRows = 4;         // rows of a span
+constexpr int kFewMost = 64;        // rows of a call that takes this way
+constexpr int kFewRanks = 8;        // ranks of a down block
+constexpr int kFewWarps = 8;
+constexpr int kFewCols = 128;       // columns of an up block, one a thread
+
+struct FewArgs {
+  Rows rows;
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* w;
+  const __nv_bfloat16* base;
+  __nv_bfloat16* h;  // [2][m][rp]
+  __nv_bfloat16* out;
+  int64_t ldx, ldbase, ldo, k, cols;
+  int rank, rp, in_place;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
+// h of a span (blockIdx.x) and 8 ranks (blockIdx.y).  The warps take every
+// eighth 512 bytes of the rows of A and x, so a warp has eight rows' loads in
+// flight at once (a warp a rank had four: 14.2 against 11.6 us);
+// their sums meet in shared memory.
+__global__ void __launch_bounds__(32 * kFewWarps) down_few_kernel(const __grid_constant__ FewArgs a) {
+  __shared__ float part[kFewWarps][kFewRanks][kFewRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Span span = find_span<kFewRows>(a.rows, blockIdx.x, lane);
+  dependents_may_start();
+  if (span.count == 0 || span.slot < 0) return;
+  const int r0 = int(blockIdx.y) * kFewRanks;
+  float sum[kFewRanks][kFewRows] = {};
+  if (r0 < a.rank) {  // a multiple of 8; the ranks that fill up to rp are zero
+    const __nv_bfloat16* w = a.w + (int64_t(span.slot) * a.rank + r0) * a.k;
+    const __nv_bfloat16* x = a.x + span.begin * a.ldx;
+    for (int64_t c = warp * 256 + lane * 8; c < a.k; c += kFewWarps * 256) {
+      uint4 f[kFewRanks], v[kFewRows];
+#pragma unroll
+      for (int r = 0; r < kFewRanks; ++r) f[r] = *reinterpret_cast<const uint4*>(w + r * a.k + c);
+#pragma unroll
+      for (int i = 0; i < kFewRows; ++i)
+        if (i < span.count) v[i] = *reinterpret_cast<const uint4*>(x + i * a.ldx + c);
+#pragma unroll
+      for (int i = 0; i < kFewRows; ++i) {
+        if (i >= span.count) break;
+        float xv[8];
+        unpack8(v[i], xv);
+#pragma unroll
+        for (int r = 0; r < kFewRanks; ++r) {
+          float fv[8];
+          unpack8(f[r], fv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[r][i] = fmaf(fv[e], xv[e], sum[r][i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kFewRanks; ++r)
+#pragma unroll
+    for (int i = 0; i < kFewRows; ++i) {
+      if (i >= span.count) break;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) sum[r][i] += __shfl_xor_sync(0xffffffffu, sum[r][i], off);
+      if (lane == 0) part[warp][r][i] = sum[r][i];
+    }
+  __syncthreads();
+  if (threadIdx.x < kFewRanks * kFewRows) {
+    const int r = threadIdx.x / kFewRows, i = threadIdx.x % kFewRows;
+    if (i < span.count) {
+      float total = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) total += part[w][r][i];
+      uint32_t hi, lo;
+      split2((a.rows.scale ? a.rows.scale[span.slot] : 1.f) * total, 0.f, hi, lo);
+      __nv_bfloat16* h = a.h + (span.begin + i) * a.rp + r0 + r;
+      *reinterpret_cast<uint16_t*>(h) = uint16_t(hi);
+      *reinterpret_cast<uint16_t*>(h + a.rows.m * a.rp) = uint16_t(lo);
+    }
+  }
+}
+
+// out of a span (blockIdx.y) and 128 columns (blockIdx.x): the columns' rows of
+// B, which lie one behind the other, go through shared memory (a thread's row 16
+// bytes further than the one before, so that its 16-byte reads meet no other's
+// bank).
+__global__ void __launch_bounds__(kFewCols) up_few_kernel(const __grid_constant__ FewArgs a) {
+  extern __shared__ uint4 few_smem[];
+  __shared__ float h[kFewRows][kMaxRank];
+  const int tid = threadIdx.x;
+  const Span span = find_span<kFewRows>(a.rows, blockIdx.y, tid & 31);
+  if (span.count == 0 || (span.slot < 0 && a.in_place)) return;
+  const int64_t c0 = int64_t(blockIdx.x) * kFewCols, col = c0 + tid;
+  const int vecs = a.rank / 8, pitch = vecs + 1;
+  const int live = int(a.cols - c0 < kFewCols ? a.cols - c0 : kFewCols);
+  if (span.slot >= 0) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.w + (int64_t(span.slot) * a.cols + c0) * a.rank);
+    for (int i = tid; i < live * vecs; i += kFewCols)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                   :: "r"(smem_u32(few_smem + (i / vecs) * pitch + i % vecs)), "l"(src + i) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  float acc[kFewRows];
+#pragma unroll
+  for (int i = 0; i < kFewRows; ++i)
+    acc[i] = i < span.count && col < a.cols ? __bfloat162float(a.base[(span.begin + i) * a.ldbase + col]) : 0.f;
+  wait_for_predecessor();
+  if (span.slot >= 0) {
+    for (int i = tid; i < span.count * a.rank; i += kFewCols) {
+      const int row = i / a.rank, r = i - row * a.rank;
+      const __nv_bfloat16* src = a.h + (span.begin + row) * a.rp + r;
+      h[row][r] = __bfloat162float(*src) + __bfloat162float(src[a.rows.m * a.rp]);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    if (col < a.cols) {
+      float sum[kFewRows] = {};
+      for (int v = 0; v < vecs; ++v) {
+        float f[8];
+        unpack8(few_smem[tid * pitch + v], f);
+#pragma unroll
+        for (int i = 0; i < kFewRows; ++i) {
+          if (i >= span.count) break;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[i] = fmaf(f[e], h[i][8 * v + e], sum[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kFewRows; ++i) acc[i] += sum[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kFewRows; ++i)
+    if (i < span.count && col < a.cols) a.out[(span.begin + i) * a.ldo + col] = __float2bfloat16_rn(acc[i]);
+}
+
+// ---------------------------------------------------------------------------
+// grad: for each adapter, d[C, R] = sum over its rows of u[row, C]^T h[row, R]:
+// dA = (x, g) and dB = (dy, h) in one launch.
+//
+// The rows go by in stages of 32 (64 above rank 64) of one request, adapter by
+// adapter; the list of all stages is cut into equal shares, so adapters of very
+// different numbers of rows keep all SMs busy.  A block owns 512 columns (256
+// above rank 64) of x or of dy and one share; where its share passes from one
+// adapter to the next it puts down what it has summed.  An adapter that lies in
+// one share is written at once; the others' sums go to the workspace and a
+// second kernel adds them in the order of the shares.
+//
+// A stage's rows behind the request's last are zeroed in shared memory: they
+// hold another request's values, which may be NaN.  hi and lo sit side by side
+// as the columns of one operand, so 16 rows and 128 columns are one MMA of
+// N = 128 (256 above rank 64); the two halves are added at the end.  h is read
+// again by every column block, which is why a block is as wide as TMEM allows.
+// ---------------------------------------------------------------------------
+constexpr int kMaxAdapters = 4096;
+__host__ __device__ constexpr int grad_cols(int atoms) { return atoms == 1 ? 512 : 256; }
+__host__ __device__ constexpr int grad_rows(int atoms) { return atoms == 1 ? 32 : 64; }
 
 struct GradMaps {
   CUtensorMap u[2], h[2];
@@ -594,21 +767,71 @@ struct GradArgs {
   Rows rows;
   Ring ring;
   int rank, atoms;
-  int problem0;           // the first problem computed (0: dA, 1: dB)
+  int problem0;                // the first problem computed (0: dA, 1: dB)
   int64_t cols[2], blocks[2];  // columns and column blocks
-  int parts;              // shares of an adapter's rows
-  float* partial;         // [parts][adapters][rank * cols] for each problem, if parts > 1
+  int shares;
+  float* partial;         // [shares + adapters][rank * cols] for each problem
   __nv_bfloat16* out[2];  // [adapters][rank][cols], [adapters][cols][rank]
   uint32_t* err;
 };
 
-__device__ __forceinline__ int request_stages(const Rows& a, int q, int slot, int64_t& begin, int64_t& end) {
-  if (q >= a.requests || a.slots[q] != slot) return 0;
+// Stages of request q, and the adapter that they belong to (-1: none).
+__device__ __forceinline__ int request_stages(const Rows& a, int q, int stage_rows, int& slot, int64_t& begin,
+                                              int64_t& end) {
+  slot = -1;
+  begin = end = 0;
+  if (q >= a.requests) return 0;
+  const int s = a.slots[q];
+  if (s < 0 || s >= a.adapters) return 0;
   begin = a.rows[q];
   end = a.rows[q + 1];
   if (begin < 0) begin = 0;
   if (end > a.m) end = a.m;
-  return end > begin ? int((end - begin + kGradRows - 1) / kGradRows) : 0;
+  if (end <= begin) return 0;
+  slot = s;
+  return int((end - begin + stage_rows - 1) / stage_rows);
+}
+
+// First stage of a share, of `total`.
+__device__ __forceinline__ int share_begin(int total, int share, int shares) {
+  return int(int64_t(total) * share / shares);
+}
+
+// The part of a share that belongs to one adapter: its stages [first, first + count) of that adapter.
+struct Piece {
+  int slot, first, count;
+  int base;    // stages of the adapters before
+  bool whole;  // all of the adapter's
+};
+
+// The piece of the share [g0, g1) behind `after` (slot -1, base 0: the first); count 0: there is none.  All lanes.
+__device__ __forceinline__ Piece next_piece(const int* stages, int adapters, int g0, int g1, const Piece& after,
+                                            int lane) {
+  Piece p{-1, 0, 0, after.base, false};
+  int from = after.slot + 1;
+  if (after.slot >= 0) p.base += stages[after.slot];
+  for (; from < adapters && p.base < g1; from += 32) {
+    const int own = from + lane < adapters ? stages[from + lane] : 0;
+    int upto = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += v;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, own > 0 && p.base + upto > g0);
+    if (hit != 0) {
+      const int src = __ffs(int(hit)) - 1;
+      const int n = __shfl_sync(0xffffffffu, own, src);
+      p.base += __shfl_sync(0xffffffffu, upto, src) - n;
+      p.slot = from + src;
+      p.first = max(g0 - p.base, 0);
+      p.count = max(min(g1 - p.base, n) - p.first, 0);
+      p.whole = p.count == n;
+      return p;
+    }
+    p.base += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return p;
 }
 
 __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ GradMaps maps,
@@ -616,166 +839,191 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  int* stages = reinterpret_cast<int*>(sm + a.ring.stages * a.ring.stage_bytes);  // [adapters]
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full, acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ int valid[kMaxStages];  // rows of a stage that are the request's
-  __shared__ int stages_total;
+  __shared__ int total;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int width = grad_cols(a.atoms), stage_rows = grad_rows(a.atoms), box = stage_rows * 128;
   int64_t id = blockIdx.x;
   int problem = a.problem0;
-  const int64_t each = int64_t(a.parts) * a.rows.adapters;
-  if (problem == 0 && id >= a.blocks[0] * each) { id -= a.blocks[0] * each; problem = 1; }
-  const int64_t col0 = (id % a.blocks[problem]) * kGradCols;
-  id /= a.blocks[problem];
-  const int part = int(id % a.parts), slot = int(id / a.parts);
+  if (problem == 0 && id >= a.blocks[0] * a.shares) { id -= a.blocks[0] * a.shares; problem = 1; }
+  const int64_t col0 = (id % a.blocks[problem]) * width;
+  const int share = int(id / a.blocks[problem]);
   const int n = 128 * a.atoms;                // accumulator columns of 128 matrix columns: hi, then lo
-  const uint32_t cols = uint32_t(2 * n);
+  constexpr uint32_t cols = 512;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.ring.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    mbar_init(&done, 1);
+    mbar_init(&acc_full, 1);
+    mbar_init(&acc_empty, 4);
     fence_barrier_init();
+    total = 0;
   }
+  for (int s = int(threadIdx.x); s < a.rows.adapters; s += kThreads) stages[s] = 0;
   if (warp == 1) { tmem_alloc(&tmem_slot, cols); tmem_relinquish(); }
-  if (warp == 0) {
-    int total = 0;
-    int64_t begin, end;
-    for (int q = lane; q < a.rows.requests; q += 32) total += request_stages(a.rows, q, slot, begin, end);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-    if (lane == 0) stages_total = total;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  for (int q = int(threadIdx.x); q < a.rows.requests; q += kThreads) {
+    int slot;
+    int64_t begin, end;
+    const int own = request_stages(a.rows, q, stage_rows, slot, begin, end);
+    if (own > 0) { atomicAdd(&stages[slot], own); atomicAdd(&total, own); }
+  }
+  __syncthreads();
   const uint32_t tmem = tmem_slot;
-  const int first = int(int64_t(stages_total) * part / a.parts);
-  const int mine = int(int64_t(stages_total) * (part + 1) / a.parts) - first;
+  const int g0 = share_begin(total, share, a.shares), g1 = share_begin(total, share + 1, a.shares);
+  const Piece none{-1, 0, 0, 0, false};
 
   if (warp == 0) {
-    // all lanes look for the adapter's requests, lane 0 issues
-    int i = 0, base = 0;
+    // all lanes look for the pieces' requests, one issues
+    Cursor c{0, 1};
+    int issued = 0;
     bool ok = true;
-    for (int q0 = 0; q0 < a.rows.requests && i < mine && ok; q0 += 32) {
-      int64_t begin = 0, end = 0;
-      const int own = request_stages(a.rows, q0 + lane, slot, begin, end);
-      int upto = own;  // inclusive prefix sum
+    for (Piece p = next_piece(stages, a.rows.adapters, g0, g1, none, lane); p.count > 0 && ok;
+         p = next_piece(stages, a.rows.adapters, g0, g1, p, lane)) {
+      int base = 0, done = 0;  // the adapter's stages in the requests so far; the piece's stages so far
+      for (int q0 = 0; q0 < a.rows.requests && done < p.count && ok; q0 += 32) {
+        int64_t begin, end;
+        int slot;
+        int own = request_stages(a.rows, q0 + lane, stage_rows, slot, begin, end);
+        if (slot != p.slot) own = 0;
+        int upto = own;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, off);
-        if (lane >= off) upto += v;
-      }
-      const uint32_t some = __ballot_sync(0xffffffffu, own > 0);
-      for (uint32_t left = some; left != 0 && i < mine && ok; left &= left - 1) {
-        const int src = __ffs(int(left)) - 1;
-        const int count = __shfl_sync(0xffffffffu, own, src);
-        const int before = base + __shfl_sync(0xffffffffu, upto, src) - count;
-        const int64_t r0 = __shfl_sync(0xffffffffu, begin, src), r1 = __shfl_sync(0xffffffffu, end, src);
-        for (int t = max(0, first + i - before); t < count && i < mine && ok; ++t, ++i) {
-          const int s = i % a.ring.stages;
-          ok = mbar_wait_bounded(&empty[s], uint32_t((i / a.ring.stages) & 1) ^ 1u);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) {
-            const int64_t row = r0 + int64_t(t) * kGradRows;
-            unsigned char* st = sm + s * a.ring.stage_bytes;
-            valid[s] = int(r1 - row < kGradRows ? r1 - row : kGradRows);
-            mbar_arrive_expect_tx(&full[s], uint32_t(a.ring.stage_bytes));
-            for (int c = 0; c < kGradCols; c += 64)
-              tma_load_3d(st + c * 128, &maps.u[problem], &full[s], int32_t(col0) + c, int32_t(row), 0);
-            for (int c = 0; c < 2 * a.atoms; ++c)
-              tma_load_3d(st + kGradU + c * 8192, &maps.h[problem], &full[s], (c % a.atoms) * 64, int32_t(row),
-                          c / a.atoms);
-          }
-          __syncwarp();
+        for (int off = 1; off < 32; off <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, off);
+          if (lane >= off) upto += v;
         }
+        for (uint32_t left = __ballot_sync(0xffffffffu, own > 0); left != 0 && done < p.count && ok;
+             left &= left - 1) {
+          const int src = __ffs(int(left)) - 1;
+          const int count = __shfl_sync(0xffffffffu, own, src);
+          const int before = base + __shfl_sync(0xffffffffu, upto, src) - count;
+          const int64_t r0 = __shfl_sync(0xffffffffu, begin, src), r1 = __shfl_sync(0xffffffffu, end, src);
+          for (int t = max(0, p.first + done - before); t < count && done < p.count && ok; ++t, ++done) {
+            ok = mbar_wait_bounded(&empty[c.at], c.parity);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (elect_one()) {
+              const int64_t row = r0 + int64_t(t) * stage_rows;
+              unsigned char* st = sm + c.at * a.ring.stage_bytes;
+              valid[c.at] = int(r1 - row < stage_rows ? r1 - row : stage_rows);
+              mbar_arrive_expect_tx(&full[c.at], uint32_t(a.ring.stage_bytes));
+              for (int x = 0; x < width / 64; ++x)
+                tma_load_3d(st + x * box, &maps.u[problem], &full[c.at], int32_t(col0) + x * 64, int32_t(row), 0);
+              for (int x = 0; x < 2 * a.atoms; ++x)
+                tma_load_3d(st + (width / 64 + x) * box, &maps.h[problem], &full[c.at], (x % a.atoms) * 64,
+                            int32_t(row), x / a.atoms);
+            }
+            __syncwarp();
+            ++issued;
+            c.next(a.ring.stages);
+          }
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31);
       }
-      base += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (!ok && lane == 0) report_operator_timeout(a.err);
-    for (int j = i > a.ring.stages ? i - a.ring.stages : 0; j < i; ++j)
+    for (int j = issued > a.ring.stages ? issued - a.ring.stages : 0; j < issued; ++j)
       mbar_wait_bounded(&full[j % a.ring.stages], uint32_t((j / a.ring.stages) & 1));
   } else if (warp == 1) {
     const uint32_t idesc = umma_idesc_bf16(128, n, true, true);
+    Cursor c{0, 0};
+    uint32_t acc_parity = 1;
     bool ok = true;
-    for (int i = 0; i < mine; ++i) {
-      const int s = i % a.ring.stages;
-      ok = mbar_wait_bounded(&full[s], uint32_t((i / a.ring.stages) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      unsigned char* st = sm + s * a.ring.stage_bytes;
-      const int rows = valid[s];
-      if (rows < kGradRows) {  // zero the other rows of every [64 rows][64] box
-        const int per_box = (kGradRows - rows) * 8, boxes = a.ring.stage_bytes / 8192;
-        for (int j = lane; j < boxes * per_box; j += 32)
-          *reinterpret_cast<uint4*>(st + (j / per_box) * 8192 + rows * 128 + (j % per_box) * 16) =
-              make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async();
+    for (Piece p = next_piece(stages, a.rows.adapters, g0, g1, none, lane); p.count > 0 && ok;
+         p = next_piece(stages, a.rows.adapters, g0, g1, p, lane)) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_empty, acc_parity));
+      acc_parity ^= 1u;
+      for (int i = 0; i < p.count && ok; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[c.at], c.parity));
+        if (!ok) break;
+        unsigned char* st = sm + c.at * a.ring.stage_bytes;
+        const int rows = valid[c.at];
+        if (rows < stage_rows) {  // zero the other rows of every box
+          const int per_box = (stage_rows - rows) * 8, boxes = width / 64 + 2 * a.atoms;
+          for (int j = lane; j < boxes * per_box; j += 32)
+            *reinterpret_cast<uint4*>(st + (j / per_box) * box + rows * 128 + (j % per_box) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (elect_one()) {
+          tc_fence_after();
+          const uint64_t ud = umma_desc_sw128(smem_u32(st), uint32_t(box), 1024);
+          const uint64_t hd = umma_desc_sw128(smem_u32(st) + uint32_t(width / 64 * box), uint32_t(box), 1024);
+          for (int x = 0; x < width / 128; ++x)
+            for (int kk = 0; kk < stage_rows / 16; ++kk)
+              mma_ss(tmem + uint32_t(x * n), ud + uint64_t((x * 2 * box + kk * 2048) >> 4),
+                     hd + uint64_t((kk * 2048) >> 4), idesc, i > 0 || kk > 0 ? 1u : 0u);
+          tc_commit(&empty[c.at]);
+          if (i == p.count - 1) tc_commit(&acc_full);
+        }
         __syncwarp();
+        c.next(a.ring.stages);
       }
-      if (elect_one()) {
-        tc_fence_after();
-        const uint64_t ud = umma_desc_sw128(smem_u32(st), 8192, 1024);
-        const uint64_t hd = umma_desc_sw128(smem_u32(st) + kGradU, 8192, 1024);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int kk = 0; kk < kGradRows / 16; ++kk)
-            mma_ss(tmem + uint32_t(c * n), ud + uint64_t((c * 16384 + kk * 2048) >> 4),
-                   hd + uint64_t((kk * 2048) >> 4), idesc, i > 0 || kk > 0 ? 1u : 0u);
-        tc_commit(&empty[s]);
-      }
-      __syncwarp();
     }
-    if (elect_one()) {
-      if (!ok) report_operator_timeout(a.err);
-      tc_commit(&done);
-    }
+    if (!ok && lane == 0) report_operator_timeout(a.err);
   } else {
     const int q = warp & 3;
-    if (!mbar_wait_bounded(&done, 0)) report_operator_timeout(a.err);
-    tc_fence_after();
     const int64_t size = int64_t(a.rank) * a.cols[problem];
-    float* partial = a.partial + (problem == 1 && a.problem0 == 0 ? each * a.rank * a.cols[0] : 0) +
-                     (int64_t(part) * a.rows.adapters + slot) * size;
-    __nv_bfloat16* out = a.out[problem] + int64_t(slot) * size;
-    for (int c = 0; c < 2; ++c) {
-      const int64_t col = col0 + c * 128 + q * 32 + lane;
-      for (int r0 = 0; r0 < a.rank; r0 += 16) {
-        uint32_t hi[16], lo[16];
-        __syncwarp();
-        const uint32_t t = tmem + (uint32_t(q * 32) << 16) + uint32_t(c * n + r0);
-        tmem_ld16(t, hi);
-        tmem_ld16(t + uint32_t(n / 2), lo);
-        tmem_wait_ld();
-        float v[16];
+    uint32_t acc_parity = 0;
+    for (Piece p = next_piece(stages, a.rows.adapters, g0, g1, none, lane); p.count > 0;
+         p = next_piece(stages, a.rows.adapters, g0, g1, p, lane)) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full, acc_parity))) {
+        if (lane == 0) report_operator_timeout(a.err);
+        break;
+      }
+      acc_parity ^= 1u;
+      tc_fence_after();
+      // a piece's place is its share and its adapter together: either grows from one piece to the next
+      float* partial = a.partial +
+                       (problem == 1 && a.problem0 == 0 ? int64_t(a.shares + a.rows.adapters) * a.rank * a.cols[0] : 0) +
+                       int64_t(share + p.slot) * size;
+      __nv_bfloat16* out = a.out[problem] + int64_t(p.slot) * size;
+      for (int x = 0; x < width / 128; ++x) {
+        const int64_t col = col0 + x * 128 + q * 32 + lane;
+        for (int r0 = 0; r0 < a.rank; r0 += 16) {
+          uint32_t hi[16], lo[16];
+          __syncwarp();
+          const uint32_t t = tmem + (uint32_t(q * 32) << 16) + uint32_t(x * n + r0);
+          tmem_ld16(t, hi);
+          tmem_ld16(t + uint32_t(n / 2), lo);
+          tmem_wait_ld();
+          float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = mine > 0 ? __uint_as_float(hi[i]) + __uint_as_float(lo[i]) : 0.f;
-        if (col < a.cols[problem]) {
+          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
+          if (col < a.cols[problem]) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 8) {
-            if (r0 + i >= a.rank) continue;  // a multiple of 8
-            if (problem == 0) {
+            for (int i = 0; i < 16; i += 8) {
+              if (r0 + i >= a.rank) continue;  // a multiple of 8
+              if (problem == 0) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int64_t at = int64_t(r0 + i + e) * a.cols[0] + col;
-                if (a.parts > 1) partial[at] = v[i + e];
-                else out[at] = __float2bfloat16_rn(v[i + e]);
-              }
-            } else {
-              const int64_t at = col * a.rank + r0 + i;
-              if (a.parts > 1) {
-                *reinterpret_cast<float4*>(partial + at) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                *reinterpret_cast<float4*>(partial + at + 4) = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
+                for (int e = 0; e < 8; ++e) {
+                  const int64_t at = int64_t(r0 + i + e) * a.cols[0] + col;
+                  if (p.whole) out[at] = __float2bfloat16_rn(v[i + e]);
+                  else partial[at] = v[i + e];
+                }
               } else {
-                *reinterpret_cast<uint4*>(out + at) =
-                    make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
-                               pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+                const int64_t at = col * a.rank + r0 + i;
+                if (p.whole) {
+                  *reinterpret_cast<uint4*>(out + at) =
+                      make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
+                                 pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+                } else {
+                  *reinterpret_cast<float4*>(partial + at) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                  *reinterpret_cast<float4*>(partial + at + 4) = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
+                }
               }
             }
           }
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty);
     }
   }
   tc_fence_before();
@@ -784,28 +1032,62 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
   if (warp == 1) tmem_dealloc(tmem, cols);
 }
 
-// out = bf16(sum over the parts, in order), 8 values a thread; dA's values, then dB's.
-__global__ void __launch_bounds__(256) grad_sum_kernel(const float* __restrict__ partial, int parts, int64_t size0,
-                                                       int64_t size1, __nv_bfloat16* out0, __nv_bfloat16* out1) {
+// The adapters (blockIdx.y) whose stages lie in several shares: out = bf16(sum
+// over the shares, in order); and zero for those without rows.  8 values a
+// thread, dA's and then dB's.
+struct SumArgs {
+  Rows rows;
+  int stage_rows, shares;
+  const float* partial;
+  int64_t size[2];  // of one adapter; 0: not computed
+  __nv_bfloat16* out[2];
+};
+
+__global__ void __launch_bounds__(256) grad_sum_kernel(const __grid_constant__ SumArgs a) {
+  __shared__ int before, mine, total;
+  const int adapter = int(blockIdx.y);
+  if (threadIdx.x == 0) before = mine = total = 0;
+  __syncthreads();
+  int sum[3] = {0, 0, 0};
+  for (int q = int(threadIdx.x); q < a.rows.requests; q += 256) {
+    int slot;
+    int64_t begin, end;
+    const int own = request_stages(a.rows, q, a.stage_rows, slot, begin, end);
+    if (own > 0) {
+      sum[2] += own;
+      if (slot < adapter) sum[0] += own;
+      if (slot == adapter) sum[1] += own;
+    }
+  }
+  if (sum[2] > 0) { atomicAdd(&before, sum[0]); atomicAdd(&mine, sum[1]); atomicAdd(&total, sum[2]); }
+  __syncthreads();
+  int first = 0, last = -1;  // the shares of the adapter's first and last stage
+  if (mine > 0) {
+    while (share_begin(total, first + 1, a.shares) <= before) ++first;
+    last = first;
+    while (share_begin(total, last + 1, a.shares) < before + mine) ++last;
+    if (first == last) return;  // written whole
+  }
   int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
-  int64_t size = size0;
-  __nv_bfloat16* out = out0;
-  if (i >= size0) {
-    i -= size0;
-    partial += size0 * parts;
-    size = size1;
-    out = out1;
-    if (i >= size1) return;
+  const float* partial = a.partial;
+  int problem = 0;
+  if (i >= a.size[0]) {
+    i -= a.size[0];
+    partial += int64_t(a.shares + a.rows.adapters) * a.size[0];
+    problem = 1;
+    if (i >= a.size[1]) return;
   }
   float v[8] = {};
-  for (int p = 0; p < parts; ++p) {
-    const float4* src = reinterpret_cast<const float4*>(partial + p * size + i);
+  for (int share = first; share <= last; ++share) {
+    // (a share without stages of its own, when there are fewer stages than shares, wrote nothing)
+    if (share_begin(total, share, a.shares) == share_begin(total, share + 1, a.shares)) continue;
+    const float4* src = reinterpret_cast<const float4*>(partial + int64_t(share + adapter) * a.size[problem] + i);
     const float4 x = src[0], y = src[1];
     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
     v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
   }
-  *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                  pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  *reinterpret_cast<uint4*>(a.out[problem] + adapter * a.size[problem] + i) =
+      make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
 // ---------------------------------------------------------------------------
@@ -908,10 +1190,11 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   a.err = err;
   // Units of a span: those with which the block that has most to do is done
   // first.  A unit costs its chunks and the time of about two more until its h
-  // is in TMEM.
+  // is in TMEM; blocks that are as good as equal still end up to one unit apart.
   double best = 0.0;
   for (int64_t split = 1; split <= a.chunks; ++split) {
-    const double time = double(cdiv(busy_spans(r) * split, 2 * sms)) * (double(cdiv(a.chunks, split)) + 2.0);
+    const double time =
+        (double(cdiv(busy_spans(r) * split, 2 * sms)) + 0.5) * (double(cdiv(a.chunks, split)) + 2.0);
     if (split == 1 || time < best * 0.98) { best = time; a.split = int(split); }
   }
   const int64_t units = span_count(r) * a.split;
@@ -931,23 +1214,82 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   return cudaLaunchKernelEx(&cfg, up_kernel<MN>, maps, a);
 }
 
-// Shares of an adapter's rows.  A block takes an SM for itself, so the shares
-// are those, of 1 to 3 waves, that leave the fewest SMs idle in the last one if
-// the adapters' rows are alike (at 40 column blocks 8 shares, a little more than
-// two waves, took 88 us where 7 take 64 us).
-int grad_parts(const Rows& r, int64_t blocks, int sms) {
-  const int64_t adapters = r.adapters < r.requests ? r.adapters : r.requests;
-  const int64_t each = blocks * adapters, most = cdiv(r.m, 4 * kGradRows * adapters);
+// The kernels for at most kFewMost rows.
+unsigned few_spans(const Rows& r) {
+  const int64_t spans = cdiv(r.m, kFewRows) + r.requests + 1;
+  return unsigned(spans < r.m ? spans : r.m);  // every span has a row
+}
+
+FewArgs few_args(const Rows& r, int rank, __nv_bfloat16* h, const void* w) {
+  FewArgs a{};
+  a.rows = r;
+  a.rank = rank;
+  a.rp = int(cdiv(rank, 16)) * 16;
+  a.h = h;
+  a.w = static_cast<const __nv_bfloat16*>(w);
+  return a;
+}
+
+cudaError_t down_few(cudaStream_t st, const Rows& r, Matrix x, int64_t k, const void* w, int rank, __nv_bfloat16* h) {
+  FewArgs a = few_args(r, rank, h, w);
+  a.x = static_cast<const __nv_bfloat16*>(x.p);
+  a.ldx = x.ld;
+  a.k = k;
+  down_few_kernel<<<dim3(few_spans(r), unsigned(a.rp / kFewRanks)), 32 * kFewWarps, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t up_few(cudaStream_t st, const Rows& r, __nv_bfloat16* h, const void* w, int rank, int64_t n, Matrix y,
+                   Matrix out) {
+  FewArgs a = few_args(r, rank, h, w);
+  a.base = static_cast<const __nv_bfloat16*>(y.p);
+  a.out = static_cast<__nv_bfloat16*>(const_cast<void*>(out.p));
+  a.ldbase = y.ld;
+  a.ldo = out.ld;
+  a.cols = n;
+  a.in_place = y.p == out.p;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(cdiv(n, kFewCols)), few_spans(r));
+  cfg.blockDim = dim3(kFewCols);
+  cfg.dynamicSmemBytes = size_t(kFewCols) * size_t(rank / 8 + 1) * 16;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, up_few_kernel, a);
+}
+
+// h of x, the same wherever it is computed.
+cudaError_t down_a(cudaStream_t st, const Rows& r, Matrix x, int64_t k, const void* a, int rank, __nv_bfloat16* h,
+                   int sms, uint32_t* err) {
+  return r.m <= kFewMost ? down_few(st, r, x, k, a, rank, h) : down<false>(st, r, x, k, a, rank, h, sms, err);
+}
+
+int64_t grad_blocks(int64_t c, int rank) { return cdiv(c, grad_cols(rank <= 64 ? 1 : 2)); }
+
+// Shares of the rows, of 1 to 3 waves of blocks (a block takes an SM for
+// itself): those with the least time, counted in stages.  A block takes as long
+// as about six more to begin and to put its sums down, and every share is read
+// again by the second kernel.  (20 column blocks and 1024 stages: 7 shares take
+// 127 us, 22 take 146 us.)
+int grad_shares(int64_t m, int64_t blocks, int rank, int sms) {
+  const double stages = double(m) / double(grad_rows(rank <= 64 ? 1 : 2));
   int64_t best = 1;
-  double best_use = 0.0;
-  for (int64_t parts = 1; parts <= most && (parts == 1 || each * parts <= 3 * sms); ++parts) {
-    const double use = double(each * parts) / double(cdiv(each * parts, sms) * sms);
-    if (use > best_use * 1.02) { best = parts; best_use = use; }
+  double best_time = 0.0;
+  for (int64_t shares = 1; shares == 1 || (blocks * shares <= 3 * sms && double(shares) * 4.0 <= stages); ++shares) {
+    const double time =
+        double(cdiv(blocks * shares, sms)) * (stages / double(shares) + 6.0) + 0.5 * double(shares > 1 ? shares : 0);
+    if (shares == 1 || time < best_time) { best = shares; best_time = time; }
   }
   return int(best);
 }
 
-int64_t grad_blocks(int64_t c) { return cdiv(c, kGradCols); }
+size_t grad_partial_bytes(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int sms) {
+  const int64_t shares = grad_shares(m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, sms);
+  return shares > 1 ? size_t(shares + adapters) * size_t(rank) * size_t(k + n) * 4 : 0;
+}
 
 cudaError_t grad(cudaStream_t st, const Rows& r, int rank, Matrix x, int64_t k, Matrix dy, int64_t n,
                  const __nv_bfloat16* g, const __nv_bfloat16* h, void* da, void* db, void* workspace, int sms,
@@ -955,33 +1297,35 @@ cudaError_t grad(cudaStream_t st, const Rows& r, int rank, Matrix x, int64_t k, 
   GradMaps maps;
   GradArgs a{};
   const int rp = int(cdiv(rank, 16)) * 16;
-  if (!make_map(&maps.u[0], x.p, k, r.m, 1, x.ld, kGradRows) || !make_map(&maps.u[1], dy.p, n, r.m, 1, dy.ld, kGradRows) ||
-      !make_map(&maps.h[0], g, rp, r.m, 2, rp, kGradRows) || !make_map(&maps.h[1], h, rp, r.m, 2, rp, kGradRows))
+  a.atoms = rp <= 64 ? 1 : 2;
+  const int rows = grad_rows(a.atoms);
+  if (!make_map(&maps.u[0], x.p, k, r.m, 1, x.ld, rows) || !make_map(&maps.u[1], dy.p, n, r.m, 1, dy.ld, rows) ||
+      !make_map(&maps.h[0], g, rp, r.m, 2, rp, rows) || !make_map(&maps.h[1], h, rp, r.m, 2, rp, rows))
     return cudaErrorInvalidValue;
   a.rows = r;
   a.rank = rank;
-  a.atoms = rp <= 64 ? 1 : 2;
-  a.ring = ring_of(kGradU + 2 * a.atoms * 8192, 2 * kSmemTwo - 4096);
+  const int list = int(cdiv(r.adapters, 256)) * 1024;  // the adapters' stages in shared memory
+  a.ring = ring_of((grad_cols(a.atoms) / 64 + 2 * a.atoms) * rows * 128, 2 * kSmemTwo - 2048 - list);
   a.problem0 = da ? 0 : 1;
   a.cols[0] = k;
   a.cols[1] = n;
-  a.blocks[0] = grad_blocks(k);
-  a.blocks[1] = grad_blocks(n);
+  a.blocks[0] = grad_blocks(k, rank);
+  a.blocks[1] = grad_blocks(n, rank);
   const int64_t blocks = (da ? a.blocks[0] : 0) + (db ? a.blocks[1] : 0);
-  a.parts = grad_parts(r, grad_blocks(k) + grad_blocks(n), sms);
+  a.shares = grad_shares(r.m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, sms);
   a.partial = static_cast<float*>(workspace);
   a.out[0] = static_cast<__nv_bfloat16*>(da);
   a.out[1] = static_cast<__nv_bfloat16*>(db);
   a.err = err;
-  const int smem = a.ring.stages * a.ring.stage_bytes + 1024;
+  const int smem = a.ring.stages * a.ring.stage_bytes + list + 1024;
   cudaError_t e = allow_smem(grad_kernel, smem);
   if (e != cudaSuccess) return e;
-  grad_kernel<<<unsigned(blocks * a.parts * r.adapters), kThreads, smem, st>>>(maps, a);
+  grad_kernel<<<unsigned(blocks * a.shares), kThreads, smem, st>>>(maps, a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || a.parts == 1) return e;
-  const int64_t size0 = da ? r.adapters * rank * k : 0, size1 = db ? r.adapters * rank * n : 0;
-  grad_sum_kernel<<<unsigned(cdiv((size0 + size1) / 8, 256)), 256, 0, st>>>(a.partial, a.parts, size0, size1,
-                                                                          a.out[0], a.out[1]);
+  if (e != cudaSuccess) return e;
+  SumArgs sum{r, rows, a.shares, a.partial, {da ? rank * k : 0, db ? rank * n : 0}, {a.out[0], a.out[1]}};
+  const dim3 grid(unsigned(cdiv((sum.size[0] + sum.size[1]) / 8, 256)), unsigned(r.adapters));
+  grad_sum_kernel<<<grid, 256, 0, st>>>(sum);
   return cudaGetLastError();
 }
 
@@ -990,7 +1334,7 @@ bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) !
 int check(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int64_t requests) {
   if (m < 0 || k < 1 || n < 1 || adapters < 1 || requests < 0) return PASA_ERR_SHAPE;
   if (k % 8 || n % 8 || rank < 8 || rank > kMaxRank || rank % 8) return PASA_ERR_SHAPE;
-  if (m > (int64_t(1) << 30) || k > (1 << 24) || n > (1 << 24) || adapters > (1 << 20) || requests > (1 << 20))
+  if (m > (int64_t(1) << 30) || k > (1 << 24) || n > (1 << 24) || adapters > kMaxAdapters || requests > (1 << 20))
     return PASA_ERR_SHAPE;
   return PASA_OK;
 }
@@ -1042,8 +1386,10 @@ int pasa_lora_update(void* stream, const void* x, int64_t ldx, const void* y, in
   const Rows r{rows, slots, scale, int(requests), int(adapters), m};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   __nv_bfloat16* hh = static_cast<__nv_bfloat16*>(h);
-  cudaError_t e = down<false>(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
-  if (e == cudaSuccess) e = up<false>(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo}, sms, err);
+  cudaError_t e = down_a(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
+  if (e == cudaSuccess)
+    e = m <= kFewMost ? up_few(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo})
+                      : up<false>(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo}, sms, err);
   return e == cudaSuccess ? PASA_OK : PASA_ERR_CUDA;
 }
 
@@ -1057,10 +1403,7 @@ int pasa_lora_backward_workspace_size(int64_t m, int64_t k, int64_t n, int rank,
   if ((st = device_sms(&sms))) return st;
   size_t h = 0;
   pasa_lora_h_size(m, rank, &h);
-  const Rows r{nullptr, nullptr, nullptr, int(requests), int(adapters), m};
-  const int parts = m && requests ? grad_parts(r, grad_blocks(k) + grad_blocks(n), sms) : 1;
-  const size_t partial = parts > 1 ? size_t(parts) * size_t(adapters) * size_t(rank) * size_t(k + n) * 4 : 0;
-  *bytes = align256(h) + partial;
+  *bytes = align256(h) + (m && requests ? grad_partial_bytes(m, k, n, rank, adapters, sms) : 0);
   return PASA_OK;
 }
 
@@ -1099,7 +1442,7 @@ int pasa_lora_update_backward(void* stream, const void* dy, int64_t lddy, const 
   size_t h_bytes = 0;
   pasa_lora_h_size(m, rank, &h_bytes);
   cudaError_t e = cudaSuccess;
-  if (db && !h_given && requests) e = down<false>(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
+  if (db && !h_given && requests) e = down_a(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
   if (e == cudaSuccess && (dx || da)) e = down<true>(s, r, Matrix{dy, lddy}, n, b, rank, g, sms, err);
   if (e == cudaSuccess && dx)
     e = up<true>(s, r, g, a, rank, k, Matrix{dx_base, ldbase}, Matrix{dx, lddx}, sms, err);

@@ -66,8 +66,8 @@ class _Call:
         if self.k % 8 or self.n % 8 or self.rank % 8 or not 8 <= self.rank <= 128 or not self.k or not self.n:
             raise ValueError(f"the columns of x and y and the rank must be multiples of 8 and the rank 8 to 128, got "
                              f"{self.k}, {self.n} and {self.rank}")
-        if not self.adapters:
-            raise ValueError("there has to be an adapter")
+        if not 1 <= self.adapters <= 4096:
+            raise ValueError(f"1 to 4096 adapters, got {self.adapters}")
         self.requests = slots.shape[0]
         if rows.shape[0] != self.requests + 1:
             raise ValueError(f"rows must hold {self.requests + 1} offsets for {self.requests} requests, got "
@@ -178,7 +178,7 @@ def lora_update(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     and b: [S, N, R] bf16, the adapters; ``scale``: fp32 [S], or None for 1.  ``rows`` int32 [Q + 1] and ``slots``
     int32 [Q], both on the GPU and read there: request q owns the rows ``rows[q]`` to ``rows[q + 1]`` and the adapter
     ``slots[q]``, or none where that is outside [0, S).  ``rows`` must not decrease.  Rows of no request keep y.
-    K, N and R are multiples of 8, R at most 128 (smaller ranks: pad with zeros).
+    K, N and R are multiples of 8, R at most 128 (other ranks: pad with zeros), S at most 4096.
 
     Returns a new tensor like y, or ``out`` (``out=y`` updates in place); with ``return_h`` also the scaled x A^T that
     ``lora_update_backward`` takes.  Sums are fp32 and the result is rounded once.  Differentiable in y, x, a and b,

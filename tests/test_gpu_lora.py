@@ -92,6 +92,9 @@ CASES = {
     "long k, few rows": dict(lengths=[9, 2], k=13824, n=64, rank=32, adapters=2),
     "long n, few rows": dict(lengths=[9, 2], k=64, n=13824, rank=112, adapters=2),
     "many rows": dict(lengths=[20001, 13, 9000], k=136, n=320, rank=16, adapters=3),
+    "uneven adapters": dict(lengths=[3000, 1, 64, 9000, 31, 700, 2, 33], k=520, n=1048, rank=64, adapters=9,
+                            slots=[7, 0, 3, 7, 5, 2, 3, 8]),
+    "more adapters than rows": dict(lengths=[1, 2, 1], k=72, n=64, rank=8, adapters=300, slots=[299, 0, 150]),
     "requests and nothing in them": dict(lengths=[0, 0], k=64, n=64, rank=8, adapters=1, tail=5),
 }
 
