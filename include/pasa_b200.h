@@ -63,6 +63,8 @@ typedef enum pasa_attn_kernel {
 
 /* Bits a kernel may set in the caller's error word (see pasa_attn). */
 #define PASA_DEVERR_WAIT_TIMEOUT 0x1u  /* a bounded barrier wait gave up */
+#define PASA_DEVERR_BAD_PAGE 0x2u      /* a block table names a page that does not exist */
+#define PASA_DEVERR_BAD_SCALE 0x4u     /* a page's scale is not a power of two */
 
 /* ABI version of the loaded library (PASA_ABI_VERSION). */
 PASA_API int pasa_abi_version(void);
@@ -493,6 +495,52 @@ PASA_API int pasa_lora_update_backward(void* stream, const void* dy, int64_t ldd
               const void* a, const void* b, const float* scale, int64_t m, int64_t k, int64_t n, int rank,
               int64_t adapters, const int32_t* rows, const int32_t* slots, int64_t requests, void* h, int h_given,
               const void* dx_base, int64_t ldbase, void* dx, int64_t lddx, void* da, void* db,
+              void* workspace, size_t workspace_bytes);
+
+/*
+ * Keys and values in 8 bits: e4m3, in pages of 64 tokens with a power-of-two
+ * scale (fp32) for each page and head.
+ *   k_cache, v_cache  [pages, heads, 64, dim] e4m3, dense; heads are the
+ *                     key/value heads, dim is 64 or 128
+ *   k_scale, v_scale  [pages, heads]
+ *   table             device int32 [batch, width]: token i of request b is row
+ *                     i % 64 of page table[b][i / 64]
+ * A table entry outside [0, pages) that is needed is an error
+ * (PASA_DEVERR_BAD_PAGE in pasa_operator_errors): nothing is written to such a
+ * page, and the attention of such a request is undefined, but reads no memory
+ * outside of the cache.
+ *
+ * pasa_kv8_write rounds new tokens (k, v: bf16 [batch, heads, tokens, dim], the
+ * host arrays' strides of batch, head and token in elements, multiples of 8)
+ * into the pages behind each request's starts[b] tokens (device int32); only its
+ * first counts[b] ones if counts is not NULL.  A page's scale is the smallest
+ * power of two, 2^-100 at least, that brings its tokens to 448 or below; where
+ * the page has earlier tokens it does not become smaller, and they are rounded
+ * again to it.  Rows behind the last token keep what they hold.  A page that
+ * gets an infinity or NaN has the scale NaN.  No page may be written for two
+ * requests at once.
+ */
+PASA_API int pasa_kv8_write(void* stream, const void* k, const int64_t* k_stride, const void* v,
+              const int64_t* v_stride, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+              int64_t pages, int64_t heads, int dim, const int32_t* table, int64_t width,
+              const int32_t* starts, const int32_t* counts, int64_t batch, int64_t tokens);
+
+/*
+ * out = softmax(scale q k^T) v over each request's first lengths[b] tokens
+ * (device int32; cut at width * 64); zero for a request without tokens.
+ *   q, out  bf16 [batch, heads * group, queries, dim]; query head h reads
+ *           key/value head h / group.  Strides as above, 16-byte aligned.
+ *   scale   positive
+ *   workspace  pasa_kv8_attention_workspace_size bytes, not shared by two calls
+ *           that may run at the same time
+ * Probabilities and queries enter the products to 8 significant bits or 2^-16 of
+ * the row's largest, sums are fp32.
+ */
+PASA_API int pasa_kv8_attention_workspace_size(int dim, size_t* bytes);
+PASA_API int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, const void* k_cache,
+              const void* v_cache, const float* k_scale, const float* v_scale, int64_t pages, int64_t heads,
+              int dim, const int32_t* table, int64_t width, const int32_t* lengths, int64_t batch,
+              int64_t queries, int64_t group, float scale, void* out, const int64_t* out_stride,
               void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus

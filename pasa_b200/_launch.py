@@ -38,15 +38,20 @@ def launch(fn: str, device: torch.device, *args) -> None:
 
 
 def check_operator_errors(device=None) -> None:
-    """Raise if a kernel of ``lora_update`` or its gradient gave up a wait on ``device`` since the last call
-    (synchronises the current stream)."""
+    """Raise if a kernel of ``lora_update``, its gradient or the ``kv8`` operators reported an error on ``device``
+    since the last call: a wait that it gave up, or a block table or scale that cannot be (synchronises the current
+    stream)."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     flags = ctypes.c_uint32(0)
     with torch.cuda.device(index):
         _lib.check("pasa_operator_errors", _lib.load().pasa_operator_errors(
             torch.cuda.current_stream().cuda_stream, ctypes.byref(flags)))
-    if flags.value & _lib.DEVERR_WAIT_TIMEOUT:
-        raise RuntimeError(f"pasa_b200: a device-side barrier wait timed out (error word {flags.value:#x})")
+    reasons = [text for bit, text in ((_lib.DEVERR_WAIT_TIMEOUT, "a device-side barrier wait timed out"),
+                                      (_lib.DEVERR_BAD_PAGE, "a block table names a page that does not exist"),
+                                      (_lib.DEVERR_BAD_SCALE, "a page's scale is not a power of two"))
+               if flags.value & bit]
+    if reasons:
+        raise RuntimeError(f"pasa_b200: {', '.join(reasons)} (error word {flags.value:#x})")
 
 
 def wants_grad(fn: str, *tensors) -> bool:

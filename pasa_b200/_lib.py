@@ -32,6 +32,8 @@ ATTN_TCGEN05 = 1
 ATTN_SIMT = 2
 
 DEVERR_WAIT_TIMEOUT = 0x1
+DEVERR_BAD_PAGE = 0x2
+DEVERR_BAD_SCALE = 0x4
 
 O_BHTD = 0
 O_BTHD = 1
@@ -52,7 +54,8 @@ EXPORTS = (
     "pasa_peer_open", "pasa_peer_close", "pasa_dit_qkv_rope_scatter", "pasa_forward_scatter",
     "pasa_sample_mse_workspace_size", "pasa_sample_mse", "pasa_forward_range_workspace_size",
     "pasa_forward_range", "pasa_rope_axes", "pasa_operator_errors", "pasa_lora_h_size", "pasa_lora_update",
-    "pasa_lora_backward_workspace_size", "pasa_lora_update_backward",
+    "pasa_lora_backward_workspace_size", "pasa_lora_update_backward", "pasa_kv8_write",
+    "pasa_kv8_attention_workspace_size", "pasa_kv8_attention",
 )
 
 _lib = None
@@ -122,6 +125,11 @@ def load() -> ctypes.CDLL:
         "pasa_lora_update_backward": (c_int, [P, P, c_int64, P, c_int64, P, P, P, c_int64, c_int64, c_int64, c_int,
                                               c_int64, P, P, c_int64, P, c_int, P, c_int64, P, c_int64, P, P, P,
                                               c_size_t]),
+        "pasa_kv8_write": (c_int, [P, P, P, P, P, P, P, P, P, c_int64, c_int64, c_int, P, c_int64, P, P, c_int64,
+                                   c_int64]),
+        "pasa_kv8_attention_workspace_size": (c_int, [c_int, POINTER(c_size_t)]),
+        "pasa_kv8_attention": (c_int, [P, P, P, P, P, P, P, c_int64, c_int64, c_int, P, c_int64, P, c_int64, c_int64,
+                                       c_int64, c_float, P, P, P, c_size_t]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -693,7 +693,10 @@ __global__ void __launch_bounds__(kFewCols) up_few_kernel(const __grid_constant_
   __shared__ float h[kFewRows][kMaxRank];
   const int tid = threadIdx.x;
   const Span span = find_span<kFewRows>(a.rows, blockIdx.y, tid & 31);
-  if (span.count == 0 || (span.slot < 0 && a.in_place)) return;
+  if (span.count == 0 || (span.slot < 0 && a.in_place)) {
+    wait_for_predecessor();  // this grid does not end before the one that it depends on
+    return;
+  }
   const int64_t c0 = int64_t(blockIdx.x) * kFewCols, col = c0 + tid;
   const int vecs = a.rank / 8, pitch = vecs + 1;
   const int live = int(a.cols - c0 < kFewCols ? a.cols - c0 : kFewCols);

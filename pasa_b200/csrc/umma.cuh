@@ -30,7 +30,9 @@ template <int N> __device__ __forceinline__ void bulk_wait() {
 }
 
 // 32 lanes x 32 bit, 8 consecutive columns per thread (the first of v).
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[16]) {
+template <int N>
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[N]) {
+  static_assert(N >= 8, "8 columns");
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");

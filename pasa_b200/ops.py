@@ -445,5 +445,6 @@ def hunyuan_hidden_states_placement(hidden_states, hidden_states_out, best_mask_
 
 # operators with modules of their own
 from ._launch import check_operator_errors  # noqa: E402,F401
+from .kv8 import KV8Cache, kv8_attention, kv8_cache, kv8_write  # noqa: E402,F401
 from .lora import lora_update, lora_update_backward  # noqa: E402,F401
 from .rope import rope_axes  # noqa: E402,F401
