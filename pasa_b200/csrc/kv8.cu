@@ -182,19 +182,22 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_const
 constexpr int kTile = 128;          // rows of a tile
 constexpr int kStep = 128;          // tokens of a step: two pages
 constexpr int kSlotBytes = kStep * 128;
-constexpr int kSlots = 5;           // ring of keys' and values' steps
+constexpr int kMaxSlots = 5;        // ring of keys' and values' steps: 5, or 4 and room for the output on its way
 constexpr int kQTile = 2 * kTile * 128;  // hi, lo
 constexpr int kQBuf = 2 * kQTile;   // two tiles
 constexpr int kThreads = 512;       // 0 TMA, 1 MMA + TMEM, 2-3 and 12-15 queries, 4-7 and 8-11 softmax
 constexpr int kLoaders = 6;
 constexpr int kOverhead = 2;        // steps' time that a unit takes besides its steps
-constexpr float kLog2P = 6.f;       // probabilities are held times 2^6 ...
-constexpr float kRescale = 2.f;     // ... and their reference lags the maximum by up to 2^2: at most 2^8 < 448
+constexpr float kLog2P = 4.f;       // probabilities are held times 2^4 ...
+constexpr float kRescale = 4.f;     // ... and their reference lags the maximum by up to 2^4: at most 2^8 < 448
 constexpr int kOffQ = 0;                        // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes]
 constexpr int kOffRing = 2 * kQBuf;
-constexpr int kOffScale = kOffRing + kSlots * kSlotBytes;  // f32 [2 buffers][256 rows]: the queries' scales
+constexpr int kOffOut = kOffRing + 4 * kSlotBytes;        // [8 warps][32 rows][64 bytes]
+constexpr int kOffScale = kOffRing + kMaxSlots * kSlotBytes;  // f32 [2 buffers][256 rows]: the queries' scales
 constexpr int kSmem = kOffScale + 2 * 2 * kTile * 4 + 1024;
-constexpr uint32_t kColS = 0, kColO = 256;      // tile t at + 128 t; P over S
+// Tile t: scores at kColS + 128 t, the probabilities (hi, then lo, 32 columns
+// each) over the first 64 of them; output at kColO + 128 t.
+constexpr uint32_t kColS = 0, kColO = 256;
 static_assert(kSmem + 1024 <= 232448, "shared memory budget");
 
 struct Maps {
@@ -311,10 +314,21 @@ struct Walk {
   }
 };
 
-// Place in the ring of K and V of a piece's step j (of n): the order in which
-// the products need them.  Steps in turn: K0 K1 V0 K2 V1 K3 ...; else K0 V0 K1 V1 ...
-__device__ __forceinline__ int k_place(int j, int both) { return both ? (j < 2 ? j : 2 * j - 1) : 2 * j; }
-__device__ __forceinline__ int v_place(int j, int n, int both) { return both ? min(n, j + 2) + j : 2 * j + 1; }
+// A place in the ring of keys' and values' steps.  They lie there in the order in
+// which the products need them: where both tiles take every step K0 V0 K1 V1 ...,
+// where they take them in turn K0 K1 V0 K2 V1 K3 ...
+struct Cursor {
+  int at;
+  uint32_t parity;
+  __device__ __forceinline__ void next(int slots) {
+    if (++at == slots) { at = 0; parity ^= 1u; }
+  }
+  __device__ __forceinline__ void skip(int n, int slots) {
+    const int to = at + n;
+    at = to % slots;
+    parity ^= uint32_t(to / slots) & 1u;
+  }
+};
 
 // kind::f8f6f4: e4m3 operands, fp32 accumulator.
 __device__ __forceinline__ void mma8_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -380,22 +394,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kSlots], empty[kSlots], q_full[2], q_empty[2];
-  __shared__ uint64_t s_full[2], p_full[2], pv_done[2], o_free[2];
+  __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], o_free[2];
+  __shared__ uint64_t s_full[2], p_full[2][2], pv_done[2];  // of a tile; p_full: of a page of a step
   __shared__ uint32_t tmem_slot;
   float* q_scale = reinterpret_cast<float*>(sm + kOffScale);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int both = a.both;
+  const int both = a.both, slots = both ? kMaxSlots : 4;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kMaxSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], kLoaders);
       mbar_init(&q_empty[t], 1 + 8);  // the last product that reads it, and the softmax warps (its scales)
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&pv_done[t], 1);
       mbar_init(&o_free[t], 4);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t][0], 4);
+      mbar_init(&p_full[t][1], 4);
+      mbar_init(&pv_done[t], 1);
     }
     fence_barrier_init();
   }
@@ -411,189 +426,230 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     set_max_registers_down<56>();
     if (warp == 0) {
       // ================= keys and values =================
-      int base = 0;  // loads of the pieces before
+      Cursor c{0, 1};
+      int issued = 0;
       bool ok = true;
       while (ok && walk.next(a, lane, p)) {
-        if (p.count == 0) continue;
-        const int tokens = request_tokens(a, p.u.b);
-        for (int l = 0; l < 2 * p.count && ok; ++l) {
-          // load l: of which step, keys or values
-          int j, values;
-          if (!both) {
-            j = l >> 1;
-            values = l & 1;
-          } else if (l < min(p.count, 2)) {
-            j = l;
-            values = 0;
-          } else {  // V0 K2 V1 K3 ..., values alone once the keys are through
-            const int m = l - min(p.count, 2), pairs = max(p.count - 2, 0);
-            values = m < 2 * pairs ? !(m & 1) : 1;
-            j = m < 2 * pairs ? (m >> 1) + (values ? 0 : 2) : m - pairs;
+        const int n = p.count, ahead = both ? 2 : 1;
+        const int left = (request_tokens(a, p.u.b) + kPage - 1) / kPage - 2 * p.first;  // pages from the first step on
+        const int32_t* row = a.table + p.u.b * a.width + 2 * p.first;
+        int k_pages = 0, v_pages = 0;  // of 16 steps, a page a lane
+        for (int jk = 0, jv = 0; jv < n && ok;) {
+          // the next load: keys until they are `ahead` of the values, then in turn
+          const bool values = jk >= min(n, jv + ahead);
+          const int j = values ? jv++ : jk++;
+          if ((j & 15) == 0) {
+            int page = 2 * j + lane < left ? row[2 * j + lane] : 0;
+            if (page < 0 || page >= a.pages) {
+              if (2 * j + lane < 2 * n) atomicOr(a.err, PASA_DEVERR_BAD_PAGE);
+              page = 0;
+            }
+            if (values) v_pages = page;
+            else k_pages = page;
           }
-          const int slot = (base + l) % kSlots;
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[slot], uint32_t(((base + l) / kSlots) & 1) ^ 1u));
+          const int pages = values ? v_pages : k_pages, at = 2 * (j & 15);
+          const int z0 = __shfl_sync(0xffffffffu, pages, at) * a.heads + p.u.head;
+          const int z1 = __shfl_sync(0xffffffffu, pages, at + 1) * a.heads + p.u.head;
+          const bool second = 2 * j + 1 < left;
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[c.at], c.parity));
           if (!ok) break;
-          const int64_t index = int64_t(p.first + j) * 2;  // the step's first page
-          const int pages = (index + 1) * kPage < tokens ? 2 : 1;
-          int64_t page = lane < pages ? a.table[p.u.b * a.width + index + lane] : 0;
-          if (page < 0 || page >= a.pages) {
-            atomicOr(a.err, PASA_DEVERR_BAD_PAGE);
-            page = 0;
-          }
-          const int32_t z0 = int32_t(__shfl_sync(0xffffffffu, page, 0) * a.heads + p.u.head);
-          const int32_t z1 = int32_t(__shfl_sync(0xffffffffu, page, 1) * a.heads + p.u.head);
           if (elect_one()) {
-            unsigned char* dst = sm + kOffRing + slot * kSlotBytes;
+            unsigned char* dst = sm + kOffRing + c.at * kSlotBytes;
             const CUtensorMap* map = values ? &maps.v : &maps.k;
-            mbar_arrive_expect_tx(&full[slot], uint32_t(pages * kPage * 128));
-            tma_load_3d(dst, map, &full[slot], 0, 0, z0);
-            if (pages == 2) tma_load_3d(dst + kPage * 128, map, &full[slot], 0, 0, z1);
+            mbar_arrive_expect_tx(&full[c.at], second ? uint32_t(kSlotBytes) : uint32_t(kSlotBytes / 2));
+            tma_load_3d(dst, map, &full[c.at], 0, 0, z0);
+            if (second) tma_load_3d(dst + kSlotBytes / 2, map, &full[c.at], 0, 0, z1);
           }
           __syncwarp();
+          ++issued;
+          c.next(slots);
         }
-        if (ok) base += 2 * p.count;
       }
       if (!ok && lane == 0) report_operator_timeout(a.err);
-      for (int l = base > kSlots ? base - kSlots : 0; l < base && ok; ++l)
-        mbar_wait_bounded(&full[l % kSlots], uint32_t((l / kSlots) & 1));
+      // the copies in flight land before the block can end
+      for (int l = issued > slots ? issued - slots : 0; l < issued; ++l)
+        mbar_wait_bounded(&full[l % slots], uint32_t((l / slots) & 1));
     } else if (warp == 1) {
       // ================= products =================
-      const uint32_t id_s = idesc_e4m3(128, kStep, false), id_o = idesc_e4m3(128, D, true);
-      int base = 0, buf = 0;
-      uint32_t q_parity = 0, p_parity[2] = {0, 0}, o_parity[2] = {1, 1};
+      // One elected lane waits and issues: a wait by the whole warp, its vote and a new election around every product
+      // took 1000 clocks a product.
+      constexpr uint32_t id_s = idesc_e4m3(128, kStep, false), id_o = idesc_e4m3(128, D, true);
+      Cursor start{0, 0};
+      int buf = 0;
+      uint32_t q_parity = 0, p_parity = 0, o_parity = 3;  // p_parity, o_parity: bit t
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
-      };
+      const uint64_t desc = umma_desc_sw128(smem_u32(sm), 16, 1024);  // of the start of shared memory
       while (ok && walk.next(a, lane, p)) {
         if (p.count == 0) continue;
         const int n = p.count;
-        const int last_valid = request_tokens(a, p.u.b) - (p.first + n - 1) * kStep;  // tokens of the piece's last step
+        const int last_valid = request_tokens(a, p.u.b) - (p.first + n - 1) * kStep;  // tokens of the last step
         const int tiles = both ? min(n, 2) : (p.u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
-        const uint32_t q_base = smem_u32(sm + kOffQ + buf * kQBuf);
-        wait(&q_full[buf], q_parity);
-        // scores of tile t and step j
-        auto scores = [&](int t, int j) {
-          const int l = base + k_place(j, both);
-          wait(&full[l % kSlots], uint32_t((l / kSlots) & 1));
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          if (ok) ok = mbar_wait_bounded(bar, parity);
+        };
+        // scores of tile t with the keys in `slot`
+        auto scores = [&](int t, int slot, bool frees_keys, bool frees_queries) {
           if (!ok) return;
           tc_fence_after();
-          if (elect_one()) {
-            const uint64_t qd = umma_desc_sw128(q_base + uint32_t(both ? 0 : t) * kQTile, 16, 1024);
-            const uint64_t kd = umma_desc_sw128(smem_u32(sm + kOffRing + l % kSlots * kSlotBytes), 16, 1024);
+          const uint64_t qd = desc + uint64_t((kOffQ + buf * kQBuf + (both ? 0 : t) * kQTile) >> 4);
+          const uint64_t kd = desc + uint64_t((kOffRing + slot * kSlotBytes) >> 4);
+          const uint32_t d = tmem + kColS + uint32_t(128 * t);
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int kk = 0; kk < D / 32; ++kk)
-                mma8_ss(tmem + kColS + 128u * uint32_t(t), qd + uint64_t((x * kTile * 128 + kk * 32) >> 4),
-                        kd + uint64_t((kk * 32) >> 4), id_s, x > 0 || kk > 0 ? 1u : 0u);
-            tc_commit(&s_full[t]);
-            if (both || t == tiles - 1) tc_commit(&empty[l % kSlots]);
-            if (j == n - 1 && (both || t == tiles - 1)) tc_commit(&q_empty[buf]);
-          }
-          __syncwarp();
+            for (int kk = 0; kk < D / 32; ++kk)
+              mma8_ss(d, qd + uint64_t((x * kTile * 128 + kk * 32) >> 4), kd + uint64_t((kk * 32) >> 4), id_s,
+                      x > 0 || kk > 0 ? 1u : 0u);
+          tc_commit(&s_full[t]);
+          if (frees_keys) tc_commit(&empty[slot]);
+          if (frees_queries) tc_commit(&q_empty[buf]);
         };
-        // output of tile t += probabilities of step j times its values
-        auto output = [&](int t, int j, bool first) {
-          const int l = base + v_place(j, n, both);
-          wait(&full[l % kSlots], uint32_t((l / kSlots) & 1));
+        // output of tile t += probabilities times the values in `slot`, a page as soon as its probabilities are there
+        auto output = [&](int t, int slot, bool first, bool frees_values) {
           if (first) {
-            wait(&o_free[t], o_parity[t]);
-            o_parity[t] ^= 1u;
+            wait(&o_free[t], (o_parity >> t) & 1u);
+            o_parity ^= 1u << t;
           }
-          if (!ok) return;
-          unsigned char* vs = sm + kOffRing + l % kSlots * kSlotBytes;
-          if (j == n - 1 && last_valid < kStep && (both || t == 0)) {
-            // what lies behind the last token is no value: it may be a NaN's bits, and 0 * NaN is NaN
-            for (int i = lane; i < (kStep - last_valid) * 8; i += 32)
-              *reinterpret_cast<uint4*>(vs + last_valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-            fence_proxy_async();
-            __syncwarp();
-          }
-          wait(&p_full[t], p_parity[t]);
-          p_parity[t] ^= 1u;
-          if (!ok) return;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t vd = umma_desc_sw128(smem_u32(vs), 16, 1024);
+          const uint64_t vd = desc + uint64_t((kOffRing + slot * kSlotBytes) >> 4);
+          const uint32_t d = tmem + kColO + uint32_t(128 * t), pt = tmem + kColS + uint32_t(128 * t);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            wait(&p_full[t][h], (p_parity >> t) & 1u);
+            if (!ok) return;
+            tc_fence_after();
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int kk = 0; kk < kStep / 32; ++kk)
-                mma8_ts(tmem + kColO + 128u * uint32_t(t), tmem + kColS + 128u * uint32_t(t) + uint32_t(x * 32 + kk * 8),
-                        vd + uint64_t((kk * 4096) >> 4), id_o, !first || x > 0 || kk > 0 ? 1u : 0u);
-            tc_commit(&pv_done[t]);
-            if (both || t == tiles - 1) tc_commit(&empty[l % kSlots]);
+              for (int kk = 0; kk < 2; ++kk)
+                mma8_ts(d, pt + uint32_t(x * 32 + h * 16 + kk * 8), vd + uint64_t((h * 8192 + kk * 4096) >> 4), id_o,
+                        !first || h > 0 || x > 0 || kk > 0 ? 1u : 0u);
           }
-          __syncwarp();
+          p_parity ^= 1u << t;
+          tc_commit(&pv_done[t]);
+          if (frees_values) tc_commit(&empty[slot]);
         };
-        if (both) {
-          for (int j = 0; j < tiles; ++j) scores(j, j);
-          for (int j = 0; j < n && ok; ++j) {
-            output(j & 1, j, j < 2);
-            if (j + 2 < n) scores(j & 1, j + 2);
-          }
-        } else {
-          for (int t = 0; t < tiles; ++t) scores(t, 0);
-          for (int j = 0; j < n && ok; ++j)
-            for (int t = 0; t < tiles; ++t) {
-              output(t, j, j == 0);
-              if (j + 1 < n) scores(t, j + 1);
+        if (elect_one()) {
+          Cursor c = start;
+          wait(&q_full[buf], q_parity);
+          // all but the last step's output
+          if (both) {
+            for (int j = 0; j < tiles; ++j, c.next(slots)) {
+              wait(&full[c.at], c.parity);
+              scores(j, c.at, true, j == n - 1);
             }
+            for (int j = 0; j < n - 1 && ok; ++j) {
+              wait(&full[c.at], c.parity);
+              output(j & 1, c.at, j < 2, true);
+              c.next(slots);
+              if (j + 2 < n) {
+                wait(&full[c.at], c.parity);
+                scores(j & 1, c.at, true, j + 2 == n - 1);
+                c.next(slots);
+              }
+            }
+          } else {
+            wait(&full[c.at], c.parity);
+            for (int t = 0; t < tiles; ++t) scores(t, c.at, t == tiles - 1, n == 1 && t == tiles - 1);
+            c.next(slots);
+            for (int j = 0; j < n - 1 && ok; ++j) {
+              const int values = c.at;
+              wait(&full[c.at], c.parity);
+              c.next(slots);
+              output(0, values, j == 0, tiles == 1);
+              wait(&full[c.at], c.parity);
+              scores(0, c.at, tiles == 1, tiles == 1 && j == n - 2);
+              if (tiles == 2) {
+                output(1, values, j == 0, true);
+                scores(1, c.at, true, j == n - 2);
+              }
+              c.next(slots);
+            }
+          }
         }
-        base += 2 * n;
+        __syncwarp();
+        start.skip(2 * n - 1, slots);
+        if (last_valid < kStep) {
+          // what lies behind the last token is no value: it may be a NaN's bits, and 0 * NaN is NaN
+          mbar_wait_bounded(&full[start.at], start.parity);
+          unsigned char* vs = sm + kOffRing + start.at * kSlotBytes;
+          for (int i = lane; i < (kStep - last_valid) * 8; i += 32)
+            *reinterpret_cast<uint4*>(vs + last_valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (elect_one()) {
+          wait(&full[start.at], start.parity);
+          if (both) {
+            output((n - 1) & 1, start.at, n <= 2, true);
+          } else {
+            for (int t = 0; t < tiles; ++t) output(t, start.at, n == 1, t == tiles - 1);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);  // the elected lane's, the others' is true
+        start.skip(1, slots);
         if ((buf ^= 1) == 0) q_parity ^= 1u;
       }
       if (!ok && lane == 0) report_operator_timeout(a.err);
     } else {
       // ================= queries =================
-      // half a warp a row: its largest value, its scale, hi and lo
+      // four lanes a row, eight rows a warp: the row's largest value, its scale, hi and lo
       const int loader = warp < 4 ? warp - 2 : warp - 10;
-      const int half = lane >> 4, c = (lane & 15) * 8;
+      const int sub = lane >> 2, part = lane & 3;
+      constexpr int kVecs = D / 32;  // 16-byte vectors of a lane: part + 4 i
       int buf = 0;
       uint32_t parity = 1;
       bool ok = true;
       while (ok && walk.next(a, lane, p)) {
         if (p.count == 0) continue;
+        const int r0 = p.u.block * 2 * kTile, live = min(a.rows - r0, both ? kTile : 2 * kTile);
+        unsigned char* qs = sm + kOffQ + buf * kQBuf;
+        Bf8 v[kVecs];
+        auto load = [&](int row) {
+          if (row >= live) return;
+          const __nv_bfloat16* src = a.q + row_offset(a, a.qs, p.u, r0 + row) + part * 8;
+#pragma unroll
+          for (int i = 0; i < kVecs; ++i) v[i].r = *reinterpret_cast<const uint4*>(src + 32 * i);
+        };
+        load(loader * 8 + sub);  // the first rows are on their way while the buffer is still in use
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_empty[buf], parity));
         if (!ok) break;
-        const int r0 = p.u.block * 2 * kTile, live = min(a.rows - r0, both ? kTile : 2 * kTile);
-        const int padded = (live + kTile - 1) / kTile * kTile;
-        unsigned char* qs = sm + kOffQ + buf * kQBuf;
-        constexpr int kBatch = 4;
-        for (int row0 = loader * 2; row0 < padded; row0 += kLoaders * 2 * kBatch) {
-          Bf8 v[kBatch];
+        for (int row8 = loader * 8; row8 < live; row8 += kLoaders * 8) {
+          const int row = row8 + sub;
+          uint4 now[kVecs];
+          uint32_t amax = 0;
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int row = row0 + i * kLoaders * 2 + half;
-            v[i].r = make_uint4(0u, 0u, 0u, 0u);
-            if (row < live && c < D)
-              v[i].r = *reinterpret_cast<const uint4*>(a.q + row_offset(a, a.qs, p.u, r0 + row) + c);
+          for (int i = 0; i < kVecs; ++i) {
+            now[i] = v[i].r;
+            amax = max(amax, v[i].amax());
           }
+          load(row + kLoaders * 8);
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          if (row >= live) continue;  // (what the rows behind the last hold makes only rows that are not kept)
+          const float scale = scale_of(amax), inv = inverse(scale);
+          unsigned char* at = qs + (row / kTile) * kQTile + (row % kTile) * 128;
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int row = row0 + i * kLoaders * 2 + half;
-            uint32_t amax = v[i].amax();
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-            if (row >= padded) continue;
-            const float scale = scale_of(amax), inv = inverse(scale);
+          for (int i = 0; i < kVecs; ++i) {
+            const uint32_t in[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
             uint16_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = v[i][2 * e] * inv, y = v[i][2 * e + 1] * inv;
-              hi[e] = to_e4m3x2(x, y);
-              const float2 h = unpack_e4m3x2(hi[e]);
-              lo[e] = to_e4m3x2(x - h.x, y - h.y);
+            for (int e = 0; e < 4; ++e) {  // exact in fp16: 8 significant bits, 448 at most
+              const __half2 x = __floats2half2_rn(__uint_as_float(in[e] << 16) * inv,
+                                                  __uint_as_float(in[e] & 0xFFFF0000u) * inv);
+              hi[e] = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&x));
+              const uint32_t h = e4m3x2_to_f16x2(hi[e]);
+              const __half2 rest = __hsub2(x, *reinterpret_cast<const __half2*>(&h));
+              lo[e] = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&rest));
             }
             // byte c of the row, 16-byte pieces swizzled by the row
-            unsigned char* at = qs + (row / kTile) * kQTile + (row % kTile) * 128 + (((c >> 4) ^ (row & 7)) << 4) + (c & 15);
-            *reinterpret_cast<uint2*>(at) =
+            const int c = part * 8 + 32 * i;
+            unsigned char* dst = at + (((c >> 4) ^ (row & 7)) << 4) + (c & 15);
+            *reinterpret_cast<uint2*>(dst) =
                 make_uint2(uint32_t(hi[0]) | uint32_t(hi[1]) << 16, uint32_t(hi[2]) | uint32_t(hi[3]) << 16);
-            *reinterpret_cast<uint2*>(at + kTile * 128) =
+            *reinterpret_cast<uint2*>(dst + kTile * 128) =
                 make_uint2(uint32_t(lo[0]) | uint32_t(lo[1]) << 16, uint32_t(lo[2]) | uint32_t(lo[3]) << 16);
-            if ((lane & 15) == 0) q_scale[buf * 2 * kTile + row] = scale;
           }
+          if (part == 0) q_scale[buf * 2 * kTile + row] = scale;
         }
         fence_proxy_async();
         __syncwarp();
@@ -609,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const uint32_t lanes = uint32_t(w * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + kColS + 128u * uint32_t(t), o_tmem = tmem + lanes + kColO + 128u * uint32_t(t);
     int buf = 0;
-    uint32_t q_parity = 0, s_parity = 0, pv_parity = 0;
+    uint32_t q_parity = 0, k_parity = 0;  // k_parity: of the tile's next step
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       if (ok && !mbar_wait_bounded(bar, parity)) {
@@ -618,8 +674,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       }
     };
     while (walk.next(a, lane, p)) {
-      const int r = p.u.block * 2 * kTile + (both ? 0 : t * kTile) + row;  // the row of the key/value head
-      const bool live = r < a.rows;
+      const int r0 = p.u.block * 2 * kTile + (both ? 0 : t * kTile);
+      const int r = r0 + row;  // the row of the key/value head
+      const bool live = r < a.rows, warp_live = r0 + w * 32 < a.rows;
       if (p.zero) {
         if (live && !(both && t == 1)) {
           __nv_bfloat16* out = a.out + row_offset(a, a.os, p.u, r);
@@ -631,40 +688,48 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const int n = p.count, tokens = request_tokens(a, p.u.b);
       const int tiles = both ? min(n, 2) : (p.u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
       wait(&q_full[buf], q_parity);
-      const float q_row = q_scale[buf * 2 * kTile + (both ? 0 : t * kTile) + row];
+      const float q_row = q_scale[buf * 2 * kTile + (both ? 0 : t * kTile) + row] * a.scale_log2;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[buf]);
       if ((buf ^= 1) == 0) q_parity ^= 1u;
-      float m = -INFINITY, l = 0.f, v_ref = -1000.f;  // reference of the exponents; denominator; largest value scale
+      // References (log2): m of the probabilities in the denominator l, v_ref of the values' scales; the output's is
+      // m + v_ref.  They are a row's own.
+      float m = -INFINITY, l = 0.f, v_ref = 0.f;
       const int stride = both ? 2 : 1, begin = both ? t : 0;
       if (t < tiles) {
-        int number[2];
         PageScale next[2];
+        int number[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           next[h] = page_scale(a, p.u, page_number(a, p.u, tokens, int64_t(p.first + begin) * 2 + h));
           number[h] = page_number(a, p.u, tokens, int64_t(p.first + begin + stride) * 2 + h);
         }
-        for (int j = begin; j < n; j += stride) {
+        for (int j = begin; j < n; j += stride, k_parity ^= 1u) {
           const PageScale page[2] = {next[0], next[1]};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             next[h] = page_scale(a, p.u, number[h]);
             number[h] = page_number(a, p.u, tokens, int64_t(p.first + j + 2 * stride) * 2 + h);
           }
-          float c[2], v_log2[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            c[h] = q_row * page[h].k * a.scale_log2;
-            if (c[h] < 1e-37f) c[h] = 1e-37f;  // -infinity times it stays that; a NaN stays NaN
-            v_log2[h] = scale_log2(a, page[h].v);
+          wait(&s_full[t], k_parity);
+          if (!warp_live) {  // (its rows' probabilities are whatever the scores' bits are: they make rows not kept)
+            if (lane == 0) {
+              mbar_arrive(&p_full[t][0]);
+              mbar_arrive(&p_full[t][1]);
+            }
+            continue;
           }
-          wait(&s_full[t], s_parity);
-          s_parity ^= 1u;
           tc_fence_after();
           uint32_t s[4][32];
 #pragma unroll
           for (int i = 0; i < 4; ++i) tmem_ld32(s_tmem + 32u * uint32_t(i), s[i]);
+          float c[2], v_log2[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            c[h] = q_row * page[h].k;
+            if (c[h] < 1e-37f) c[h] = 1e-37f;  // -infinity times it stays that; a NaN stays NaN
+            v_log2[h] = scale_log2(a, page[h].v);
+          }
           tmem_wait_ld();
           const int valid = tokens - (p.first + j) * kStep;
           if (valid < kStep) {
@@ -672,36 +737,40 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             for (int i = 0; i < 128; ++i)
               if (i >= valid) s[i >> 5][i & 31] = 0xFF800000u;
           }
-          float top = fmaxf(fmaxf(max_tree32(s[0]), max_tree32(s[1])) * c[0],
-                            valid > kPage ? fmaxf(max_tree32(s[2]), max_tree32(s[3])) * c[1] : -INFINITY);
-          // the references move: the maximum by more than 2^2, or a page's value scale above all before
-          const float v_new = fmaxf(v_ref, fmaxf(v_log2[0], v_log2[1]));
-          const bool moves = top > m + kRescale || v_new > v_ref;
-          const float m_new = top > m + kRescale ? top : m;
-          if (__any_sync(0xffffffffu, moves) && j > begin) {
-            const float factor = exp2_ftz(fmaxf(m - m_new, -200.f) + fmaxf(v_ref - v_new, -200.f));
-            wait(&pv_done[t], pv_parity ^ 1u);
-            tc_fence_after();
+          const float top0 = fmaxf(max_tree32(s[0]), max_tree32(s[1])) * c[0];
+          const float top1 = fmaxf(max_tree32(s[2]), max_tree32(s[3])) * c[1];
+          const float top = fmaxf(top0, top1), v_top = fmaxf(top0 + v_log2[0], top1 + v_log2[1]);
+          // the references move when a probability, or one times its value's scale, is more than 2^4 above them
+          const bool moves = top > m + kRescale || v_top > m + v_ref + kRescale;
+          if (__any_sync(0xffffffffu, moves)) {
+            const float m_new = moves ? fmaxf(m, top) : m;
+            const float v_new = moves ? (j > begin ? fmaxf(m + v_ref, v_top) : v_top) - m_new : v_ref;
+            if (j > begin) {
+              const float fall = exp2_ftz(fmaxf(m - m_new, -200.f));
+              const float factor = exp2_ftz(fmaxf((m + v_ref) - (m_new + v_new), -200.f));
+              wait(&pv_done[t], k_parity ^ 1u);
+              tc_fence_after();
 #pragma unroll 1
-            for (int i = 0; i < D / 16; ++i) {
-              uint32_t o[16];
-              tmem_ld16(o_tmem + 16u * uint32_t(i), o);
-              tmem_wait_ld();
+              for (int i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+                tmem_ld32(o_tmem + 32u * uint32_t(i), o);
+                tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-              tmem_st16(o_tmem + 16u * uint32_t(i), o);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                tmem_st32(o_tmem + 32u * uint32_t(i), o);
+              }
+              l *= fall;
             }
-            l *= exp2_ftz(fmaxf(m - m_new, -200.f));
+            m = m_new;
+            v_ref = v_new;
           }
-          m = m_new;
-          v_ref = v_new;
-          const float m_used = m == -INFINITY ? 0.f : m;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            // probabilities times the page's value scale over the reference; times 2^-60 at the least, which is
-            // nothing next to the reference's page
+            // probabilities times the page's value scale over the reference; times 2^-60 at the least, which is nothing
+            // next to what set the reference
             const float dv = v_log2[h] == v_log2[h] ? fmaxf(v_log2[h] - v_ref, -60.f) : v_log2[h];
-            const float2 mul = make_float2(c[h], c[h]), add = make_float2(dv + kLog2P - m_used, dv + kLog2P - m_used);
+            const float shift = dv + kLog2P - (m == -INFINITY ? 0.f : m);
+            const float2 mul = make_float2(c[h], c[h]), add = make_float2(shift, shift);
             float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
@@ -728,18 +797,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               tmem_st8(s_tmem + uint32_t(16 * h + 8 * g), hi);
               tmem_st8(s_tmem + uint32_t(32 + 16 * h + 8 * g), lo);
             }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t][h]);
             l += ((sum0.x + sum0.y) + (sum1.x + sum1.y)) * exp2_ftz(-dv - kLog2P);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
-          pv_parity ^= 1u;
         }
-        wait(&pv_done[t], pv_parity ^ 1u);  // the last step's output
+        wait(&pv_done[t], k_parity ^ 1u);  // the last step's output
         tc_fence_after();
       }
-      const float to_true = exp2_ftz(v_ref - kLog2P);  // the accumulator's unit
+      const float to_true = exp2f(v_ref - kLog2P);  // the accumulator's unit
       if (!p.whole) {
         // a part of the unit: sums, maximum and denominator for the second kernel
         const int64_t at = (int64_t(blockIdx.x) * 2 + p.part) * 2 * kTile + t * kTile + row;
@@ -809,24 +877,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           named_bar_sync(2, 256);  // the space may be written again
         }
       } else if (t < tiles) {
-        __nv_bfloat16* out = a.out + row_offset(a, a.os, p.u, live ? r : 0);
+        // through shared memory, 32 columns at a time: 4 lanes then write 64 bytes of a row
         const float f = to_true / l;
+        unsigned char* stage = sm + kOffOut + (warp - 4) * 2048;
+        int64_t at[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int rr = r0 + w * 32 + x * 8 + (lane >> 2);
+          at[x] = rr < a.rows ? row_offset(a, a.os, p.u, rr) + (lane & 3) * 8 : -1;
+        }
 #pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
           __syncwarp();
           tmem_ld32(o_tmem + 32u * uint32_t(i), o);
           tmem_wait_ld();
-          if (live) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const uint32_t* x = &o[8 * v];
-              *reinterpret_cast<uint4*>(out + 32 * i + 8 * v) =
-                  make_uint4(pack_bf16x2(__uint_as_float(x[0]) * f, __uint_as_float(x[1]) * f),
-                             pack_bf16x2(__uint_as_float(x[2]) * f, __uint_as_float(x[3]) * f),
-                             pack_bf16x2(__uint_as_float(x[4]) * f, __uint_as_float(x[5]) * f),
-                             pack_bf16x2(__uint_as_float(x[6]) * f, __uint_as_float(x[7]) * f));
-            }
+          for (int v = 0; v < 4; ++v) {
+            const uint32_t* x = &o[8 * v];
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(pack_bf16x2(__uint_as_float(x[0]) * f, __uint_as_float(x[1]) * f),
+                           pack_bf16x2(__uint_as_float(x[2]) * f, __uint_as_float(x[3]) * f),
+                           pack_bf16x2(__uint_as_float(x[4]) * f, __uint_as_float(x[5]) * f),
+                           pack_bf16x2(__uint_as_float(x[6]) * f, __uint_as_float(x[7]) * f));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int rr = x * 8 + (lane >> 2);
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+            if (at[x] >= 0) *reinterpret_cast<uint4*>(a.out + at[x] + 32 * i) = y;
           }
         }
       }
