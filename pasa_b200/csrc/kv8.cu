@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_const
 constexpr int kTile = 128;          // rows of a tile
 constexpr int kStep = 128;          // tokens of a step: two pages
 constexpr int kSlotBytes = kStep * 128;
-constexpr int kMaxSlots = 5;        // ring of keys' and values' steps: 5, or 4 and room for the output on its way
+constexpr int kMaxSlots = 4;        // ring of keys' and values' steps
 constexpr int kQTile = 2 * kTile * 128;  // hi, lo
 constexpr int kQBuf = 2 * kQTile;   // two tiles
 constexpr int kThreads = 512;       // 0 TMA, 1 MMA + TMEM, 2-3 and 12-15 queries, 4-7 and 8-11 softmax
@@ -192,8 +192,8 @@ constexpr float kLog2P = 4.f;       // probabilities are held times 2^4 ...
 constexpr float kRescale = 4.f;     // ... and their reference lags the maximum by up to 2^4: at most 2^8 < 448
 constexpr int kOffQ = 0;                        // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes]
 constexpr int kOffRing = 2 * kQBuf;
-constexpr int kOffOut = kOffRing + 4 * kSlotBytes;        // [8 warps][32 rows][64 bytes]
-constexpr int kOffScale = kOffRing + kMaxSlots * kSlotBytes;  // f32 [2 buffers][256 rows]: the queries' scales
+constexpr int kOffOut = kOffRing + kMaxSlots * kSlotBytes;   // [8 warps][32 rows][64 bytes]
+constexpr int kOffScale = kOffOut + 8 * 32 * 64;  // f32 [2 buffers][256 rows]: the queries' scales
 constexpr int kSmem = kOffScale + 2 * 2 * kTile * 4 + 1024;
 // Tile t: scores at kColS + 128 t, the probabilities (hi, then lo, 32 columns
 // each) over the first 64 of them; output at kColO + 128 t.
@@ -399,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   __shared__ uint32_t tmem_slot;
   float* q_scale = reinterpret_cast<float*>(sm + kOffScale);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int both = a.both, slots = both ? kMaxSlots : 4;
+  const int both = a.both;
+  constexpr int slots = kMaxSlots;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -713,6 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           }
           wait(&s_full[t], k_parity);
           if (!warp_live) {  // (its rows' probabilities are whatever the scores' bits are: they make rows not kept)
+            __syncwarp();  // a lane still in its wait could miss the phase that lane 0's arrivals let begin
             if (lane == 0) {
               mbar_arrive(&p_full[t][0]);
               mbar_arrive(&p_full[t][1]);

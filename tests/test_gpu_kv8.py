@@ -211,6 +211,20 @@ def test_long(cuda_device, lengths, heads, group, queries):
     check_attention(out, q, p)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,group,queries", [(4, 1, 1), (3, 5, 1), (2, 4, 9), (2, 1, 70), (1, 3, 40)])
+def test_many_short_requests(cuda_device, dim, heads, group, queries):
+    """Several units of few rows and steps for each block, of one step and of more in turn."""
+    lengths = [(37 * i) % 131 if i % 5 else (101 * i) % 700 for i in range(400)]
+    p = Pages(lengths, heads, dim).fill(spread=True)
+    q = randn(len(lengths), heads * group, queries, dim, seed=9)
+    out = ops.kv8_attention(q, p.cache, p.table, i32(lengths))
+    ops.check_operator_errors()
+    check_attention(out, q, p)
+    for _ in range(5):
+        assert torch.equal(out, ops.kv8_attention(q, p.cache, p.table, i32(lengths)))
+
+
 def test_sharp_and_wide_scores(cuda_device):
     """One token takes all; scores of some hundreds that grow along the tokens; q's elements far apart; zeros."""
     p = Pages([700], 1, 64).fill()
