@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_const
 constexpr int kTile = 128;          // rows of a tile
 constexpr int kStep = 128;          // tokens of a step: two pages
 constexpr int kSlotBytes = kStep * 128;
-constexpr int kMaxSlots = 4;        // ring of keys' and values' steps
+constexpr int kSlots = 4, kSlotsBoth = 8;  // ring of keys' and values' steps; more where a unit has 128 rows
+constexpr int kScaleSteps = 8;      // ring of the steps' scales: a step's stay until both its products are done
 constexpr int kQTile = 2 * kTile * 128;  // hi, lo
 constexpr int kQBuf = 2 * kQTile;   // two tiles
 constexpr int kThreads = 512;       // 0 TMA, 1 MMA + TMEM, 2-3 and 12-15 queries, 4-7 and 8-11 softmax
@@ -190,13 +191,13 @@ constexpr int kLoaders = 6;
 constexpr int kOverhead = 2;        // steps' time that a unit takes besides its steps
 constexpr float kLog2P = 4.f;       // probabilities are held times 2^4 ...
 constexpr float kRescale = 4.f;     // ... and their reference lags the maximum by up to 2^4: at most 2^8 < 448
-constexpr int kOffQ = 0;                        // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes]
-constexpr int kOffRing = 2 * kQBuf;
-constexpr int kOffOut = kOffRing + kMaxSlots * kSlotBytes;   // [8 warps][32 rows][64 bytes]
-constexpr int kOffScale = kOffOut + 8 * 32 * 64;  // f32 [2 buffers][256 rows]: the queries' scales
+constexpr int kOffQ = 0;                        // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes], then the ring
+constexpr int kOffOut = 2 * kQBuf + kSlots * kSlotBytes;  // the output on its way, 16 KB
+constexpr int kOffScale = kOffOut + 16384;      // f32 [2 buffers][256 rows]: the queries' scales
+static_assert(2 * kQTile + kSlotsBoth * kSlotBytes == kOffOut, "both layouts end there");
 constexpr int kSmem = kOffScale + 2 * 2 * kTile * 4 + 1024;
-// Tile t: scores at kColS + 128 t, the probabilities (hi, then lo, 32 columns
-// each) over the first 64 of them; output at kColO + 128 t.
+// Tile t: scores at kColS + 128 t, over them the probabilities (of 32 tokens: hi
+// in the first 8 columns of their scores, lo in the next 8); output at kColO + 128 t.
 constexpr uint32_t kColS = 0, kColO = 256;
 static_assert(kSmem + 1024 <= 232448, "shared memory budget");
 
@@ -213,8 +214,10 @@ struct Args {
   const int32_t* lengths;      // [batch]
   int64_t pages, width;
   int batch, heads, group;     // key/value heads; query heads of each
+  uint32_t group_magic;        // 2^32 / group + 1, rounded down; 0 for 1
   int rows, blocks;            // rows of a key/value head (queries x group); units of 256 of them
   int both;                    // 1: both tiles hold the same rows and take the steps in turn
+  int quarters;                // 1: so do the 4 warps of a tile, each with a quarter of a step's tokens
   float scale_log2;            // softmax scale * log2(e)
   float* part_o;               // [2 parts a CTA][256][D]
   float2* part_ml;             // [2 parts a CTA][256]: maximum, denominator
@@ -238,13 +241,19 @@ __device__ __forceinline__ int64_t total_ticks(const Args& a, int lane) {
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   return sum * a.heads * a.blocks;
 }
-__device__ __forceinline__ int64_t part_begin(int64_t total, int part, int parts) {
-  return total / parts * part + total % parts * part / parts;
-}
+// The line's parts: part c is [begin(c), begin(c + 1)).
+struct Parts {
+  int64_t total, each;
+  int rest, parts;
+  __device__ __forceinline__ Parts(int64_t total_, int parts_) : total(total_), each(total_ / parts_), parts(parts_) {
+    rest = int(total_ - each * parts_);
+  }
+  __device__ __forceinline__ int64_t begin(int c) const { return each * c + unsigned(rest * c) / unsigned(parts); }
+};
 
 struct Unit {
   int b, head, block;
-  int steps;       // of the request
+  int tokens, steps;  // of the request
   int64_t begin;   // first tick
 };
 
@@ -254,7 +263,7 @@ __device__ __forceinline__ Unit find_unit(const Args& a, int64_t tick, int lane)
   int64_t before = 0;
   for (int b0 = 0;; b0 += 32) {
     const int b = b0 + lane;
-    const int steps = b < a.batch ? request_steps(a, b) : 0;
+    const int tokens = b < a.batch ? request_tokens(a, b) : 0, steps = (tokens + kStep - 1) / kStep;
     const int64_t own = b < a.batch ? (steps + kOverhead) * units : 0;
     int64_t upto = own;
 #pragma unroll
@@ -267,16 +276,17 @@ __device__ __forceinline__ Unit find_unit(const Args& a, int64_t tick, int lane)
       const int src = __ffs(int(reached)) - 1;
       Unit u;
       u.b = b0 + src;
-      u.steps = __shfl_sync(0xffffffffu, steps, src);
+      u.tokens = __shfl_sync(0xffffffffu, tokens, src);
+      u.steps = (u.tokens + kStep - 1) / kStep;
       const int64_t first = before + __shfl_sync(0xffffffffu, upto - own, src);
       const int64_t index = (tick - first) / (u.steps + kOverhead);
       u.begin = first + index * (u.steps + kOverhead);
-      u.head = int(index / a.blocks);
-      u.block = int(index % a.blocks);
+      u.block = int(index / a.heads);
+      u.head = int(index % a.heads);
       return u;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
-    if (b0 + 32 >= a.batch) return Unit{0, 0, 0, 0, before};  // (no unit: a tick behind the last)
+    if (b0 + 32 >= a.batch) return Unit{0, 0, 0, 0, 0, before};  // (no unit: a tick behind the last)
   }
 }
 
@@ -289,25 +299,38 @@ struct Piece {
   int part;          // 0 if it begins with the CTA's part of the line, else 1
 };
 
-// Goes through a CTA's part of the line of units.  Every warp has one of its own.
+// Goes through a CTA's part of the line of units.
 struct Walk {
   int64_t at, begin, end;
+  Unit u;
   __device__ __forceinline__ Walk(const Args& a, int lane) {
-    const int64_t total = total_ticks(a, lane);
-    begin = at = part_begin(total, int(blockIdx.x), int(gridDim.x));
-    end = part_begin(total, int(blockIdx.x) + 1, int(gridDim.x));
+    const Parts line(total_ticks(a, lane), int(gridDim.x));
+    begin = at = line.begin(int(blockIdx.x));
+    end = line.begin(int(blockIdx.x) + 1);
+    u = find_unit(a, at, lane);
   }
-  __device__ __forceinline__ bool next(const Args& a, int lane, Piece& p) {
+  __device__ __forceinline__ bool next(const Args& a, Piece& p) {
     while (at < end) {
-      p.u = find_unit(a, at, lane);
-      const int lo = int(at - p.u.begin), most = p.u.steps + kOverhead;
-      const int hi = end - p.u.begin < most ? int(end - p.u.begin) : most;
+      const int lo = int(at - u.begin), most = u.steps + kOverhead;
+      const int hi = end - u.begin < most ? int(end - u.begin) : most;
+      p.u = u;
       p.first = max(lo - kOverhead, 0);
       p.count = max(hi - kOverhead, 0) - p.first;
-      p.whole = p.first == 0 && p.count == p.u.steps;
-      p.zero = p.u.steps == 0 && lo == 0;
+      p.whole = p.first == 0 && p.count == u.steps;
+      p.zero = u.steps == 0 && lo == 0;
       p.part = at == begin ? 0 : 1;
-      at = p.u.begin + hi;
+      at = u.begin + hi;
+      if (at < end) {  // the next unit
+        u.begin = at;
+        if (++u.head == a.heads) {
+          u.head = 0;
+          if (++u.block == a.blocks) {
+            u.block = 0;
+            u.tokens = request_tokens(a, ++u.b);
+            u.steps = (u.tokens + kStep - 1) / kStep;
+          }
+        }
+      }
       if (p.count > 0 || p.zero) return true;
     }
     return false;
@@ -349,6 +372,14 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool b_mn_major)
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {  // all but the last N groups have landed
+  asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
+}
+
 template <int N> __device__ __forceinline__ void set_max_registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N));
 }
@@ -356,36 +387,50 @@ template <int N> __device__ __forceinline__ void set_max_registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N));
 }
 
-// Row r of a unit's (query, query head): its place in q or out.
-__device__ __forceinline__ int64_t row_offset(const Args& a, const int64_t (&s)[3], const Unit& u, int row) {
-  const int query = row / a.group, h = u.head * a.group + (row - query * a.group);
-  return u.b * s[0] + h * s[1] + query * s[2];
+// Row r of a unit's (query, query head): its place in q or out, from the unit's first.
+__device__ __forceinline__ int64_t unit_offset(const Args& a, const int64_t (&s)[3], const Unit& u) {
+  return u.b * s[0] + u.head * a.group * s[1];
+}
+__device__ __forceinline__ int64_t row_offset(const Args& a, const int64_t (&s)[3], int row) {
+  // row < 2^30, so the product is 1 too large at most
+  int query = a.group_magic ? int(__umulhi(uint32_t(row), a.group_magic)) : row;
+  if (query * int64_t(a.group) > row) --query;
+  return (row - query * a.group) * s[1] + query * s[2];
 }
 
-// A page's scales.  They are read a step before they are used, and the page's
-// number (-1: all tokens of the page are masked) a step before that.
-struct PageScale {
-  float k;
-  uint32_t v;
-};
-__device__ __forceinline__ int page_number(const Args& a, const Unit& u, int tokens, int64_t index) {
-  if (index * kPage >= tokens) return -1;
-  const int page = a.table[u.b * a.width + index];
-  return page < 0 || page >= a.pages ? 0 : page;  // (reported where the page is loaded)
-}
-__device__ __forceinline__ PageScale page_scale(const Args& a, const Unit& u, int page) {
-  // (masked: scores are -infinity whatever the scale, the values' is below any other)
-  if (page < 0) return PageScale{1.f, 0x00800000u};
-  const int64_t at = int64_t(page) * a.heads + u.head;
-  return PageScale{a.k_scale[at], __float_as_uint(a.v_scale[at])};
-}
 // The exponent of a values' scale; NaN for NaN, and for what is no power of two (an error).
-__device__ __forceinline__ float scale_log2(const Args& a, uint32_t v) {
+__device__ __forceinline__ float scale_log2(const Args& a, float scale) {
+  const uint32_t v = __float_as_uint(scale);
   if (v >= 0x7F800000u || (v & 0x7FFFFFu) || v == 0) {
     if (v != 0x7FC00000u) atomicOr(a.err, PASA_DEVERR_BAD_SCALE);
     return __uint_as_float(0x7FC00000u);
   }
   return float(int(v >> 23) - 127);
+}
+
+// 2^(x mul + shift) of 32 scores, as e4m3 terms hi + lo, and their sums.
+__device__ __forceinline__ void probabilities(const uint32_t (&s)[32], float mul_, float shift, uint32_t (&hi)[8],
+                                              uint32_t (&lo)[8], float2& sum0, float2& sum1) {
+  const float2 mul = make_float2(mul_, mul_), add = make_float2(shift, shift);
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    const uint32_t* x = &s[e];
+    float2 x01 = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), mul, add);
+    float2 x23 = __ffma2_rn(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), mul, add);
+    x01.x = exp2_ftz(x01.x); x01.y = exp2_ftz(x01.y);
+    x23.x = exp2_ftz(x23.x); x23.y = exp2_ftz(x23.y);
+    sum0 = __fadd2_rn(sum0, x01);
+    sum1 = __fadd2_rn(sum1, x23);
+    const __half2 p01 = __floats2half2_rn(x01.x, x01.y), p23 = __floats2half2_rn(x23.x, x23.y);
+    const uint16_t h01 = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&p01));
+    const uint16_t h23 = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&p23));
+    const uint32_t b01 = e4m3x2_to_f16x2(h01), b23 = e4m3x2_to_f16x2(h23);
+    const __half2 l01 = __hsub2(p01, *reinterpret_cast<const __half2*>(&b01));
+    const __half2 l23 = __hsub2(p23, *reinterpret_cast<const __half2*>(&b23));
+    hi[e >> 2] = uint32_t(h01) | uint32_t(h23) << 16;
+    lo[e >> 2] = uint32_t(f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&l01))) |
+                 uint32_t(f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&l23))) << 16;
+  }
 }
 
 template <int D>
@@ -394,16 +439,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], q_full[2], q_empty[2], o_free[2];
+  __shared__ uint64_t full[kSlotsBoth], empty[kSlotsBoth], q_full[2], q_empty[2], o_free[2];
   __shared__ uint64_t s_full[2], p_full[2][2], pv_done[2];  // of a tile; p_full: of a page of a step
   __shared__ uint32_t tmem_slot;
+  __shared__ float2 step_scale[kScaleSteps][2];  // of a step's two pages: the keys' scale, log2 of the values'
+  __shared__ float2 copy_ml[2 * kTile];          // maximum and denominator of every copy of a row
+  __shared__ uint64_t copies;
+  __shared__ Piece work[2];                      // what a buffer of queries is for; no steps: the end
   float* q_scale = reinterpret_cast<float*>(sm + kOffScale);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int both = a.both;
-  constexpr int slots = kMaxSlots;
+  const int both = a.both, slots = both ? kSlotsBoth : kSlots;
+  const int q_buf = both ? kQTile : kQBuf, ring = 2 * q_buf;  // bytes of a buffer of queries; the ring's place
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kMaxSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kSlotsBoth; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], kLoaders);
       mbar_init(&q_empty[t], 1 + 8);  // the last product that reads it, and the softmax warps (its scales)
@@ -413,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       mbar_init(&p_full[t][1], 4);
       mbar_init(&pv_done[t], 1);
     }
+    mbar_init(&copies, 8);
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
@@ -420,47 +470,73 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  Walk walk(a, lane);
-  Piece p;
 
   if (warp < 4 || warp >= 12) {
-    set_max_registers_down<56>();
+    set_max_registers_down<96>();
     if (warp == 0) {
       // ================= keys and values =================
+      Walk walk(a, lane);
+      auto next_steps = [&](Piece& x) {
+        while (walk.next(a, x))
+          if (x.count > 0) return true;
+        return false;
+      };
+      auto pages_left = [&](const Piece& x, int j) { return (x.u.tokens + kPage - 1) / kPage - 2 * (x.first + j); };
+      // the table's entry for this lane's page of 16 steps
+      auto entry = [&](const Piece& x, int j) {
+        return lane < pages_left(x, j) ? a.table[x.u.b * a.width + 2 * (x.first + j) + lane] : 0;
+      };
+      Piece p, after;
+      bool more = next_steps(p), ok = true;
+      int coming = more ? entry(p, 0) : 0;  // the entry for the next 16 steps of keys, read that much ahead
       Cursor c{0, 1};
-      int issued = 0;
-      bool ok = true;
-      while (ok && walk.next(a, lane, p)) {
+      int issued = 0, step = 0;  // step: of step_scale
+      for (bool more_after; more && ok; more = more_after, p = after) {
+        more_after = next_steps(after);
         const int n = p.count, ahead = both ? 2 : 1;
-        const int left = (request_tokens(a, p.u.b) + kPage - 1) / kPage - 2 * p.first;  // pages from the first step on
-        const int32_t* row = a.table + p.u.b * a.width + 2 * p.first;
         int k_pages = 0, v_pages = 0;  // of 16 steps, a page a lane
+        float2 scales = make_float2(1.f, 0.f);
         for (int jk = 0, jv = 0; jv < n && ok;) {
           // the next load: keys until they are `ahead` of the values, then in turn
           const bool values = jk >= min(n, jv + ahead);
           const int j = values ? jv++ : jk++;
           if ((j & 15) == 0) {
-            int page = 2 * j + lane < left ? row[2 * j + lane] : 0;
-            if (page < 0 || page >= a.pages) {
-              if (2 * j + lane < 2 * n) atomicOr(a.err, PASA_DEVERR_BAD_PAGE);
-              page = 0;
+            if (values) {
+              v_pages = k_pages;  // (the keys are less than 16 steps ahead)
+            } else {
+              const bool mine = lane < pages_left(p, j) && lane < 2 * (n - j);
+              const bool bad = coming < 0 || coming >= a.pages;
+              if (bad && mine) atomicOr(a.err, PASA_DEVERR_BAD_PAGE);
+              k_pages = bad ? 0 : coming;
+              // (a page behind the last token is masked: scores are -infinity whatever the scale, the values' is below any)
+              scales = make_float2(1.f, __uint_as_float(0x00800000u));
+              if (mine) {
+                const int64_t z = int64_t(k_pages) * a.heads + p.u.head;
+                scales = make_float2(a.k_scale[z], a.v_scale[z]);
+              }
+              coming = j + 16 < n ? entry(p, j + 16) : more_after ? entry(after, 0) : 0;
             }
-            if (values) v_pages = page;
-            else k_pages = page;
           }
           const int pages = values ? v_pages : k_pages, at = 2 * (j & 15);
           const int z0 = __shfl_sync(0xffffffffu, pages, at) * a.heads + p.u.head;
           const int z1 = __shfl_sync(0xffffffffu, pages, at + 1) * a.heads + p.u.head;
-          const bool second = 2 * j + 1 < left;
+          const bool second = pages_left(p, j) > 1;
           ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[c.at], c.parity));
           if (!ok) break;
           if (elect_one()) {
-            unsigned char* dst = sm + kOffRing + c.at * kSlotBytes;
+            unsigned char* dst = sm + ring + c.at * kSlotBytes;
             const CUtensorMap* map = values ? &maps.v : &maps.k;
-            mbar_arrive_expect_tx(&full[c.at], second ? uint32_t(kSlotBytes) : uint32_t(kSlotBytes / 2));
             tma_load_3d(dst, map, &full[c.at], 0, 0, z0);
             if (second) tma_load_3d(dst + kSlotBytes / 2, map, &full[c.at], 0, 0, z1);
           }
+          // the scales are on their way while the tiles are: what the barrier expects comes behind them
+          if (!values) {
+            if ((j & 15) == 0) scales.y = scale_log2(a, scales.y);
+            if ((lane >> 1) == (j & 15)) step_scale[step % kScaleSteps][lane & 1] = scales;
+            ++step;
+          }
+          __syncwarp();
+          if (elect_one()) mbar_arrive_expect_tx(&full[c.at], second ? uint32_t(kSlotBytes) : uint32_t(kSlotBytes / 2));
           __syncwarp();
           ++issued;
           c.next(slots);
@@ -480,11 +556,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       uint32_t q_parity = 0, p_parity = 0, o_parity = 3;  // p_parity, o_parity: bit t
       bool ok = true;
       const uint64_t desc = umma_desc_sw128(smem_u32(sm), 16, 1024);  // of the start of shared memory
-      while (ok && walk.next(a, lane, p)) {
-        if (p.count == 0) continue;
-        const int n = p.count;
-        const int last_valid = request_tokens(a, p.u.b) - (p.first + n - 1) * kStep;  // tokens of the last step
-        const int tiles = both ? min(n, 2) : (p.u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
+      for (;;) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(&q_full[buf], q_parity));
+        if (!ok) break;
+        const int n = work[buf].count;
+        if (n == 0) break;
+        const int last_valid = work[buf].u.tokens - (work[buf].first + n - 1) * kStep;  // tokens of the last step
+        const int tiles = both ? min(n, 2) : (work[buf].u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
+        __syncwarp();
         auto wait = [&](uint64_t* bar, uint32_t parity) {
           if (ok) ok = mbar_wait_bounded(bar, parity);
         };
@@ -492,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         auto scores = [&](int t, int slot, bool frees_keys, bool frees_queries) {
           if (!ok) return;
           tc_fence_after();
-          const uint64_t qd = desc + uint64_t((kOffQ + buf * kQBuf + (both ? 0 : t) * kQTile) >> 4);
-          const uint64_t kd = desc + uint64_t((kOffRing + slot * kSlotBytes) >> 4);
+          const uint64_t qd = desc + uint64_t((kOffQ + buf * q_buf + (both ? 0 : t) * kQTile) >> 4);
+          const uint64_t kd = desc + uint64_t((ring + slot * kSlotBytes) >> 4);
           const uint32_t d = tmem + kColS + uint32_t(128 * t);
 #pragma unroll
           for (int x = 0; x < 2; ++x)
@@ -511,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             wait(&o_free[t], (o_parity >> t) & 1u);
             o_parity ^= 1u << t;
           }
-          const uint64_t vd = desc + uint64_t((kOffRing + slot * kSlotBytes) >> 4);
+          const uint64_t vd = desc + uint64_t((ring + slot * kSlotBytes) >> 4);
           const uint32_t d = tmem + kColO + uint32_t(128 * t), pt = tmem + kColS + uint32_t(128 * t);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -522,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             for (int x = 0; x < 2; ++x)
 #pragma unroll
               for (int kk = 0; kk < 2; ++kk)
-                mma8_ts(d, pt + uint32_t(x * 32 + h * 16 + kk * 8), vd + uint64_t((h * 8192 + kk * 4096) >> 4), id_o,
+                mma8_ts(d, pt + uint32_t(h * 64 + kk * 32 + x * 8), vd + uint64_t((h * 8192 + kk * 4096) >> 4), id_o,
                         !first || h > 0 || x > 0 || kk > 0 ? 1u : 0u);
           }
           p_parity ^= 1u << t;
@@ -531,7 +610,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         };
         if (elect_one()) {
           Cursor c = start;
-          wait(&q_full[buf], q_parity);
           // all but the last step's output
           if (both) {
             for (int j = 0; j < tiles; ++j, c.next(slots)) {
@@ -572,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         if (last_valid < kStep) {
           // what lies behind the last token is no value: it may be a NaN's bits, and 0 * NaN is NaN
           mbar_wait_bounded(&full[start.at], start.parity);
-          unsigned char* vs = sm + kOffRing + start.at * kSlotBytes;
+          unsigned char* vs = sm + ring + start.at * kSlotBytes;
           for (int i = lane; i < (kStep - last_valid) * 8; i += 32)
             *reinterpret_cast<uint4*>(vs + last_valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
@@ -593,53 +671,89 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       if (!ok && lane == 0) report_operator_timeout(a.err);
     } else {
       // ================= queries =================
-      // four lanes a row, eight rows a warp: the row's largest value, its scale, hi and lo
+      // Four lanes a row, eight rows a warp at a time: the row's largest value, its scale, hi and lo.  The bf16 row has
+      // the size of its two e4m3 rows: it is copied to their place asynchronously, all rows of the buffer at once (48 in
+      // flight, through registers, took 20000 clocks a buffer), and split there.
       const int loader = warp < 4 ? warp - 2 : warp - 10;
       const int sub = lane >> 2, part = lane & 3;
       constexpr int kVecs = D / 32;  // 16-byte vectors of a lane: part + 4 i
+      constexpr int kRounds = (2 * kTile + 8 * kLoaders - 1) / (8 * kLoaders);
+      constexpr int kRowLanes = D / 8, kRowsAtOnce = 32 / kRowLanes;  // a copy's lanes in a row, its rows
+      Walk walk(a, lane);
+      Piece p{}, after{};
       int buf = 0;
       uint32_t parity = 1;
-      bool ok = true;
-      while (ok && walk.next(a, lane, p)) {
-        if (p.count == 0) continue;
-        const int r0 = p.u.block * 2 * kTile, live = min(a.rows - r0, both ? kTile : 2 * kTile);
-        unsigned char* qs = sm + kOffQ + buf * kQBuf;
-        Bf8 v[kVecs];
-        auto load = [&](int row) {
-          if (row >= live) return;
-          const __nv_bfloat16* src = a.q + row_offset(a, a.qs, p.u, r0 + row) + part * 8;
+      bool ok = true, more = walk.next(a, p);
+      for (bool last = false; !last; p = after) {
+        last = !more;
+        const bool here = more;
+        if (more) more = walk.next(a, after);
+        if (more) {  // the next piece's rows, on their way to L2 meanwhile
+          const int kept = min(a.rows - after.u.block * 2 * kTile, 2 * kTile);
+          const __nv_bfloat16* q = a.q + unit_offset(a, a.qs, after.u);
+          for (int row = loader * 32 + lane; row < kept; row += 32 * kLoaders) {
+            const __nv_bfloat16* src = q + row_offset(a, a.qs, after.u.block * 2 * kTile + row);
 #pragma unroll
-          for (int i = 0; i < kVecs; ++i) v[i].r = *reinterpret_cast<const uint4*>(src + 32 * i);
-        };
-        load(loader * 8 + sub);  // the first rows are on their way while the buffer is still in use
+            for (int i = 0; i < D; i += 64) asm volatile("prefetch.global.L2 [%0];" :: "l"(src + i));
+          }
+        }
+        const int r0 = p.u.block * 2 * kTile;
+        // rows of the buffer; with quarters every 32 of them are the same
+        const int mask = a.quarters ? 31 : 255, kept = min(a.rows - r0, 2 * kTile);
+        const int live = !here ? 0 : a.quarters ? kTile : kept;
+        if (here && p.zero) {
+          for (int row = loader * 8 + sub; row < kept; row += kLoaders * 8) {
+            __nv_bfloat16* dst = a.out + unit_offset(a, a.os, p.u) + row_offset(a, a.os, r0 + row) + part * 8;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) *reinterpret_cast<uint4*>(dst + 32 * i) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          continue;  // (a piece: not the last)
+        }
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_empty[buf], parity));
         if (!ok) break;
-        for (int row8 = loader * 8; row8 < live; row8 += kLoaders * 8) {
-          const int row = row8 + sub;
-          uint4 now[kVecs];
+        const __nv_bfloat16* q = a.q + unit_offset(a, a.qs, p.u) + lane % kRowLanes * 8;
+        unsigned char* qs = sm + kOffQ + buf * q_buf;
+        auto place = [&](int row) { return qs + (row / kTile) * kQTile + (row % kTile) * 128; };
+        // (what the rows behind the last hold makes only rows that are not kept)
+        auto has = [&](int row) { return row < live && (row & mask) < kept; };
+#pragma unroll 1
+        for (int x = 0; x < kRounds; ++x) {
+#pragma unroll
+          for (int i = 0; i < kVecs; ++i) {
+            const int row = x * 8 * kLoaders + loader * 8 + i * kRowsAtOnce + lane / kRowLanes, c = lane % kRowLanes;
+            if (has(row))  // the first 128 bytes lie in the row of hi, the others in that of lo
+              cp_async16(smem_u32(place(row)) + uint32_t((c & 7) * 16 + (c >> 3) * kTile * 128),
+                         q + row_offset(a, a.qs, r0 + (row & mask)));
+          }
+          cp_async_commit();
+        }
+        auto split = [&](int x) {
+          const int row = x * 8 * kLoaders + loader * 8 + sub;
+          if (x * 8 * kLoaders + loader * 8 >= live) return;
+          unsigned char* at = place(row < live ? row : x * 8 * kLoaders + loader * 8);
+          Bf8 v[kVecs];
           uint32_t amax = 0;
 #pragma unroll
           for (int i = 0; i < kVecs; ++i) {
-            now[i] = v[i].r;
+            v[i].r = *reinterpret_cast<const uint4*>(at + part * 16 + (i & 1) * 64 + (i >> 1) * kTile * 128);
             amax = max(amax, v[i].amax());
           }
-          load(row + kLoaders * 8);
           amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
           amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          if (row >= live) continue;  // (what the rows behind the last hold makes only rows that are not kept)
+          __syncwarp();  // all of a row is read before any of it is written
+          if (!has(row)) return;
           const float scale = scale_of(amax), inv = inverse(scale);
-          unsigned char* at = qs + (row / kTile) * kQTile + (row % kTile) * 128;
 #pragma unroll
           for (int i = 0; i < kVecs; ++i) {
-            const uint32_t in[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+            const uint32_t in[4] = {v[i].r.x, v[i].r.y, v[i].r.z, v[i].r.w};
             uint16_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // exact in fp16: 8 significant bits, 448 at most
-              const __half2 x = __floats2half2_rn(__uint_as_float(in[e] << 16) * inv,
+              const __half2 h = __floats2half2_rn(__uint_as_float(in[e] << 16) * inv,
                                                   __uint_as_float(in[e] & 0xFFFF0000u) * inv);
-              hi[e] = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&x));
-              const uint32_t h = e4m3x2_to_f16x2(hi[e]);
-              const __half2 rest = __hsub2(x, *reinterpret_cast<const __half2*>(&h));
+              hi[e] = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&h));
+              const uint32_t back = e4m3x2_to_f16x2(hi[e]);
+              const __half2 rest = __hsub2(h, *reinterpret_cast<const __half2*>(&back));
               lo[e] = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&rest));
             }
             // byte c of the row, 16-byte pieces swizzled by the row
@@ -651,6 +765,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 make_uint2(uint32_t(lo[0]) | uint32_t(lo[1]) << 16, uint32_t(lo[2]) | uint32_t(lo[3]) << 16);
           }
           if (part == 0) q_scale[buf * 2 * kTile + row] = scale;
+        };
+        static_assert(kRounds == 6, "the waits below");
+#pragma unroll 1
+        for (int x = 0; x < kRounds; ++x) {
+          if (x == 0) cp_async_wait<4>();
+          else if (x == 2) cp_async_wait<2>();
+          else if (x == 4) cp_async_wait<0>();
+          __syncwarp();
+          split(x);
+        }
+        if (loader == 0 && lane == 0) {
+          if (last) p.count = 0;
+          work[buf] = p;
         }
         fence_proxy_async();
         __syncwarp();
@@ -660,11 +787,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       if (!ok && lane == 0) report_operator_timeout(a.err);
     }
   } else {
-    set_max_registers_up<200>();
+    set_max_registers_up<160>();
     // ================= softmax of tile t: a thread a row =================
     const int t = (warp - 4) >> 2, w = warp & 3, row = w * 32 + lane;
     const uint32_t lanes = uint32_t(w * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + kColS + 128u * uint32_t(t), o_tmem = tmem + lanes + kColO + 128u * uint32_t(t);
+    const bool quarters = a.quarters;
     int buf = 0;
     uint32_t q_parity = 0, k_parity = 0;  // k_parity: of the tile's next step
     bool ok = true;
@@ -674,21 +802,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         report_operator_timeout(a.err);
       }
     };
-    while (walk.next(a, lane, p)) {
-      const int r0 = p.u.block * 2 * kTile + (both ? 0 : t * kTile);
-      const int r = r0 + row;  // the row of the key/value head
-      const bool live = r < a.rows, warp_live = r0 + w * 32 < a.rows;
-      if (p.zero) {
-        if (live && !(both && t == 1)) {
-          __nv_bfloat16* out = a.out + row_offset(a, a.os, p.u, r);
-#pragma unroll
-          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        continue;
-      }
-      const int n = p.count, tokens = request_tokens(a, p.u.b);
-      const int tiles = both ? min(n, 2) : (p.u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
+    uint32_t copies_parity = 0;
+    auto all_copies = [&] {  // a barrier of the 8 warps that ends
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&copies);
+      wait(&copies, copies_parity);
+      copies_parity ^= 1u;
+    };
+    for (int base = 0;;) {  // base: the piece's first step in step_scale
       wait(&q_full[buf], q_parity);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const Piece p = work[buf];
+      const int n = p.count, tokens = p.u.tokens;
+      if (n == 0) break;
+      const int r0 = p.u.block * 2 * kTile + (both ? 0 : t * kTile);
+      const int r = r0 + (quarters ? lane : row);  // the row of the key/value head
+      const bool live = r < a.rows, warp_live = quarters || r0 + w * 32 < a.rows;
+      const int tiles = both ? min(n, 2) : (p.u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
       const float q_row = q_scale[buf * 2 * kTile + (both ? 0 : t * kTile) + row] * a.scale_log2;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[buf]);
@@ -697,21 +827,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       // m + v_ref.  They are a row's own.
       float m = -INFINITY, l = 0.f, v_ref = 0.f;
       const int stride = both ? 2 : 1, begin = both ? t : 0;
-      if (t < tiles) {
-        PageScale next[2];
-        int number[2];
+      // The references move when a probability, or one times its value's scale, is more than 2^4 above them.
+      auto follow = [&](float top, float v_top, bool first) {
+        const bool moves = top > m + kRescale || v_top > m + v_ref + kRescale;
+        if (!__any_sync(0xffffffffu, moves)) return;
+        const float m_new = moves ? fmaxf(m, top) : m;
+        const float v_new = moves ? (first ? v_top : fmaxf(m + v_ref, v_top)) - m_new : v_ref;
+        if (!first) {
+          const float fall = exp2_ftz(fmaxf(m - m_new, -200.f));
+          const float factor = exp2_ftz(fmaxf((m + v_ref) - (m_new + v_new), -200.f));
+          wait(&pv_done[t], k_parity ^ 1u);
+          tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tmem_ld32(o_tmem + 32u * uint32_t(i), o);
+            tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          next[h] = page_scale(a, p.u, page_number(a, p.u, tokens, int64_t(p.first + begin) * 2 + h));
-          number[h] = page_number(a, p.u, tokens, int64_t(p.first + begin + stride) * 2 + h);
-        }
-        for (int j = begin; j < n; j += stride, k_parity ^= 1u) {
-          const PageScale page[2] = {next[0], next[1]};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            next[h] = page_scale(a, p.u, number[h]);
-            number[h] = page_number(a, p.u, tokens, int64_t(p.first + j + 2 * stride) * 2 + h);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st32(o_tmem + 32u * uint32_t(i), o);
           }
+          l *= fall;
+        }
+        m = m_new;
+        v_ref = v_new;
+      };
+      // log2 of a page's value scale over the reference; -60 at the least, which is nothing next to what set the reference
+      auto value_shift = [&](float v_log2) { return v_log2 == v_log2 ? fmaxf(v_log2 - v_ref, -60.f) : v_log2; };
+      if (t < tiles) {
+        for (int j = begin; j < n; j += stride, k_parity ^= 1u) {
           wait(&s_full[t], k_parity);
           if (!warp_live) {  // (its rows' probabilities are whatever the scores' bits are: they make rows not kept)
             __syncwarp();  // a lane still in its wait could miss the phase that lane 0's arrivals let begin
@@ -722,82 +866,82 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             continue;
           }
           tc_fence_after();
-          uint32_t s[4][32];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(s_tmem + 32u * uint32_t(i), s[i]);
-          float c[2], v_log2[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            c[h] = q_row * page[h].k;
-            if (c[h] < 1e-37f) c[h] = 1e-37f;  // -infinity times it stays that; a NaN stays NaN
-            v_log2[h] = scale_log2(a, page[h].v);
-          }
-          tmem_wait_ld();
+          const float2 page[2] = {step_scale[(base + j) % kScaleSteps][0], step_scale[(base + j) % kScaleSteps][1]};
           const int valid = tokens - (p.first + j) * kStep;
-          if (valid < kStep) {
+          auto score_scale = [&](int h) {
+            const float c = q_row * page[h].x;
+            return c < 1e-37f ? 1e-37f : c;  // -infinity times it stays that; a NaN stays NaN
+          };
+          if (quarters) {
+            uint32_t s[32];
+            tmem_ld32(s_tmem + 32u * uint32_t(w), s);
+            const float c = score_scale(w >> 1), v_log2 = page[w >> 1].y;
+            tmem_wait_ld();
+            if (valid < kStep) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i >= valid) s[i >> 5][i & 31] = 0xFF800000u;
-          }
-          const float top0 = fmaxf(max_tree32(s[0]), max_tree32(s[1])) * c[0];
-          const float top1 = fmaxf(max_tree32(s[2]), max_tree32(s[3])) * c[1];
-          const float top = fmaxf(top0, top1), v_top = fmaxf(top0 + v_log2[0], top1 + v_log2[1]);
-          // the references move when a probability, or one times its value's scale, is more than 2^4 above them
-          const bool moves = top > m + kRescale || v_top > m + v_ref + kRescale;
-          if (__any_sync(0xffffffffu, moves)) {
-            const float m_new = moves ? fmaxf(m, top) : m;
-            const float v_new = moves ? (j > begin ? fmaxf(m + v_ref, v_top) : v_top) - m_new : v_ref;
-            if (j > begin) {
-              const float fall = exp2_ftz(fmaxf(m - m_new, -200.f));
-              const float factor = exp2_ftz(fmaxf((m + v_ref) - (m_new + v_new), -200.f));
-              wait(&pv_done[t], k_parity ^ 1u);
-              tc_fence_after();
-#pragma unroll 1
-              for (int i = 0; i < D / 32; ++i) {
-                uint32_t o[32];
-                tmem_ld32(o_tmem + 32u * uint32_t(i), o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                tmem_st32(o_tmem + 32u * uint32_t(i), o);
-              }
-              l *= fall;
+              for (int i = 0; i < 32; ++i)
+                if (i + 32 * w >= valid) s[i] = 0xFF800000u;
             }
-            m = m_new;
-            v_ref = v_new;
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // probabilities times the page's value scale over the reference; times 2^-60 at the least, which is nothing
-            // next to what set the reference
-            const float dv = v_log2[h] == v_log2[h] ? fmaxf(v_log2[h] - v_ref, -60.f) : v_log2[h];
-            const float shift = dv + kLog2P - (m == -INFINITY ? 0.f : m);
-            const float2 mul = make_float2(c[h], c[h]), add = make_float2(shift, shift);
+            const float top = max_tree32(s) * c;
+            follow(top, top + v_log2, j == begin);
+            const float dv = value_shift(v_log2);
             float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+            uint32_t hi[8], lo[8];
+            probabilities(s, c, dv + kLog2P - (m == -INFINITY ? 0.f : m), hi, lo, sum0, sum1);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {  // nothing for the tokens of the other quarters
+              uint32_t x[8], y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                x[e] = g == w ? hi[e] : 0u;
+                y[e] = g == w ? lo[e] : 0u;
+              }
+              tmem_st8(s_tmem + uint32_t(32 * g), x);
+              tmem_st8(s_tmem + uint32_t(32 * g + 8), y);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&p_full[t][0]);
+              mbar_arrive(&p_full[t][1]);
+            }
+            l += ((sum0.x + sum0.y) + (sum1.x + sum1.y)) * exp2_ftz(-dv - kLog2P);
+            continue;
+          }
+          const float c0 = score_scale(0), c1 = score_scale(1);
+          auto load = [&](int h, uint32_t (&s)[2][32]) {  // a page's scores
+            tmem_ld32(s_tmem + 64u * uint32_t(h), s[0]);
+            tmem_ld32(s_tmem + 64u * uint32_t(h) + 32u, s[1]);
+            tmem_wait_ld();
+            if (valid < kStep) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i)
+                if (i + 64 * h >= valid) s[i >> 5][i & 31] = 0xFF800000u;
+            }
+          };
+          float top = -INFINITY, v_top = -INFINITY;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t s[2][32];
+            load(h, s);
+            const float x = fmaxf(max_tree32(s[0]), max_tree32(s[1])) * (h ? c1 : c0);
+            top = fmaxf(top, x);
+            v_top = fmaxf(v_top, x + (h ? page[1].y : page[0].y));
+          }
+          follow(top, v_top, j == begin);
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const float dv = value_shift(h ? page[1].y : page[0].y), shift = dv + kLog2P - (m == -INFINITY ? 0.f : m);
+            float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+            uint32_t s[2][32];
+            load(h, s);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               uint32_t hi[8], lo[8];
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const uint32_t* x = &s[2 * h + g][e];
-                float2 x01 = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), mul, add);
-                float2 x23 = __ffma2_rn(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), mul, add);
-                x01.x = exp2_ftz(x01.x); x01.y = exp2_ftz(x01.y);
-                x23.x = exp2_ftz(x23.x); x23.y = exp2_ftz(x23.y);
-                sum0 = __fadd2_rn(sum0, x01);
-                sum1 = __fadd2_rn(sum1, x23);
-                const __half2 p01 = __floats2half2_rn(x01.x, x01.y), p23 = __floats2half2_rn(x23.x, x23.y);
-                const uint16_t h01 = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&p01));
-                const uint16_t h23 = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&p23));
-                const uint32_t b01 = e4m3x2_to_f16x2(h01), b23 = e4m3x2_to_f16x2(h23);
-                const __half2 l01 = __hsub2(p01, *reinterpret_cast<const __half2*>(&b01));
-                const __half2 l23 = __hsub2(p23, *reinterpret_cast<const __half2*>(&b23));
-                hi[e >> 2] = uint32_t(h01) | uint32_t(h23) << 16;
-                lo[e >> 2] = uint32_t(f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&l01))) |
-                             uint32_t(f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&l23))) << 16;
-              }
-              tmem_st8(s_tmem + uint32_t(16 * h + 8 * g), hi);
-              tmem_st8(s_tmem + uint32_t(32 + 16 * h + 8 * g), lo);
+              probabilities(s[g], h ? c1 : c0, shift, hi, lo, sum0, sum1);
+              tmem_st8(s_tmem + uint32_t(64 * h + 32 * g), hi);
+              tmem_st8(s_tmem + uint32_t(64 * h + 32 * g + 8), lo);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -809,6 +953,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         wait(&pv_done[t], k_parity ^ 1u);  // the last step's output
         tc_fence_after();
       }
+      base += n;
+      __nv_bfloat16* out = a.out + unit_offset(a, a.os, p.u);
       const float to_true = exp2f(v_ref - kLog2P);  // the accumulator's unit
       if (!p.whole) {
         // a part of the unit: sums, maximum and denominator for the second kernel
@@ -831,52 +977,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             }
           }
         }
-      } else if (both && tiles == 2) {
-        // both tiles have the same rows: tile 1 hands its sums over through shared memory, 32 columns at a time (the
-        // space of a second tile of queries, and of its scales in either buffer)
-        float4* xch = reinterpret_cast<float4*>(sm + kOffQ + kQTile);
-        float* xch_ml = q_scale + kTile;
-        if (t == 1) {
-          xch_ml[row] = m;
-          xch_ml[2 * kTile + row] = l;
-        }
-        __nv_bfloat16* out = a.out + row_offset(a, a.os, p.u, live ? r : 0);
-        float f0 = 0.f, f1 = 0.f;
+      } else if (both) {
+        // the copies of a row (2 tiles, or 8 warps) are added through shared memory, 16 columns at a time
+        float4* xch = reinterpret_cast<float4*>(sm + kOffOut);
+        const int me = t * kTile + row, rows = quarters ? 32 : kTile, r_me = me & (rows - 1);
+        copy_ml[me] = make_float2(m, l);
+        all_copies();
+        float top = m, sum = 0.f;
+        for (int c = r_me; c < 2 * kTile; c += rows) top = fmaxf(top, copy_ml[c].x);
+        for (int c = r_me; c < 2 * kTile; c += rows)
+          sum += copy_ml[c].y * exp2_ftz(fmaxf(copy_ml[c].x - top, -200.f));
+        const float f = to_true * exp2_ftz(fmaxf(m - top, -200.f)) / sum;
+        const bool none = l == 0.f;  // (the output of a tile without steps is not set)
 #pragma unroll 1
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t o[16];
           __syncwarp();
-          tmem_ld32(o_tmem + 32u * uint32_t(i), o);
+          tmem_ld16(o_tmem + 16u * uint32_t(i), o);
           tmem_wait_ld();
-          if (t == 1) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              xch[e * kTile + row] = make_float4(__uint_as_float(o[4 * e]) * to_true, __uint_as_float(o[4 * e + 1]) * to_true,
-                                                 __uint_as_float(o[4 * e + 2]) * to_true,
-                                                 __uint_as_float(o[4 * e + 3]) * to_true);
-          }
-          named_bar_sync(1, 256);
-          if (t == 0) {
-            if (i == 0) {
-              const float m1 = xch_ml[row], l1 = xch_ml[2 * kTile + row], top = fmaxf(m, m1);
-              const float e0 = exp2_ftz(fmaxf(m - top, -200.f)), e1 = exp2_ftz(fmaxf(m1 - top, -200.f));
-              const float inv = 1.f / (l * e0 + l1 * e1);
-              f0 = to_true * e0 * inv;
-              f1 = e1 * inv;
-            }
+          for (int e = 0; e < 16; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const float4 u0 = xch[(2 * v) * kTile + row], u1 = xch[(2 * v + 1) * kTile + row];
-              const uint32_t* x = &o[8 * v];
-              const uint4 y = make_uint4(
-                  pack_bf16x2(fmaf(u0.x, f1, __uint_as_float(x[0]) * f0), fmaf(u0.y, f1, __uint_as_float(x[1]) * f0)),
-                  pack_bf16x2(fmaf(u0.z, f1, __uint_as_float(x[2]) * f0), fmaf(u0.w, f1, __uint_as_float(x[3]) * f0)),
-                  pack_bf16x2(fmaf(u1.x, f1, __uint_as_float(x[4]) * f0), fmaf(u1.y, f1, __uint_as_float(x[5]) * f0)),
-                  pack_bf16x2(fmaf(u1.z, f1, __uint_as_float(x[6]) * f0), fmaf(u1.w, f1, __uint_as_float(x[7]) * f0)));
-              if (live) *reinterpret_cast<uint4*>(out + 32 * i + 8 * v) = y;
+          for (int v = 0; v < 4; ++v)
+            xch[v * 2 * kTile + me] = *reinterpret_cast<const float4*>(&o[4 * v]);
+          all_copies();
+          for (int at = me; at < 4 * rows; at += 2 * kTile) {
+            const int v = at / rows, rr = at & (rows - 1);
+            float4 y = xch[v * 2 * kTile + rr];
+            for (int c = rr + rows; c < 2 * kTile; c += rows) {
+              const float4 z = xch[v * 2 * kTile + c];
+              y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
             }
+            if (p.u.block * 2 * kTile + rr < a.rows)
+              *reinterpret_cast<uint2*>(out + row_offset(a, a.os, rr) + 16 * i + 4 * v) =
+                  make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
           }
-          named_bar_sync(2, 256);  // the space may be written again
+          all_copies();  // the space may be written again
         }
       } else if (t < tiles) {
         // through shared memory, 32 columns at a time: 4 lanes then write 64 bytes of a row
@@ -886,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int rr = r0 + w * 32 + x * 8 + (lane >> 2);
-          at[x] = rr < a.rows ? row_offset(a, a.os, p.u, rr) + (lane & 3) * 8 : -1;
+          at[x] = rr < a.rows ? row_offset(a, a.os, rr) + (lane & 3) * 8 : -1;
         }
 #pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
@@ -908,7 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           for (int x = 0; x < 4; ++x) {
             const int rr = x * 8 + (lane >> 2);
             const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
-            if (at[x] >= 0) *reinterpret_cast<uint4*>(a.out + at[x] + 32 * i) = y;
+            if (at[x] >= 0) *reinterpret_cast<uint4*>(out + at[x] + 32 * i) = y;
           }
         }
       }
@@ -925,44 +1061,69 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 }
 
 // Joins the parts of a unit that was cut.  Block (c, y): the unit that begins in
-// CTA c's part of the line and goes on in the next; a warp a row.
+// CTA c's part of the line and goes on in the next; a warp a row at a time.  The
+// parts' maxima and denominators are read by a lane each, so that the loads of
+// their sums wait for nothing.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a, int parts) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Args a, int parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_predecessor();
-  const int64_t total = total_ticks(a, lane);
-  const int64_t cut = part_begin(total, int(blockIdx.x) + 1, parts);
-  if (cut >= total) return;
+  const int first = int(blockIdx.x);
+  const Parts line(total_ticks(a, lane), parts);
+  const int64_t cut = line.begin(first + 1);
+  if (cut >= line.total) return;
   const Unit u = find_unit(a, cut, lane);
   // the unit's steps before the cut: some, and all of them CTA c's
-  if (cut - u.begin <= kOverhead || part_begin(total, int(blockIdx.x), parts) > u.begin + kOverhead) return;
-  const int row = int(blockIdx.y) * 8 + warp, r = u.block * 2 * kTile + row;
-  if (r >= a.rows || (a.both && row >= kTile)) return;
-  constexpr int kCols = D / 32;
-  float o[kCols] = {}, m = -INFINITY, l = 0.f;
+  if (cut - u.begin <= kOverhead || line.begin(first) > u.begin + kOverhead) return;
   const int64_t end = u.begin + kOverhead + u.steps;
-  for (int c = int(blockIdx.x); c < parts; ++c) {
-    const int64_t begin = part_begin(total, c, parts), stop = part_begin(total, c + 1, parts);
-    if (begin >= end) break;
-    const int64_t first = max(begin - u.begin - kOverhead, int64_t(0));
-    if (min(stop, end) - u.begin - kOverhead <= first) continue;  // none of the unit's steps
-    const int part = begin >= u.begin ? 0 : 1;
-    for (int t = 0; t < (a.both ? 2 : 1); ++t) {
-      const int64_t at = (int64_t(c) * 2 + part) * 2 * kTile + t * kTile + row;
-      const float2 ml = a.part_ml[at];
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a tile without steps
-      const float top = fmaxf(m, ml.x);
-      const float e0 = m == -INFINITY ? 0.f : exp2f(m - top), e1 = exp2f(ml.x - top);
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) o[i] = o[i] * e0 + a.part_o[at * D + lane * kCols + i] * e1;
-      l = l * e0 + ml.y * e1;
-      m = top;
-    }
+  int count = 1;  // CTAs with steps of the unit
+  for (int c0 = first + 1; c0 < parts; c0 += 32) {
+    const uint32_t has = __ballot_sync(0xffffffffu, c0 + lane < parts && line.begin(c0 + lane) < end);
+    count += __popc(has);
+    if (has != 0xffffffffu) break;
   }
-  __nv_bfloat16* out = a.out + row_offset(a, a.os, u, r) + lane * kCols;
-  const float inv = 1.f / l;
+  const int part = line.begin(first) >= u.begin ? 0 : 1;  // the first one's; the others' begin with the unit
+  const int apart = a.quarters ? 32 : kTile, copies = a.both ? 2 * kTile / apart : 1;
+  constexpr int kCols = D / 32;
+  const int rows = min(a.rows - u.block * 2 * kTile, 2 * kTile);
+  for (int row = int(blockIdx.y) * kJoinWarps + warp; row < rows; row += int(gridDim.y) * kJoinWarps) {
+    float o[kCols] = {}, m = -INFINITY, l = 0.f;
+    for (int e0 = 0; e0 < count * copies; e0 += 32) {
+      const int e = e0 + lane, c = e / copies;
+      const int64_t mine = (int64_t(first + c) * 2 + (c ? 0 : part)) * 2 * kTile + (e - c * copies) * apart + row;
+      // (with fewer ticks than CTAs some have none)
+      const bool some = e < count * copies && line.begin(first + c + 1) > line.begin(first + c);
+      const float2 ml = some ? a.part_ml[mine] : make_float2(-INFINITY, 0.f);
+      float top = fmaxf(m, ml.x);
 #pragma unroll
-  for (int i = 0; i < kCols; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float fall = exp2_ftz(fmaxf(m - top, -200.f)), share = exp2_ftz(fmaxf(ml.x - top, -200.f));
+      float sum = ml.y * share;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      l = l * fall + sum;
+      m = top;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] *= fall;
+      uint32_t left = __ballot_sync(0xffffffffu, ml.y != 0.f);  // (a copy without tokens has no sums)
+#pragma unroll 4
+      for (; left != 0; left &= left - 1) {
+        const int src = __ffs(int(left)) - 1;
+        const float f = __shfl_sync(0xffffffffu, share, src);
+        const float* from = a.part_o + __shfl_sync(0xffffffffu, mine, src) * D + lane * kCols;
+        float x[kCols];
+        if constexpr (kCols == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
+        else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) o[i] = fmaf(x[i], f, o[i]);
+      }
+    }
+    __nv_bfloat16* out = a.out + unit_offset(a, a.os, u) + row_offset(a, a.os, u.block * 2 * kTile + row) + lane * kCols;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < kCols; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1022,8 +1183,8 @@ cudaError_t launch_attention(cudaStream_t st, const Maps& maps, const Args& a, i
   if (e != cudaSuccess) return e;
   const int rows = a.rows < 2 * kTile ? a.rows : 2 * kTile;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(sms - 1), unsigned(cdiv(rows, 8)));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(unsigned(sms - 1), unsigned(cdiv(rows, 4 * kJoinWarps)));
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1132,9 +1293,11 @@ int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, con
   a.batch = int(batch);
   a.heads = int(heads);
   a.group = int(group);
+  a.group_magic = group == 1 ? 0u : uint32_t((uint64_t(1) << 32) / uint64_t(group) + 1);
   a.rows = int(queries * group);
   a.blocks = int(cdiv(a.rows, 2 * kTile));
   a.both = a.rows <= kTile ? 1 : 0;
+  a.quarters = a.rows <= 32 ? 1 : 0;
   a.scale_log2 = scale * kLog2e;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + size_t(sms) * 2 * 2 * kTile * size_t(dim));
