@@ -188,7 +188,6 @@ constexpr int kQTile = 2 * kTile * 128;  // hi, lo
 constexpr int kQBuf = 2 * kQTile;   // two tiles
 constexpr int kThreads = 512;       // 0 TMA, 1 MMA + TMEM, 2-3 and 12-15 queries, 4-7 and 8-11 softmax
 constexpr int kLoaders = 6;
-constexpr int kOverhead = 2;        // steps' time that a unit takes besides its steps
 constexpr float kLog2P = 4.f;       // probabilities are held times 2^4 ...
 constexpr float kRescale = 4.f;     // ... and their reference lags the maximum by up to 2^4: at most 2^8 < 448
 constexpr int kOffQ = 0;                        // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes], then the ring
@@ -216,6 +215,7 @@ struct Args {
   int batch, heads, group;     // key/value heads; query heads of each
   uint32_t group_magic;        // 2^32 / group + 1, rounded down; 0 for 1
   int rows, blocks;            // rows of a key/value head (queries x group); units of 256 of them
+  int overhead;                // steps' time that a unit takes besides its steps
   int both;                    // 1: both tiles hold the same rows and take the steps in turn
   int quarters;                // 1: so do the 4 warps of a tile, each with a quarter of a step's tokens
   float scale_log2;            // softmax scale * log2(e)
@@ -233,10 +233,10 @@ __device__ __forceinline__ int request_steps(const Args& a, int b) {
   return (request_tokens(a, b) + kStep - 1) / kStep;
 }
 
-// Ticks of the line of all units: a unit takes kOverhead and its steps.  All lanes.
+// Ticks of the line of all units: a unit takes a.overhead and its steps.  All lanes.
 __device__ __forceinline__ int64_t total_ticks(const Args& a, int lane) {
   int64_t sum = 0;
-  for (int b = lane; b < a.batch; b += 32) sum += request_steps(a, b) + kOverhead;
+  for (int b = lane; b < a.batch; b += 32) sum += request_steps(a, b) + a.overhead;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   return sum * a.heads * a.blocks;
@@ -264,7 +264,7 @@ __device__ __forceinline__ Unit find_unit(const Args& a, int64_t tick, int lane)
   for (int b0 = 0;; b0 += 32) {
     const int b = b0 + lane;
     const int tokens = b < a.batch ? request_tokens(a, b) : 0, steps = (tokens + kStep - 1) / kStep;
-    const int64_t own = b < a.batch ? (steps + kOverhead) * units : 0;
+    const int64_t own = b < a.batch ? (steps + a.overhead) * units : 0;
     int64_t upto = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -279,8 +279,8 @@ __device__ __forceinline__ Unit find_unit(const Args& a, int64_t tick, int lane)
       u.tokens = __shfl_sync(0xffffffffu, tokens, src);
       u.steps = (u.tokens + kStep - 1) / kStep;
       const int64_t first = before + __shfl_sync(0xffffffffu, upto - own, src);
-      const int64_t index = (tick - first) / (u.steps + kOverhead);
-      u.begin = first + index * (u.steps + kOverhead);
+      const int64_t index = (tick - first) / (u.steps + a.overhead);
+      u.begin = first + index * (u.steps + a.overhead);
       u.block = int(index / a.heads);
       u.head = int(index % a.heads);
       return u;
@@ -311,11 +311,11 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(const Args& a, Piece& p) {
     while (at < end) {
-      const int lo = int(at - u.begin), most = u.steps + kOverhead;
+      const int lo = int(at - u.begin), most = u.steps + a.overhead;
       const int hi = end - u.begin < most ? int(end - u.begin) : most;
       p.u = u;
-      p.first = max(lo - kOverhead, 0);
-      p.count = max(hi - kOverhead, 0) - p.first;
+      p.first = max(lo - a.overhead, 0);
+      p.count = max(hi - a.overhead, 0) - p.first;
       p.whole = p.first == 0 && p.count == u.steps;
       p.zero = u.steps == 0 && lo == 0;
       p.part = at == begin ? 0 : 1;
@@ -673,30 +673,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       // ================= queries =================
       // Four lanes a row, eight rows a warp at a time: the row's largest value, its scale, hi and lo.  The bf16 row has
       // the size of its two e4m3 rows: it is copied to their place asynchronously, all rows of the buffer at once (48 in
-      // flight, through registers, took 20000 clocks a buffer), and split there.
+      // flight, through registers, took 20000 clocks a buffer, this takes 15000), and split there.
       const int loader = warp < 4 ? warp - 2 : warp - 10;
       const int sub = lane >> 2, part = lane & 3;
       constexpr int kVecs = D / 32;  // 16-byte vectors of a lane: part + 4 i
       constexpr int kRounds = (2 * kTile + 8 * kLoaders - 1) / (8 * kLoaders);
       constexpr int kRowLanes = D / 8, kRowsAtOnce = 32 / kRowLanes;  // a copy's lanes in a row, its rows
       Walk walk(a, lane);
-      Piece p{}, after{};
+      Piece p{};
       int buf = 0;
       uint32_t parity = 1;
-      bool ok = true, more = walk.next(a, p);
-      for (bool last = false; !last; p = after) {
-        last = !more;
-        const bool here = more;
-        if (more) more = walk.next(a, after);
-        if (more) {  // the next piece's rows, on their way to L2 meanwhile
-          const int kept = min(a.rows - after.u.block * 2 * kTile, 2 * kTile);
-          const __nv_bfloat16* q = a.q + unit_offset(a, a.qs, after.u);
-          for (int row = loader * 32 + lane; row < kept; row += 32 * kLoaders) {
-            const __nv_bfloat16* src = q + row_offset(a, a.qs, after.u.block * 2 * kTile + row);
-#pragma unroll
-            for (int i = 0; i < D; i += 64) asm volatile("prefetch.global.L2 [%0];" :: "l"(src + i));
-          }
-        }
+      bool ok = true;
+      for (bool here = true; here;) {
+        here = walk.next(a, p);
         const int r0 = p.u.block * 2 * kTile;
         // rows of the buffer; with quarters every 32 of them are the same
         const int mask = a.quarters ? 31 : 255, kept = min(a.rows - r0, 2 * kTile);
@@ -707,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) *reinterpret_cast<uint4*>(dst + 32 * i) = make_uint4(0u, 0u, 0u, 0u);
           }
-          continue;  // (a piece: not the last)
+          continue;
         }
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_empty[buf], parity));
         if (!ok) break;
@@ -728,9 +717,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           cp_async_commit();
         }
         auto split = [&](int x) {
-          const int row = x * 8 * kLoaders + loader * 8 + sub;
-          if (x * 8 * kLoaders + loader * 8 >= live) return;
-          unsigned char* at = place(row < live ? row : x * 8 * kLoaders + loader * 8);
+          const int first = x * 8 * kLoaders + loader * 8, row = first + sub;
+          if (first >= live) return;
+          unsigned char* at = place(row < live ? row : first);
           Bf8 v[kVecs];
           uint32_t amax = 0;
 #pragma unroll
@@ -776,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           split(x);
         }
         if (loader == 0 && lane == 0) {
-          if (last) p.count = 0;
+          if (!here) p.count = 0;
           work[buf] = p;
         }
         fence_proxy_async();
@@ -956,28 +945,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       base += n;
       __nv_bfloat16* out = a.out + unit_offset(a, a.os, p.u);
       const float to_true = exp2f(v_ref - kLog2P);  // the accumulator's unit
-      if (!p.whole) {
-        // a part of the unit: sums, maximum and denominator for the second kernel
-        const int64_t at = (int64_t(blockIdx.x) * 2 + p.part) * 2 * kTile + t * kTile + row;
-        if (live) a.part_ml[at] = make_float2(m, l);
-        if (t < tiles) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + at * D);
-#pragma unroll 1
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t o[16];
-            __syncwarp();
-            tmem_ld16(o_tmem + 16u * uint32_t(i), o);
-            tmem_wait_ld();
-            if (live) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                dst[4 * i + e] = make_float4(__uint_as_float(o[4 * e]) * to_true, __uint_as_float(o[4 * e + 1]) * to_true,
-                                             __uint_as_float(o[4 * e + 2]) * to_true,
-                                             __uint_as_float(o[4 * e + 3]) * to_true);
-            }
-          }
-        }
-      } else if (both) {
+      const int64_t part_row = (int64_t(blockIdx.x) * 2 + p.part) * 2 * kTile;  // the first of a part of the unit
+      if (both) {
         // the copies of a row (2 tiles, or 8 warps) are added through shared memory, 16 columns at a time
         float4* xch = reinterpret_cast<float4*>(sm + kOffOut);
         const int me = t * kTile + row, rows = quarters ? 32 : kTile, r_me = me & (rows - 1);
@@ -987,7 +956,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         for (int c = r_me; c < 2 * kTile; c += rows) top = fmaxf(top, copy_ml[c].x);
         for (int c = r_me; c < 2 * kTile; c += rows)
           sum += copy_ml[c].y * exp2_ftz(fmaxf(copy_ml[c].x - top, -200.f));
-        const float f = to_true * exp2_ftz(fmaxf(m - top, -200.f)) / sum;
+        float f = to_true * exp2_ftz(fmaxf(m - top, -200.f));
+        if (p.whole) f /= sum;
+        else if (me < rows && live) a.part_ml[part_row + me] = make_float2(top, sum);
         const bool none = l == 0.f;  // (the output of a tile without steps is not set)
 #pragma unroll 1
         for (int i = 0; i < D / 16; ++i) {
@@ -1008,11 +979,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               const float4 z = xch[v * 2 * kTile + c];
               y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
             }
-            if (p.u.block * 2 * kTile + rr < a.rows)
-              *reinterpret_cast<uint2*>(out + row_offset(a, a.os, rr) + 16 * i + 4 * v) =
+            if (rr >= a.rows) continue;
+            const int col = 16 * i + 4 * v;
+            if (p.whole)
+              *reinterpret_cast<uint2*>(out + row_offset(a, a.os, rr) + col) =
                   make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+            else
+              *reinterpret_cast<float4*>(a.part_o + (part_row + rr) * D + col) = y;
           }
           all_copies();  // the space may be written again
+        }
+      } else if (!p.whole) {
+        // sums, maximum and denominator for the second kernel
+        const int64_t at = part_row + t * kTile + row;
+        if (live) a.part_ml[at] = make_float2(m, l);
+        if (t < tiles) {
+          float4* dst = reinterpret_cast<float4*>(a.part_o + at * D);
+#pragma unroll 1
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t o[16];
+            __syncwarp();
+            tmem_ld16(o_tmem + 16u * uint32_t(i), o);
+            tmem_wait_ld();
+            if (live) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                dst[4 * i + e] = make_float4(__uint_as_float(o[4 * e]) * to_true, __uint_as_float(o[4 * e + 1]) * to_true,
+                                             __uint_as_float(o[4 * e + 2]) * to_true,
+                                             __uint_as_float(o[4 * e + 3]) * to_true);
+            }
+          }
         }
       } else if (t < tiles) {
         // through shared memory, 32 columns at a time: 4 lanes then write 64 bytes of a row
@@ -1075,8 +1071,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   if (cut >= line.total) return;
   const Unit u = find_unit(a, cut, lane);
   // the unit's steps before the cut: some, and all of them CTA c's
-  if (cut - u.begin <= kOverhead || line.begin(first) > u.begin + kOverhead) return;
-  const int64_t end = u.begin + kOverhead + u.steps;
+  if (cut - u.begin <= a.overhead || line.begin(first) > u.begin + a.overhead) return;
+  const int64_t end = u.begin + a.overhead + u.steps;
   int count = 1;  // CTAs with steps of the unit
   for (int c0 = first + 1; c0 < parts; c0 += 32) {
     const uint32_t has = __ballot_sync(0xffffffffu, c0 + lane < parts && line.begin(c0 + lane) < end);
@@ -1084,16 +1080,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
     if (has != 0xffffffffu) break;
   }
   const int part = line.begin(first) >= u.begin ? 0 : 1;  // the first one's; the others' begin with the unit
-  const int apart = a.quarters ? 32 : kTile, copies = a.both ? 2 * kTile / apart : 1;
   constexpr int kCols = D / 32;
   const int rows = min(a.rows - u.block * 2 * kTile, 2 * kTile);
   for (int row = int(blockIdx.y) * kJoinWarps + warp; row < rows; row += int(gridDim.y) * kJoinWarps) {
     float o[kCols] = {}, m = -INFINITY, l = 0.f;
-    for (int e0 = 0; e0 < count * copies; e0 += 32) {
-      const int e = e0 + lane, c = e / copies;
-      const int64_t mine = (int64_t(first + c) * 2 + (c ? 0 : part)) * 2 * kTile + (e - c * copies) * apart + row;
+    for (int c0 = 0; c0 < count; c0 += 32) {
+      const int c = c0 + lane;
+      const int64_t mine = (int64_t(first + c) * 2 + (c ? 0 : part)) * 2 * kTile + row;
       // (with fewer ticks than CTAs some have none)
-      const bool some = e < count * copies && line.begin(first + c + 1) > line.begin(first + c);
+      const bool some = c < count && line.begin(first + c + 1) > line.begin(first + c);
       const float2 ml = some ? a.part_ml[mine] : make_float2(-INFINITY, 0.f);
       float top = fmaxf(m, ml.x);
 #pragma unroll
@@ -1106,7 +1101,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
       m = top;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) o[i] *= fall;
-      uint32_t left = __ballot_sync(0xffffffffu, ml.y != 0.f);  // (a copy without tokens has no sums)
+      uint32_t left = __ballot_sync(0xffffffffu, ml.y != 0.f);  // (one without tokens has no sums)
 #pragma unroll 4
       for (; left != 0; left &= left - 1) {
         const int src = __ffs(int(left)) - 1;
@@ -1298,6 +1293,9 @@ int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, con
   a.blocks = int(cdiv(a.rows, 2 * kTile));
   a.both = a.rows <= kTile ? 1 : 0;
   a.quarters = a.rows <= 32 ? 1 : 0;
+  // a unit takes about as long as that many steps besides its own (one token, 8 requests of 130 to 32767: 165 us at 2,
+  // 92 at 12; 32760 queries over 512 and 77 tokens: 966 at 2, 840 at 5)
+  a.overhead = a.quarters ? 12 : 5;
   a.scale_log2 = scale * kLog2e;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + size_t(sms) * 2 * 2 * kTile * size_t(dim));
