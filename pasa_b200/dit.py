@@ -36,6 +36,13 @@ Two implementations of the same step:
   rotary embedding in float64).  It runs on any device and is the comparison
   for the fused path.
 
+Two options serve many requests at once, on both paths.  ``adapters`` adds
+each request's low-rank update to the projections (``ops.lora_update``).
+``text_kv`` holds the text's keys and values of every block in pages of 8 bits:
+they are the same in all steps of a request, so they are made once
+(``text_cache``) and read by ``ops.kv8_attention`` in place of two projections
+and SDPA.
+
 With a process group of P ranks each rank holds T/P consecutive tokens
 (Ulysses): q, k, v go sequence-sharded -> head-sharded with one all-to-all
 each, the attention core runs on H/P heads over all T tokens, and one
@@ -45,7 +52,7 @@ from __future__ import annotations
 
 import dataclasses
 import math
-from typing import Callable, List, Optional, Tuple
+from typing import Callable, Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 import torch.distributed as dist
@@ -178,6 +185,106 @@ def head_to_tokens(t: torch.Tensor, group) -> torch.Tensor:
     return recv.permute(1, 3, 0, 2, 4).reshape(B, L // P, P * Hl * D)
 
 
+class Adapters(NamedTuple):
+    """Low-rank adapters of a step's requests.  ``slots`` int32 [B]: the adapter of each batch entry, -1 for none;
+    ``scale`` fp32 [adapters] or None for 1; ``blocks``: for each block the adapted projections (of "q", "k", "v",
+    "o", "cq", "co", "ffn1", "ffn2") with their a [adapters, rank, in] and b [adapters, out, rank]."""
+    slots: torch.Tensor
+    scale: Optional[torch.Tensor]
+    blocks: Sequence[Dict[str, Tuple[torch.Tensor, torch.Tensor]]]
+
+
+class TextCache(NamedTuple):
+    """The text's normalised keys and values of every block, in pages of 64 tokens with 8 bits a value.  ``table``
+    int32 [B, W] and ``lengths`` int32 [B] as for ``ops.kv8_attention``, the same for all blocks."""
+    blocks: Sequence[ops.KV8Cache]
+    table: torch.Tensor
+    lengths: torch.Tensor
+
+
+def _project(t: torch.Tensor, w: dict, name: str, lora, fused: bool) -> torch.Tensor:
+    """t [B, L, in] through a projection, with the adapters (a block's ``_BlockAdapters`` or None)."""
+    y = F.linear(t, w[name], w[name + "_b"])
+    if lora is None or name not in lora.weights:
+        return y
+    a, b = lora.weights[name]
+    if fused:
+        return ops.lora_update(y, t, a, b, lora.rows, lora.slots, lora.scale, out=y)
+    y = y.clone()
+    for i, slot in enumerate(lora.slots.tolist()):
+        if 0 <= slot < a.shape[0]:
+            update = F.linear(F.linear(t[i], a[slot].to(t.dtype)), b[slot].to(t.dtype)).float()
+            y[i] = (y[i].float() + update * (1.0 if lora.scale is None else lora.scale[slot])).to(y.dtype)
+    return y
+
+
+class _BlockAdapters(NamedTuple):
+    rows: torch.Tensor
+    slots: torch.Tensor
+    scale: Optional[torch.Tensor]
+    weights: Dict[str, Tuple[torch.Tensor, torch.Tensor]]
+
+
+def _block_adapters(adapters: Optional[Adapters], batch: int, tokens: int, blocks: int):
+    """For each block its adapters over a batch of ``tokens`` rows a request, or None."""
+    if adapters is None:
+        return [None] * blocks
+    if adapters.slots.shape != (batch,) or len(adapters.blocks) != blocks:
+        raise ValueError(f"adapters must hold {batch} slots and {blocks} blocks, got {tuple(adapters.slots.shape)} and "
+                         f"{len(adapters.blocks)}")
+    unknown = {n for block in adapters.blocks for n in block} - {"q", "k", "v", "o", "cq", "co", "ffn1", "ffn2"}
+    if unknown:
+        raise ValueError(f"no such projections to adapt: {', '.join(sorted(unknown))}")
+    rows = torch.arange(batch + 1, dtype=torch.int32, device=adapters.slots.device) * tokens
+    return [_BlockAdapters(rows, adapters.slots, adapters.scale, block) for block in adapters.blocks]
+
+
+def _heads(t: torch.Tensor, cfg: DiTConfig) -> torch.Tensor:
+    return t.unflatten(2, (cfg.heads, cfg.head_dim)).transpose(1, 2)
+
+
+def _text_keys(text: torch.Tensor, w: dict, cfg: DiTConfig, fused: bool) -> torch.Tensor:
+    ck = F.linear(text, w["ck"], w["ck_b"])
+    if fused:
+        return ops.dit_qkv_rope(ck, None, None, w["cnorm_k_f"], None, None, None, cfg.heads, cfg.eps,
+                                head_major=False)[0]
+    return rms_norm(ck, w["cnorm_k"], cfg.eps)
+
+
+def text_cache(text_embed: torch.Tensor, embed: dict, blocks: List[dict], cfg: DiTConfig,
+               lengths: Optional[torch.Tensor] = None) -> TextCache:
+    """The cache of a batch of texts for ``step``'s ``text_kv`` (bf16 weights on a GPU; heads of 64 or 128
+    dimensions).  ``text_embed`` [B, Lt, text_dim]; ``lengths`` int32 [B]: the texts' tokens (all Lt by default), which
+    are all that is attended to."""
+    text = project_text(embed, text_embed)
+    batch, tokens = text.shape[:2]
+    width = -(-tokens // 64)
+    table = torch.arange(batch * width, dtype=torch.int32, device=text.device).view(batch, width)
+    starts = torch.zeros(batch, dtype=torch.int32, device=text.device)
+    if lengths is None:
+        lengths = torch.full_like(starts, tokens)
+    caches = []
+    for w in blocks:
+        cache = ops.kv8_cache(batch * width, cfg.heads, cfg.head_dim, device=text.device)
+        ops.kv8_write(cache, _heads(_text_keys(text, w, cfg, fused=True), cfg),
+                      _heads(F.linear(text, w["cv"], w["cv_b"]), cfg), table, starts, lengths)
+        caches.append(cache)
+    return TextCache(caches, table, lengths)
+
+
+def _cached_attention_plain(q: torch.Tensor, cache, table: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
+    """q [B, H, L, D] over a ``TextCache`` block, in torch ops."""
+    out = torch.zeros_like(q)
+    for b, n in enumerate(lengths.tolist()):
+        n = min(n, 64 * table.shape[1])
+        if n > 0:
+            pages = table[b, :-(-n // 64)].long()
+            k, v = ((t[pages].float() * s[pages][:, :, None, None]).transpose(0, 1).flatten(1, 2)[:, :n]
+                    for t, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+            out[b] = F.scaled_dot_product_attention(q[b].float(), k, v).to(q.dtype)
+    return out
+
+
 def pasa_core(density: float) -> Callable:
     """PASA as the self-attention core; its output is stored token-major so
     the output projection reads it without a transpose copy."""
@@ -186,32 +293,31 @@ def pasa_core(density: float) -> Callable:
     return core
 
 
-def _self_attention(q, k, v, w, attn_core, group):
+def _self_attention(q, k, v, w, attn_core, group, lora=None, fused=False):
     """Head-major q, k, v of this rank's tokens -> the projected attention
     output [B, L_local, C]."""
     if group is not None:
         q, k, v = (seq_to_head(t, group) for t in (q, k, v))
     o = attn_core(q.contiguous(), k.contiguous(), v.contiguous())
     o = head_to_tokens(o, group) if group is not None else o.transpose(1, 2).flatten(2, 3)
-    return F.linear(o, w["o"], w["o_b"])
+    return _project(o, w, "o", lora, fused)
 
 
-def _cross_attention(cq, text, w, cfg, fused: bool):
-    """cq [B, L, C] normalised queries -> the projected cross-attention output."""
-    H, D = cfg.heads, cfg.head_dim
-    if fused:
-        ck = ops.dit_qkv_rope(F.linear(text, w["ck"], w["ck_b"]), None, None, w["cnorm_k_f"], None, None, None,
-                              H, cfg.eps, head_major=False)[0]
+def _cross_attention(cq, text, w, cfg, fused: bool, lora=None, text_kv=None):
+    """cq [B, L, C] normalised queries -> the projected cross-attention output.
+    ``text_kv``: (cache, table, lengths) in place of the text's projections."""
+    if text_kv is not None:
+        attend = ops.kv8_attention if fused else _cached_attention_plain
+        co = attend(_heads(cq, cfg), *text_kv)
     else:
-        ck = rms_norm(F.linear(text, w["ck"], w["ck_b"]), w["cnorm_k"], cfg.eps)
-    cv = F.linear(text, w["cv"], w["cv_b"])
-    heads = lambda t: t.unflatten(2, (H, D)).transpose(1, 2)
-    co = F.scaled_dot_product_attention(heads(cq), heads(ck), heads(cv))
-    return F.linear(co.transpose(1, 2).flatten(2, 3), w["co"], w["co_b"])
+        ck = _text_keys(text, w, cfg, fused)
+        cv = F.linear(text, w["cv"], w["cv_b"])
+        co = F.scaled_dot_product_attention(_heads(cq, cfg), _heads(ck, cfg), _heads(cv, cfg))
+    return _project(co.transpose(1, 2).flatten(2, 3), w, "co", lora, fused)
 
 
 def block_forward(x: torch.Tensor, text: torch.Tensor, temb: torch.Tensor, rope, w: dict, cfg: DiTConfig,
-                  attn_core: Callable, group=None) -> torch.Tensor:
+                  attn_core: Callable, group=None, lora=None, text_kv=None) -> torch.Tensor:
     """One block in torch ops on this rank's tokens.  x [B, L_local, C], text
     [B, Lt, C], temb [B, 6, C] fp32, rope = float64 (cos, sin) of this rank's
     tokens."""
@@ -222,23 +328,23 @@ def block_forward(x: torch.Tensor, text: torch.Tensor, temb: torch.Tensor, rope,
     # 1. self-attention
     h = F.layer_norm(x.float(), (C,), eps=cfg.eps)
     h = (h * (1 + scale) + shift).to(x.dtype)
-    q = rms_norm(F.linear(h, w["q"], w["q_b"]), w["norm_q"], cfg.eps)
-    k = rms_norm(F.linear(h, w["k"], w["k_b"]), w["norm_k"], cfg.eps)
-    v = F.linear(h, w["v"], w["v_b"])
+    q = rms_norm(_project(h, w, "q", lora, False), w["norm_q"], cfg.eps)
+    k = rms_norm(_project(h, w, "k", lora, False), w["norm_k"], cfg.eps)
+    v = _project(h, w, "v", lora, False)
     q, k, v = (t.unflatten(2, (H, D)).transpose(1, 2).contiguous() for t in (q, k, v))
     q, k = apply_rope(q, *rope), apply_rope(k, *rope)
-    o = _self_attention(q, k, v, w, attn_core, group)
+    o = _self_attention(q, k, v, w, attn_core, group, lora)
     x = (x.float() + o.float() * gate).to(x.dtype)
 
     # 2. cross-attention over the text tokens
     h = F.layer_norm(x.float(), (C,), w["norm2_w"], w["norm2_b"], eps=cfg.eps).to(x.dtype)
-    cq = rms_norm(F.linear(h, w["cq"], w["cq_b"]), w["cnorm_q"], cfg.eps)
-    x = x + _cross_attention(cq, text, w, cfg, fused=False)
+    cq = rms_norm(_project(h, w, "cq", lora, False), w["cnorm_q"], cfg.eps)
+    x = x + _cross_attention(cq, text, w, cfg, False, lora, text_kv)
 
     # 3. feed-forward
     h = F.layer_norm(x.float(), (C,), eps=cfg.eps)
     h = (h * (1 + c_scale) + c_shift).to(x.dtype)
-    f = F.linear(F.gelu(F.linear(h, w["ffn1"], w["ffn1_b"]), approximate="tanh"), w["ffn2"], w["ffn2_b"])
+    f = _project(F.gelu(_project(h, w, "ffn1", lora, False), approximate="tanh"), w, "ffn2", lora, False)
     return (x.float() + f.float() * c_gate).to(x.dtype)
 
 
@@ -246,7 +352,8 @@ Pending = Optional[Tuple[torch.Tensor, torch.Tensor]]
 
 
 def block_forward_fused(x: torch.Tensor, pending: Pending, text: torch.Tensor, temb: torch.Tensor, rope, w: dict,
-                        cfg: DiTConfig, attn_core: Callable, group=None, exchange=None) -> Tuple[torch.Tensor, Pending]:
+                        cfg: DiTConfig, attn_core: Callable, group=None, exchange=None, lora=None,
+                        text_kv=None) -> Tuple[torch.Tensor, Pending]:
     """One block with the row kernels; ``x`` (bf16, contiguous) is updated in
     place.  ``pending`` = (ffn output, its gate) of the previous block, whose
     residual update is folded into this block's first norm; the block returns
@@ -260,24 +367,24 @@ def block_forward_fused(x: torch.Tensor, pending: Pending, text: torch.Tensor, t
     # 1. (previous FFN residual) + LayerNorm + modulation -> self-attention
     h = ops.dit_row_norm(x, add=add, gate=add_gate, x_out=x if add is not None else None, scale=scale,
                          shift=shift, eps=cfg.eps)
-    xq, xk, xv = F.linear(h, w["q"], w["q_b"]), F.linear(h, w["k"], w["k_b"]), F.linear(h, w["v"], w["v_b"])
+    xq, xk, xv = (_project(h, w, name, lora, True) for name in ("q", "k", "v"))
     if exchange is not None:
         q, k, v = exchange.scatter_qkv(xq, xk, xv, w["norm_q_f"], w["norm_k_f"], rope[0], rope[1], cfg.eps)
-        o = F.linear(exchange.attention(q, k, v, cfg.density), w["o"], w["o_b"])
+        o = _project(exchange.attention(q, k, v, cfg.density), w, "o", lora, True)
     else:
         q, k, v = ops.dit_qkv_rope(xq, xk, xv, w["norm_q_f"], w["norm_k_f"], rope[0], rope[1], cfg.heads, cfg.eps,
                                    head_major=True)
-        o = _self_attention(q, k, v, w, attn_core, group)
+        o = _self_attention(q, k, v, w, attn_core, group, lora, fused=True)
 
     # 2. gated residual + affine LayerNorm -> cross-attention
     h = ops.dit_row_norm(x, add=o, gate=gate, x_out=x, weight=w["norm2_w"], bias=w["norm2_b"], eps=cfg.eps)
-    cq = ops.dit_qkv_rope(F.linear(h, w["cq"], w["cq_b"]), None, None, w["cnorm_q_f"], None, None, None,
+    cq = ops.dit_qkv_rope(_project(h, w, "cq", lora, True), None, None, w["cnorm_q_f"], None, None, None,
                           cfg.heads, cfg.eps, head_major=False)[0]
-    co = _cross_attention(cq, text, w, cfg, fused=True)
+    co = _cross_attention(cq, text, w, cfg, True, lora, text_kv)
 
     # 3. residual + LayerNorm + modulation -> FFN (its residual goes to the next norm)
     h = ops.dit_row_norm(x, add=co, x_out=x, scale=c_scale, shift=c_shift, eps=cfg.eps)
-    f = F.linear(F.gelu(F.linear(h, w["ffn1"], w["ffn1_b"]), approximate="tanh"), w["ffn2"], w["ffn2_b"])
+    f = _project(F.gelu(_project(h, w, "ffn1", lora, True), approximate="tanh"), w, "ffn2", lora, True)
     return x, (f, c_gate)
 
 
@@ -327,41 +434,52 @@ def timestep_features(t: torch.Tensor, dim: int) -> torch.Tensor:
     return torch.cat((torch.cos(ang), torch.sin(ang)), dim=1)
 
 
-def condition(e: dict, timestep: torch.Tensor, text_embed: torch.Tensor):
+def project_text(e: dict, text_embed: torch.Tensor) -> torch.Tensor:
+    return F.linear(F.gelu(F.linear(text_embed.to(e["x1"].dtype), e["x1"], e["x1_b"]), approximate="tanh"), e["x2"],
+                    e["x2_b"])
+
+
+def condition(e: dict, timestep: torch.Tensor, text_embed: Optional[torch.Tensor]):
     """temb [B, C] fp32, the blocks' modulation [B, 6, C] fp32 and the
-    projected text [B, Lt, C]."""
+    projected text [B, Lt, C] (None without a text)."""
     dt = e["t1"].dtype
     f = timestep_features(timestep, e["t1"].shape[1]).to(dt)
     temb = F.linear(F.silu(F.linear(f, e["t1"], e["t1_b"])), e["t2"], e["t2_b"])
     tproj = F.linear(F.silu(temb), e["tproj"], e["tproj_b"])
-    text = F.linear(F.gelu(F.linear(text_embed.to(dt), e["x1"], e["x1_b"]), approximate="tanh"), e["x2"], e["x2_b"])
+    text = None if text_embed is None else project_text(e, text_embed)
     return temb.float(), tproj.float().unflatten(1, (6, -1)), text
 
 
-def step(latents_local: torch.Tensor, timestep: torch.Tensor, text_embed: torch.Tensor, rope, embed: dict,
+def step(latents_local: torch.Tensor, timestep: torch.Tensor, text_embed: Optional[torch.Tensor], rope, embed: dict,
          blocks: List[dict], cfg: DiTConfig, attn_core: Callable, group=None, fused: bool = False,
-         exchange=None) -> torch.Tensor:
+         exchange=None, adapters: Optional[Adapters] = None, text_kv: Optional[TextCache] = None) -> torch.Tensor:
     """One denoising step (the transformer forward of the reference's
     WanTransformer3DModel_Sparse.forward, svg/models/wan/custom_models.py:115-200)
     on this rank's tokens: patch embedding, condition embedder, every block,
     output norm and projection.  ``latents_local`` holds this rank's patches
     [B, L_local, c*4]; returns the predicted patches [B, L_local, c*4].
     ``fused`` selects the row-kernel path (bf16 CUDA tensors); ``exchange``
-    (with ``fused``) replaces the NCCL all-to-alls by the peer-memory scatter."""
-    temb, tproj, text = condition(embed, timestep, text_embed)
+    (with ``fused``) replaces the NCCL all-to-alls by the peer-memory scatter.
+    ``adapters`` are added to the projections of their requests; with ``text_kv``
+    the cross-attention reads its pages and ``text_embed`` is not used."""
+    if text_kv is not None and len(text_kv.blocks) != len(blocks):
+        raise ValueError(f"text_kv must hold {len(blocks)} blocks, got {len(text_kv.blocks)}")
+    temb, tproj, text = condition(embed, timestep, None if text_kv is not None else text_embed)
     x = F.linear(latents_local.to(embed["patch"].dtype), embed["patch"], embed["patch_b"])
+    lora = _block_adapters(adapters, x.shape[0], x.shape[1], len(blocks))
+    kv = [None] * len(blocks) if text_kv is None else [(c, text_kv.table, text_kv.lengths) for c in text_kv.blocks]
     shift, scale = (embed["out_table"] + temb.unsqueeze(1)).chunk(2, dim=1)
     if fused:
         x = x.contiguous()
         pending: Pending = None
-        for w in blocks:
-            x, pending = block_forward_fused(x, pending, text, tproj, rope, w, cfg, attn_core, group, exchange)
+        for w, a, c in zip(blocks, lora, kv):
+            x, pending = block_forward_fused(x, pending, text, tproj, rope, w, cfg, attn_core, group, exchange, a, c)
         add, add_gate = pending if pending is not None else (None, None)
         h = ops.dit_row_norm(x, add=add, gate=add_gate, x_out=x if add is not None else None,
                              scale=scale.contiguous(), shift=shift.contiguous(), eps=cfg.eps)
     else:
-        for w in blocks:
-            x = block_forward(x, text, tproj, rope, w, cfg, attn_core, group)
+        for w, a, c in zip(blocks, lora, kv):
+            x = block_forward(x, text, tproj, rope, w, cfg, attn_core, group, a, c)
         h = (F.layer_norm(x.float(), (cfg.hidden,), eps=cfg.eps) * (1 + scale) + shift).to(x.dtype)
     return F.linear(h, embed["proj_out"], embed["proj_out_b"])
 
