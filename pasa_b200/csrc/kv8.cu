@@ -11,7 +11,8 @@
 //
 //   write      rounds new tokens into pages.  Where a page has earlier tokens its
 //              scale is the larger of theirs and the new ones', and they are
-//              rounded again to it.  Bound: HBM, 2 bytes read and 1 written a value.
+//              rounded again to it.  Bound: HBM, 2 bytes read and 1 written a value
+//              (4680 tokens, 12 heads of 128, 43 MB: 12 us, 3.6 TB/s).
 //   attention  out = softmax(q k^T scale) v over a request's first `length`
 //              tokens.  Bound: the tensor cores for many queries, HBM (one byte a
 //              value) for single tokens.
@@ -28,12 +29,24 @@
 //
 // Work split.  A unit is a request, a key/value head and 256 of the rows
 // (query, query head of the group) that attend with it; its cost is its steps of
-// 128 tokens and two more.  The line of all units is cut into equal parts, one
+// 128 tokens and an overhead.  The line of all units is cut into equal parts, one
 // for each of the GPU's SMs, so neither the number of units nor their lengths
 // leave SMs idle; a unit that is cut leaves its parts (fp32 sums, maximum and
-// denominator) in the workspace, and a second kernel joins them.  With at most
-// 128 rows (single tokens) the two tiles of a unit hold the same rows and take
-// the steps in turn, which hides the one's softmax behind the other's products.
+// denominator) in the workspace, and a second kernel joins them in order.  With
+// at most 128 rows the two tiles of a unit hold the same rows and take the steps
+// in turn, which hides the one's softmax behind the other's products.  With at
+// most 32 rows (single tokens) each of a tile's four warps has those rows and a
+// quarter of a step's tokens as well, and the ring of keys and values is twice as
+// long: 80 us for 333 MB of pages (8 requests of 130 to 32767 tokens, 8 heads of
+// 128), 147 us with one warp of four at work and the shorter ring.
+//
+// What bounds it (12 heads, 4680 queries over 18720 tokens, D = 128: 537 us, 1.0
+// PFLOP/s, 2.0 with both terms counted): a step of a pair of tiles takes 4200 clocks,
+// of which the products take 2100, 2^x 2050 and the conversions 2050.  They
+// overlap between the two tiles only, since scores, probabilities and outputs of
+// two tiles fill TMEM; 64-token steps with two places for scores made the products
+// the bound (585 us: one of N = 64 takes as long as one of N = 128), and 16 softmax
+// warps in place of 8 took 587 us.
 #include <cuda_fp16.h>
 
 #include "umma.cuh"
@@ -1059,7 +1072,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 // Joins the parts of a unit that was cut.  Block (c, y): the unit that begins in
 // CTA c's part of the line and goes on in the next; a warp a row at a time.  The
 // parts' maxima and denominators are read by a lane each, so that the loads of
-// their sums wait for nothing.
+// their sums wait for nothing: 20 us for 147 cut units of 256 rows, 6 us for 5.
 constexpr int kJoinWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Args a, int parts) {
@@ -1094,10 +1107,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       const float fall = exp2_ftz(fmaxf(m - top, -200.f)), share = exp2_ftz(fmaxf(ml.x - top, -200.f));
-      float sum = ml.y * share;
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      l = l * fall + sum;
+      const float part_l = ml.y * share;
+      l *= fall;
       m = top;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) o[i] *= fall;
@@ -1106,6 +1117,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
       for (; left != 0; left &= left - 1) {
         const int src = __ffs(int(left)) - 1;
         const float f = __shfl_sync(0xffffffffu, share, src);
+        l += __shfl_sync(0xffffffffu, part_l, src);  // (in order, wherever CTAs without ticks lie)
         const float* from = a.part_o + __shfl_sync(0xffffffffu, mine, src) * D + lane * kCols;
         float x[kCols];
         if constexpr (kCols == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);

@@ -14,7 +14,9 @@
 // and dy.  h and g are R wide; passing them through memory costs R / K of the
 // traffic and lets each kernel split its own long axis: down splits K over a
 // cluster of up to 8 CTAs when there are few rows (the partial sums meet in
-// distributed shared memory, in rank order), up splits N.
+// distributed shared memory, in rank order), up splits N.  Measured: 75600 rows,
+// 5120 -> 5120, R = 32: down 133 us (5.8 TB/s), up 328 us (4.7 TB/s); 32760 rows,
+// R = 64: grad 137 us (4.9 TB/s).
 //
 // Rounding: h and g are products' operands again, and are kept as two bf16
 // terms, v = hi + lo to 2^-17 of v, each multiplied and accumulated in fp32:

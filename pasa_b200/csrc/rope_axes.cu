@@ -17,7 +17,8 @@
 // of one 16-byte vector of one token and applies them to up to kMaxHeads heads
 // (of q and of k), four heads' loads in flight.  With fewer tokens than fill
 // the GPU the heads are split over more threads instead, down to one head a
-// thread.
+// thread.  Measured: q and k of 75600 tokens, 40 heads of 128 (3.1 GB moved) in
+// 515 us, 6.0 TB/s.
 #include "common.cuh"
 
 namespace pasa {
