@@ -388,10 +388,7 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool b_mn_major)
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() {  // all but the last N groups have landed
-  asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
-}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <int N> __device__ __forceinline__ void set_max_registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N));
@@ -727,7 +724,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               cp_async16(smem_u32(place(row)) + uint32_t((c & 7) * 16 + (c >> 3) * kTile * 128),
                          q + row_offset(a, a.qs, r0 + (row & mask)));
           }
-          cp_async_commit();
         }
         auto split = [&](int x) {
           const int first = x * 8 * kLoaders + loader * 8, row = first + sub;
@@ -768,15 +764,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           }
           if (part == 0) q_scale[buf * 2 * kTile + row] = scale;
         };
-        static_assert(kRounds == 6, "the waits below");
+        cp_async_wait_all();
+        __syncwarp();
 #pragma unroll 1
-        for (int x = 0; x < kRounds; ++x) {
-          if (x == 0) cp_async_wait<4>();
-          else if (x == 2) cp_async_wait<2>();
-          else if (x == 4) cp_async_wait<0>();
-          __syncwarp();
-          split(x);
-        }
+        for (int x = 0; x < kRounds; ++x) split(x);
         if (loader == 0 && lane == 0) {
           if (!here) p.count = 0;
           work[buf] = p;
@@ -1306,8 +1297,8 @@ int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, con
   a.both = a.rows <= kTile ? 1 : 0;
   a.quarters = a.rows <= 32 ? 1 : 0;
   // a unit takes about as long as that many steps besides its own (one token, 8 requests of 130 to 32767: 165 us at 2,
-  // 92 at 12; 32760 queries over 512 and 77 tokens: 966 at 2, 840 at 5)
-  a.overhead = a.quarters ? 12 : 5;
+  // 92 at 12; 32760 queries over 512 and 77 tokens: 966 at 2, 810 at 4, 840 at 6)
+  a.overhead = a.quarters ? 12 : 4;
   a.scale_log2 = scale * kLog2e;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + size_t(sms) * 2 * 2 * kTile * size_t(dim));

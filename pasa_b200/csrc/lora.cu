@@ -1197,7 +1197,7 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   // first.  A unit costs its chunks and the time of about two more until its h
   // is in TMEM; blocks that are as good as equal still end up to one unit apart.
   double best = 0.0;
-  for (int64_t split = 1; split <= a.chunks; ++split) {
+  for (int64_t split = 1; split <= a.chunks && split <= 8 * sms; ++split) {
     const double time =
         (double(cdiv(busy_spans(r) * split, 2 * sms)) + 0.5) * (double(cdiv(a.chunks, split)) + 2.0);
     if (split == 1 || time < best * 0.98) { best = time; a.split = int(split); }
