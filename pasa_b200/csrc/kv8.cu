@@ -229,8 +229,7 @@ struct Args {
   uint32_t group_magic;        // 2^32 / group + 1, rounded down; 0 for 1
   int rows, blocks;            // rows of a key/value head (queries x group); units of 256 of them
   int overhead;                // steps' time that a unit takes besides its steps
-  int both;                    // 1: both tiles hold the same rows and take the steps in turn
-  int quarters;                // 1: so do the 4 warps of a tile, each with a quarter of a step's tokens
+  int quarters;                // 1: the 4 warps of a tile have the same rows, each with a quarter of a step's tokens
   float scale_log2;            // softmax scale * log2(e)
   float* part_o;               // [2 parts a CTA][256][D]
   float2* part_ml;             // [2 parts a CTA][256]: maximum, denominator
@@ -443,7 +442,8 @@ __device__ __forceinline__ void probabilities(const uint32_t (&s)[32], float mul
   }
 }
 
-template <int D>
+// both: both tiles hold the same rows and take the steps in turn.
+template <int D, bool both>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Maps maps,
                                                                 const __grid_constant__ Args a) {
   extern __shared__ unsigned char smem_raw[];
@@ -458,8 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   __shared__ Piece work[2];                      // what a buffer of queries is for; no steps: the end
   float* q_scale = reinterpret_cast<float*>(sm + kOffScale);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int both = a.both, slots = both ? kSlotsBoth : kSlots;
-  const int q_buf = both ? kQTile : kQBuf, ring = 2 * q_buf;  // bytes of a buffer of queries; the ring's place
+  constexpr int slots = both ? kSlotsBoth : kSlots;
+  constexpr int q_buf = both ? kQTile : kQBuf, ring = 2 * q_buf;  // bytes of a buffer of queries; the ring's place
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlotsBoth; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -698,8 +698,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         here = walk.next(a, p);
         const int r0 = p.u.block * 2 * kTile;
         // rows of the buffer; with quarters every 32 of them are the same
-        const int mask = a.quarters ? 31 : 255, kept = min(a.rows - r0, 2 * kTile);
-        const int live = !here ? 0 : a.quarters ? kTile : kept;
+        const bool quarters = both && a.quarters;
+        const int mask = quarters ? 31 : 255, kept = min(a.rows - r0, 2 * kTile);
+        const int live = !here ? 0 : quarters ? kTile : kept;
         if (here && p.zero) {
           for (int row = loader * 8 + sub; row < kept; row += kLoaders * 8) {
             __nv_bfloat16* dst = a.out + unit_offset(a, a.os, p.u) + row_offset(a, a.os, r0 + row) + part * 8;
@@ -785,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int t = (warp - 4) >> 2, w = warp & 3, row = w * 32 + lane;
     const uint32_t lanes = uint32_t(w * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + kColS + 128u * uint32_t(t), o_tmem = tmem + lanes + kColO + 128u * uint32_t(t);
-    const bool quarters = a.quarters;
+    const bool quarters = both && a.quarters;
     int buf = 0;
     uint32_t q_parity = 0, k_parity = 0;  // k_parity: of the tile's next step
     bool ok = true;
@@ -1174,9 +1175,10 @@ size_t part_bytes(int sms, int dim) { return size_t(sms) * 2 * 2 * kTile * (size
 
 template <int D>
 cudaError_t launch_attention(cudaStream_t st, const Maps& maps, const Args& a, int sms) {
-  cudaError_t e = cudaFuncSetAttribute(attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const auto kernel = a.rows <= kTile ? attention_kernel<D, true> : attention_kernel<D, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  attention_kernel<D><<<unsigned(sms), kThreads, kSmem, st>>>(maps, a);
+  kernel<<<unsigned(sms), kThreads, kSmem, st>>>(maps, a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int rows = a.rows < 2 * kTile ? a.rows : 2 * kTile;
@@ -1294,7 +1296,6 @@ int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, con
   a.group_magic = group == 1 ? 0u : uint32_t((uint64_t(1) << 32) / uint64_t(group) + 1);
   a.rows = int(queries * group);
   a.blocks = int(cdiv(a.rows, 2 * kTile));
-  a.both = a.rows <= kTile ? 1 : 0;
   a.quarters = a.rows <= 32 ? 1 : 0;
   // a unit takes about as long as that many steps besides its own (one token, 8 requests of 130 to 32767: 165 us at 2,
   // 92 at 12; 32760 queries over 512 and 77 tokens: 966 at 2, 810 at 4, 840 at 6)
