@@ -40,13 +40,13 @@
 // long: 80 us for 333 MB of pages (8 requests of 130 to 32767 tokens, 8 heads of
 // 128), 147 us with one warp of four at work and the shorter ring.
 //
-// What bounds it (12 heads, 4680 queries over 18720 tokens, D = 128: 537 us, 1.0
-// PFLOP/s, 2.0 with both terms counted): a step of a pair of tiles takes 4200 clocks,
-// of which the products take 2100, 2^x 2050 and the conversions 2050.  They
+// What bounds it (12 heads, 4680 queries over 18720 tokens, D = 128: 510 us, 1.05
+// PFLOP/s, 2.1 with both terms counted): a step of a pair of tiles takes some 4000
+// clocks, of which the products take 2100, 2^x 2050 and the conversions 2050.  They
 // overlap between the two tiles only, since scores, probabilities and outputs of
 // two tiles fill TMEM; 64-token steps with two places for scores made the products
-// the bound (585 us: one of N = 64 takes as long as one of N = 128), and 16 softmax
-// warps in place of 8 took 587 us.
+// the bound (585 us, from 537 then: one of N = 64 takes as long as one of N = 128),
+// and 16 softmax warps in place of 8 took 587 us.
 #include <cuda_fp16.h>
 
 #include "umma.cuh"
@@ -1062,10 +1062,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 }
 
 // Joins the parts of a unit that was cut.  Block (c, y): the unit that begins in
-// CTA c's part of the line and goes on in the next; a warp a row at a time.  The
+// CTA c's part of the line and goes on in the next; a warp four rows.  The
 // parts' maxima and denominators are read by a lane each, so that the loads of
-// their sums wait for nothing: 20 us for 147 cut units of 256 rows, 6 us for 5.
-constexpr int kJoinWarps = 8;
+// their sums wait for nothing: 16 us for 147 cut units of 256 rows, 6 us for 5.
+constexpr int kJoinWarps = 8, kJoinRows = 4;
 template <int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Args a, int parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1087,41 +1087,62 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   const int part = line.begin(first) >= u.begin ? 0 : 1;  // the first one's; the others' begin with the unit
   constexpr int kCols = D / 32;
   const int rows = min(a.rows - u.block * 2 * kTile, 2 * kTile);
-  for (int row = int(blockIdx.y) * kJoinWarps + warp; row < rows; row += int(gridDim.y) * kJoinWarps) {
-    float o[kCols] = {}, m = -INFINITY, l = 0.f;
-    for (int c0 = 0; c0 < count; c0 += 32) {
-      const int c = c0 + lane;
-      const int64_t mine = (int64_t(first + c) * 2 + (c ? 0 : part)) * 2 * kTile + row;
-      // (with fewer ticks than CTAs some have none)
-      const bool some = c < count && line.begin(first + c + 1) > line.begin(first + c);
-      const float2 ml = some ? a.part_ml[mine] : make_float2(-INFINITY, 0.f);
-      float top = fmaxf(m, ml.x);
+  const int row0 = (int(blockIdx.y) * kJoinWarps + warp) * kJoinRows;
+  if (row0 >= rows) return;
+  float o[kJoinRows][kCols] = {}, m[kJoinRows], l[kJoinRows] = {};
+#pragma unroll
+  for (int x = 0; x < kJoinRows; ++x) m[x] = -INFINITY;
+  for (int c0 = 0; c0 < count; c0 += 32) {
+    const int c = c0 + lane;
+    const int64_t mine = (int64_t(first + c) * 2 + (c ? 0 : part)) * 2 * kTile + row0;
+    // (with fewer ticks than CTAs some have none)
+    const bool some = c < count && line.begin(first + c + 1) > line.begin(first + c);
+    float2 ml[kJoinRows];
+    float share[kJoinRows];
+#pragma unroll
+    for (int x = 0; x < kJoinRows; ++x)
+      ml[x] = some && row0 + x < rows ? a.part_ml[mine + x] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int x = 0; x < kJoinRows; ++x) {
+      float top = fmaxf(m[x], ml[x].x);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      const float fall = exp2_ftz(fmaxf(m - top, -200.f)), share = exp2_ftz(fmaxf(ml.x - top, -200.f));
-      const float part_l = ml.y * share;
-      l *= fall;
-      m = top;
+      const float fall = exp2_ftz(fmaxf(m[x] - top, -200.f));
+      share[x] = exp2_ftz(fmaxf(ml[x].x - top, -200.f));
+      l[x] *= fall;
+      m[x] = top;
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) o[i] *= fall;
-      uint32_t left = __ballot_sync(0xffffffffu, ml.y != 0.f);  // (one without tokens has no sums)
-#pragma unroll 4
-      for (; left != 0; left &= left - 1) {
-        const int src = __ffs(int(left)) - 1;
-        const float f = __shfl_sync(0xffffffffu, share, src);
-        l += __shfl_sync(0xffffffffu, part_l, src);  // (in order, wherever CTAs without ticks lie)
-        const float* from = a.part_o + __shfl_sync(0xffffffffu, mine, src) * D + lane * kCols;
-        float x[kCols];
-        if constexpr (kCols == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
-        else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from);
+      for (int i = 0; i < kCols; ++i) o[x][i] *= fall;
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, some); left != 0; left &= left - 1) {
+      const int src = __ffs(int(left)) - 1;
+      const float* from = a.part_o + __shfl_sync(0xffffffffu, mine, src) * D + lane * kCols;
+      float v[kJoinRows][kCols];
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) o[i] = fmaf(x[i], f, o[i]);
+      for (int x = 0; x < kJoinRows; ++x) {
+        if (row0 + x >= rows) continue;
+        if constexpr (kCols == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(from + x * D);
+        else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(from + x * D);
+      }
+#pragma unroll
+      for (int x = 0; x < kJoinRows; ++x) {  // (in order, wherever CTAs without ticks lie)
+        const float f = __shfl_sync(0xffffffffu, share[x], src), part_l = __shfl_sync(0xffffffffu, ml[x].y, src);
+        if (part_l == 0.f) continue;  // (one without tokens has no sums)
+        l[x] = fmaf(part_l, f, l[x]);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) o[x][i] = fmaf(v[x][i], f, o[x][i]);
       }
     }
-    __nv_bfloat16* out = a.out + unit_offset(a, a.os, u) + row_offset(a, a.os, u.block * 2 * kTile + row) + lane * kCols;
-    const float inv = 1.f / l;
+  }
+  __nv_bfloat16* out = a.out + unit_offset(a, a.os, u) + lane * kCols;
 #pragma unroll
-    for (int i = 0; i < kCols; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+  for (int x = 0; x < kJoinRows; ++x) {
+    if (row0 + x >= rows) continue;
+    __nv_bfloat16* at = out + row_offset(a, a.os, u.block * 2 * kTile + row0 + x);
+    const float inv = 1.f / l[x];
+#pragma unroll
+    for (int i = 0; i < kCols; i += 2)
+      *reinterpret_cast<uint32_t*>(at + i) = pack_bf16x2(o[x][i] * inv, o[x][i + 1] * inv);
   }
 }
 
@@ -1179,11 +1200,10 @@ cudaError_t launch_attention(cudaStream_t st, const Maps& maps, const Args& a, i
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   kernel<<<unsigned(sms), kThreads, kSmem, st>>>(maps, a);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int rows = a.rows < 2 * kTile ? a.rows : 2 * kTile;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(sms - 1), unsigned(cdiv(rows, 4 * kJoinWarps)));
+  cfg.gridDim = dim3(unsigned(sms - 1), unsigned(cdiv(rows, kJoinRows * kJoinWarps)));
   cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
