@@ -418,3 +418,34 @@ def test_streams_and_graph(cuda_device):
             g.replay()
             check_attention(out, q, p, [x + 1 for x in lengths])
     ops.check_operator_errors()
+
+
+def test_pages_past_4_gib(cuda_device):
+    """A cache of more than 2^32 bytes for keys and for values, its last pages in use; 2^31 elements between the
+    queries' requests."""
+    heads, dim, tokens = 8, 128, 700
+    cache = ops.kv8_cache(66000, heads, dim)
+    assert cache.k.numel() > 1 << 32
+    p = Pages([tokens], heads, dim)
+    p.cache, p.pages = cache, 66000
+    p.rows = [[66000 - 1 - 5 * i for i in range(11)]]
+    p.table = i32(p.rows)
+    p.fill(spread=True)
+    store = torch.empty(2 * (1 << 31) + 64 * heads * dim, dtype=torch.bfloat16, device="cuda")
+    q = store.as_strided((2, heads, 3, dim), ((1 << 31) + 512, dim, heads * dim, 1))
+    q.copy_(randn(2, heads, 3, dim, seed=4))
+    out = ops.kv8_attention(q, cache, p.table.expand(2, -1), i32([tokens, 130]))
+    ops.check_operator_errors()
+    p.rows = p.rows * 2
+    check_attention(out, q, p, [tokens, 130])
+
+
+@pytest.mark.parametrize("queries,group", [(1, 33), (1, 32), (4, 8), (127, 1), (43, 3)])
+def test_row_counts_at_the_kernels_edges(cuda_device, queries, group):
+    """32 and 33, 127 to 129 rows: quarters of a step, copies of the rows, two tiles."""
+    for n in (1, 31, 33, 64, 97, 129, 385):
+        p = Pages([n, 0, n + 700], 1, 64).fill(spread=True)
+        q = randn(3, group, queries, 64, seed=n)
+        out = ops.kv8_attention(q, p.cache, p.table, i32(p.lengths))
+        ops.check_operator_errors()
+        check_attention(out, q, p)

@@ -312,3 +312,12 @@ def test_stream_and_graph(cuda_device):
             p.check_grads(*results[1:])
     assert torch.isfinite(alive).all()
     ops.check_operator_errors()
+
+
+@pytest.mark.parametrize("most", [1, 9])
+def test_many_requests(cuda_device, most):
+    """More requests than a warp or a block looks through at once, single rows and none among them."""
+    lengths = [(7 * i) % (most + 1) for i in range(700)]
+    p = Problem(lengths, 128, 192, 16, 37, slots=[(11 * i) % 39 - 1 for i in range(700)], lead=3, tail=5)
+    p.check_out(ops.lora_update(p.y, *p.args))
+    p.check_grads(*ops.lora_update_backward(p.dy, *p.args))
