@@ -46,7 +46,9 @@
 // overlap between the two tiles only, since scores, probabilities and outputs of
 // two tiles fill TMEM; 64-token steps with two places for scores made the products
 // the bound (585 us, from 537 then: one of N = 64 takes as long as one of N = 128),
-// and 16 softmax warps in place of 8 took 587 us.
+// 16 softmax warps in place of 8 took 587 us, and probabilities in shared memory,
+// which lets the scores run ahead, 554: products with both operands there take all
+// of its bandwidth, and barriers and copies wait behind them.
 #include <cuda_fp16.h>
 
 #include "umma.cuh"

@@ -449,3 +449,35 @@ def test_row_counts_at_the_kernels_edges(cuda_device, queries, group):
         out = ops.kv8_attention(q, p.cache, p.table, i32(p.lengths))
         ops.check_operator_errors()
         check_attention(out, q, p)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lengths,heads,group,queries", [
+    ([1], 1, 1, 129), ([0], 2, 1, 300), ([63, 65, 127, 128, 129], 2, 1, 200), ([700, 90, 0], 1, 1, 129),
+    ([200, 64], 2, 2, 200), ([513], 1, 1, 256), ([77, 512], 3, 1, 700), ([130, 1, 257] * 40, 1, 2, 150), ([6000, 300], 1, 3, 100)])
+def test_wide_tables(cuda_device, dim, lengths, heads, group, queries):
+    """Tables of many pages for each request, of which few are in use; several units of two tiles, and of one that is
+    not full, for each block."""
+    p = Pages(lengths, heads, dim, width=100).fill(spread=True)
+    q = randn(len(lengths), heads * group, queries, dim, seed=9)
+    out = ops.kv8_attention(q, p.cache, p.table, i32(lengths))
+    ops.check_operator_errors()
+    check_attention(out, q, p)
+    for _ in range(3):
+        assert torch.equal(out, ops.kv8_attention(q, p.cache, p.table, i32(lengths)))
+    if lengths != [6000, 300]:
+        narrow = p.table[:, :max(1, -(-max(lengths) // 64))]
+        check_attention(ops.kv8_attention(q, p.cache, narrow, i32(lengths)), q, p)
+
+
+def test_wide_tables_sharp_scores_and_nan(cuda_device):
+    p = Pages([700, 300], 1, 64, width=40).fill()
+    for q in (p.values(0, 0, 700)[0][300].bfloat16().expand(2, 1, 300, 64) * 20, randn(2, 1, 300, 64) * 30,
+              torch.zeros(2, 1, 300, 64, device="cuda").bfloat16()):
+        check_attention(ops.kv8_attention(q, p.cache, p.table, i32([700, 300])), q, p)
+    q = randn(2, 1, 300, 64)
+    clean = ops.kv8_attention(q, p.cache, p.table, i32([700, 300]))
+    q[0, 0, 7, 3] = float("inf")
+    out = ops.kv8_attention(q, p.cache, p.table, i32([700, 300]))
+    keep = torch.arange(300, device="cuda") != 7
+    assert out[0, 0, 7].isnan().all() and torch.equal(out[0, 0, keep], clean[0, 0, keep]) and torch.equal(out[1], clean[1])
