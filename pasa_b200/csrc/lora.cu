@@ -27,6 +27,8 @@
 // the kernels for few rows) and at every request's first row, and ends at the
 // next of either, so a span has one adapter.  Every block finds its span from `rows` on the device (no host
 // copy; a captured graph follows new lengths).
+#include <atomic>
+
 #include "umma.cuh"
 
 namespace pasa {
@@ -948,10 +950,10 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
         unsigned char* st = sm + c.at * a.ring.stage_bytes;
         const int rows = valid[c.at];
         if (rows < stage_rows) {  // zero the other rows of every box
-          const int per_box = (stage_rows - rows) * 8, boxes = width / 64 + 2 * a.atoms;
-          for (int j = lane; j < boxes * per_box; j += 32)
-            *reinterpret_cast<uint4*>(st + (j / per_box) * box + rows * 128 + (j % per_box) * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
+          const int boxes = width / 64 + 2 * a.atoms;
+          for (int b = 0; b < boxes; ++b)
+            for (int at = rows * 128 + lane * 16; at < box; at += 512)
+              *reinterpret_cast<uint4*>(st + b * box + at) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
           __syncwarp();
         }
@@ -1118,9 +1120,17 @@ Ring ring_of(int stage_bytes, int room) {
   return Ring{stages, stage_bytes};
 }
 
-template <typename F>
-cudaError_t allow_smem(F kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Lets a kernel have `bytes` (the same for every call) of shared memory; once for each device.
+template <auto kKernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (e != cudaSuccess || (done.load(std::memory_order_acquire) & bit)) return e;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // at most: every segment ends one
@@ -1155,7 +1165,7 @@ cudaError_t down(cudaStream_t st, const Rows& r, Matrix u, int64_t c, const void
   a.split = 1;
   while (a.split < 8 && busy_spans(r) * a.split * 2 <= 2 * sms && a.steps >= a.split * 4) a.split *= 2;
   const int smem = a.room + 1024;
-  cudaError_t e = allow_smem(down_kernel<MN>, smem);
+  cudaError_t e = allow_smem<down_kernel<MN>>(smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(span_count(r) * a.split));
@@ -1204,7 +1214,7 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   }
   const int64_t units = span_count(r) * a.split;
   const int smem = a.room + 1024;
-  cudaError_t e = allow_smem(up_kernel<MN>, smem);
+  cudaError_t e = allow_smem<up_kernel<MN>>(smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(units < 2 * sms ? units : 2 * sms));
@@ -1275,24 +1285,27 @@ cudaError_t down_a(cudaStream_t st, const Rows& r, Matrix x, int64_t k, const vo
 int64_t grad_blocks(int64_t c, int rank) { return cdiv(c, grad_cols(rank <= 64 ? 1 : 2)); }
 
 // Shares of the rows, of 1 to 3 waves of blocks (a block takes an SM for
-// itself): those with the least time, counted in stages.  A block takes as long
-// as about six more to begin and to put its sums down, and every share is read
-// again by the second kernel.  (20 column blocks and 1024 stages: 7 shares take
-// 127 us, 22 take 146 us.)
-int grad_shares(int64_t m, int64_t blocks, int rank, int sms) {
-  const double stages = double(m) / double(grad_rows(rank <= 64 ? 1 : 2));
+// itself): those with the least time, counted in stages.  Every request ends a
+// stage.  A block takes as long as about six more for every adapter that it
+// puts down, and every share is read again by the second kernel.  (20 column
+// blocks and 1024 stages: 7 shares take 127 us, 22 take 146 us; 27 rows of 16
+// adapters, 240 and 224 columns, rank 120: 8 shares take 35 us, one 220 us.)
+int grad_shares(int64_t m, int64_t blocks, int rank, int64_t adapters, int64_t requests, int sms) {
+  const int64_t busy = requests < m ? requests : m, pieces = busy < adapters ? busy : adapters;
+  const double stages = double(m) / double(grad_rows(rank <= 64 ? 1 : 2)) + double(busy) * 0.5;
   int64_t best = 1;
   double best_time = 0.0;
-  for (int64_t shares = 1; shares == 1 || (blocks * shares <= 3 * sms && double(shares) * 4.0 <= stages); ++shares) {
+  for (int64_t shares = 1; shares == 1 || (blocks * shares <= 3 * sms && double(shares) <= stages); ++shares) {
+    const double put = 6.0 * double(cdiv(pieces, shares)) + (shares > 1 ? 6.0 : 0.0) * double(pieces > 1);
     const double time =
-        double(cdiv(blocks * shares, sms)) * (stages / double(shares) + 6.0) + 0.5 * double(shares > 1 ? shares : 0);
+        double(cdiv(blocks * shares, sms)) * (stages / double(shares) + put) + 0.5 * double(shares > 1 ? shares : 0);
     if (shares == 1 || time < best_time) { best = shares; best_time = time; }
   }
   return int(best);
 }
 
-size_t grad_partial_bytes(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int sms) {
-  const int64_t shares = grad_shares(m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, sms);
+size_t grad_partial_bytes(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int64_t requests, int sms) {
+  const int64_t shares = grad_shares(m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, adapters, requests, sms);
   return shares > 1 ? size_t(shares + adapters) * size_t(rank) * size_t(k + n) * 4 : 0;
 }
 
@@ -1317,13 +1330,13 @@ cudaError_t grad(cudaStream_t st, const Rows& r, int rank, Matrix x, int64_t k, 
   a.blocks[0] = grad_blocks(k, rank);
   a.blocks[1] = grad_blocks(n, rank);
   const int64_t blocks = (da ? a.blocks[0] : 0) + (db ? a.blocks[1] : 0);
-  a.shares = grad_shares(r.m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, sms);
+  a.shares = grad_shares(r.m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, r.adapters, r.requests, sms);
   a.partial = static_cast<float*>(workspace);
   a.out[0] = static_cast<__nv_bfloat16*>(da);
   a.out[1] = static_cast<__nv_bfloat16*>(db);
   a.err = err;
   const int smem = a.ring.stages * a.ring.stage_bytes + list + 1024;
-  cudaError_t e = allow_smem(grad_kernel, smem);
+  cudaError_t e = allow_smem<grad_kernel>(2 * kSmemTwo);
   if (e != cudaSuccess) return e;
   grad_kernel<<<unsigned(blocks * a.shares), kThreads, smem, st>>>(maps, a);
   e = cudaGetLastError();
@@ -1408,7 +1421,7 @@ int pasa_lora_backward_workspace_size(int64_t m, int64_t k, int64_t n, int rank,
   if ((st = device_sms(&sms))) return st;
   size_t h = 0;
   pasa_lora_h_size(m, rank, &h);
-  *bytes = align256(h) + (m && requests ? grad_partial_bytes(m, k, n, rank, adapters, sms) : 0);
+  *bytes = align256(h) + (m && requests ? grad_partial_bytes(m, k, n, rank, adapters, requests, sms) : 0);
   return PASA_OK;
 }
 

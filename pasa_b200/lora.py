@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -45,6 +46,15 @@ def _target(t: torch.Tensor, name: str, shape, device):
         raise ValueError(f"{name} is written in place: it must be 16-byte aligned with unit column stride and a row "
                          "stride that is a multiple of 8")
     return m, cols if rows <= 1 else step
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(m, k, n, rank, adapters, requests, index: int) -> int:
+    size = ctypes.c_size_t()
+    with torch.cuda.device(index):
+        _lib.check("pasa_lora_backward_workspace_size", _lib.load().pasa_lora_backward_workspace_size(
+            m, k, n, rank, adapters, requests, ctypes.byref(size)))
+    return size.value
 
 
 class _Call:
@@ -136,15 +146,12 @@ def _backward(call: _Call, dy, x_shape, h, dx, need_x, need_a, need_b):
         h = call.h()
     da = torch.empty_like(call.a) if need_a else None
     db = torch.empty_like(call.b) if need_b else None
-    size = ctypes.c_size_t()
-    with torch.cuda.device(call.device):
-        _lib.check("pasa_lora_backward_workspace_size", _lib.load().pasa_lora_backward_workspace_size(
-            call.m, call.k, call.n, call.rank, call.adapters, call.requests, ctypes.byref(size)))
-    workspace = torch.empty(size.value, dtype=torch.uint8, device=call.device)
+    size = _workspace_bytes(call.m, call.k, call.n, call.rank, call.adapters, call.requests, call.device.index)
+    workspace = torch.empty(size, dtype=torch.uint8, device=call.device)
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     launch("pasa_lora_update_backward", call.device, grad.data_ptr(), lddy, call.x.data_ptr(), call.ldx, *call.weights,
            *call.sizes, h.data_ptr(), int(given), base or None, ldbase, target.data_ptr() if dx is not None else None,
-           lddx if dx is not None else 0, ptr(da), ptr(db), workspace.data_ptr(), size.value)
+           lddx if dx is not None else 0, ptr(da), ptr(db), workspace.data_ptr(), size)
     return dx, da, db
 
 
