@@ -1289,7 +1289,7 @@ int64_t grad_blocks(int64_t c, int rank) { return cdiv(c, grad_cols(rank <= 64 ?
 // stage.  A block takes as long as about six more for every adapter that it
 // puts down, and every share is read again by the second kernel.  (20 column
 // blocks and 1024 stages: 7 shares take 127 us, 22 take 146 us; 27 rows of 16
-// adapters, 240 and 224 columns, rank 120: 8 shares take 35 us, one 220 us.)
+// adapters, 240 and 224 columns, rank 120: 8 shares take 24 us, one 153 us.)
 int grad_shares(int64_t m, int64_t blocks, int rank, int64_t adapters, int64_t requests, int sms) {
   const int64_t busy = requests < m ? requests : m, pieces = busy < adapters ? busy : adapters;
   const double stages = double(m) / double(grad_rows(rank <= 64 ? 1 : 2)) + double(busy) * 0.5;
