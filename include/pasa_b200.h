@@ -533,8 +533,9 @@ PASA_API int pasa_kv8_write(void* stream, const void* k, const int64_t* k_stride
  *   scale   positive
  *   workspace  pasa_kv8_attention_workspace_size bytes, not shared by two calls
  *           that may run at the same time
- * Probabilities and queries enter the products to 8 significant bits or 2^-16 of
- * the row's largest, sums are fp32.
+ * Queries enter the products to 8 significant bits or 2^-17 of the row's largest,
+ * probabilities to 11 or 2^-36 of the row's largest (times its value scale), sums
+ * are fp32.
  */
 PASA_API int pasa_kv8_attention_workspace_size(int dim, size_t* bytes);
 PASA_API int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, const void* k_cache,

@@ -17,15 +17,18 @@
 //              tokens.  Bound: the tensor cores for many queries, HBM (one byte a
 //              value) for single tokens.
 //
-// Attention on the tensor cores (tcgen05) takes the pages as they are, without
-// converting them: both products run on e4m3 operands (twice the rate of bf16),
-// and the 16-bit operand of each goes in as two e4m3 terms, hi + lo.  A bf16
-// value has 8 significant bits and an e4m3 value 4, so q = s (hi + lo) is exact
-// for a row's elements down to 2^-11 of its largest, and 2^-19 of the largest
-// off below (s: a power of two for each row); the probabilities are kept to 8
-// significant bits or 2^-16 of the largest, as a bf16 one would be.  The two
-// terms together take the time of one bf16 product and read 8-bit keys and
-// values from shared memory.  Scores, maxima, sums and the output are fp32.
+// Attention on the tensor cores (tcgen05).  The scores' products run on the pages
+// as they are: a bf16 value has 8 significant bits and an e4m3 value 4, so a query
+// goes in as two e4m3 terms, q = s (hi + lo) (s: a power of two for each row), exact
+// for a row's elements down to 2^-9 of its largest and 2^-17 of the largest off
+// below.  The two terms take the time of one bf16 product (e4m3 has twice its rate)
+// and read 8-bit keys from shared memory.  The probabilities' products run in fp16:
+// four warps widen the values once, which is exact, and a probability is held times
+// 2^11 over a reference that lags the maximum by up to 2^4.  So it keeps 11
+// significant bits, or 2^-36 of the largest, and a long tail far below one key
+// weighs what the denominator says.  (As two e4m3 terms, which end at 2^-14 of the
+// largest, half of such a tail of 18720 tokens was lost.)  Scores, maxima, sums and
+// the output are fp32.
 //
 // Work split.  A unit is a request, a key/value head and 256 of the rows
 // (query, query head of the group) that attend with it; its cost is its steps of
@@ -36,19 +39,19 @@
 // at most 128 rows the two tiles of a unit hold the same rows and take the steps
 // in turn, which hides the one's softmax behind the other's products.  With at
 // most 32 rows (single tokens) each of a tile's four warps has those rows and a
-// quarter of a step's tokens as well, and the ring of keys and values is twice as
-// long: 80 us for 333 MB of pages (8 requests of 130 to 32767 tokens, 8 heads of
-// 128), 147 us with one warp of four at work and the shorter ring.
+// quarter of a step's tokens as well, and the rings of keys and values are longer.
 //
-// What bounds it (12 heads, 4680 queries over 18720 tokens, D = 128: 510 us, 1.05
-// PFLOP/s, 2.1 with both terms counted): a step of a pair of tiles takes some 4000
-// clocks, of which the products take 2100, 2^x 2050 and the conversions 2050.  They
-// overlap between the two tiles only, since scores, probabilities and outputs of
-// two tiles fill TMEM; 64-token steps with two places for scores made the products
-// the bound (585 us, from 537 then: one of N = 64 takes as long as one of N = 128),
-// 16 softmax warps in place of 8 took 587 us, and probabilities in shared memory,
-// which lets the scores run ahead, 554: products with both operands there take all
-// of its bandwidth, and barriers and copies wait behind them.
+// What bounds it (12 heads, 4680 queries over 18720 tokens, D = 128: 530 us, 1.01
+// PFLOP/s): a step of a pair of tiles takes some 4000 clocks, of which the products
+// take 2100 and 2^x 2050.  They overlap between the two tiles only, since scores,
+// probabilities and outputs of two tiles fill TMEM; 64-token steps with two places
+// for scores made the products the bound (one of N = 64 takes as long as one of
+// N = 128).  Units of few steps (40 heads, 32760 queries over 512 and 77 tokens:
+// 840 us) wait for their queries, whose copying and splitting takes 15000 clocks a
+// buffer.  Single tokens (8 requests of 130 to 32767 tokens, 8 heads of 128, 333 MB
+// of pages: 103 us) wait for the chain scores, softmax, output of two tiles, some
+// 2700 clocks a step; widening the values is 14 us of it, and the rings' lengths
+// make no difference.
 #include <cuda_fp16.h>
 
 #include "umma.cuh"
@@ -196,24 +199,38 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_const
 // ---------------------------------------------------------------------------
 constexpr int kTile = 128;          // rows of a tile
 constexpr int kStep = 128;          // tokens of a step: two pages
-constexpr int kSlotBytes = kStep * 128;
-constexpr int kSlots = 4, kSlotsBoth = 8;  // ring of keys' and values' steps; more where a unit has 128 rows
+constexpr int kKeyBytes = kStep * 128;   // a step's keys
+constexpr int kRawBytes = kPage * 128;   // a page's values as they lie in the cache
+constexpr int kWideBytes = kPage * 256;  // in fp16: for every 64 dimensions the tokens' rows of 128 bytes
+// Places of the three rings; the second number where both tiles have the same rows.
+constexpr int key_slots(bool both) { return both ? 4 : 2; }
+constexpr int raw_slots(bool both) { return both ? 5 : 2; }
+constexpr int wide_slots(bool both) { return both ? 2 : 2; }
+constexpr int kMaxSlots = 5;
 constexpr int kScaleSteps = 8;      // ring of the steps' scales: a step's stay until both its products are done
 constexpr int kQTile = 2 * kTile * 128;  // hi, lo
 constexpr int kQBuf = 2 * kQTile;   // two tiles
-constexpr int kThreads = 512;       // 0 TMA, 1 MMA + TMEM, 2-3 and 12-15 queries, 4-7 and 8-11 softmax
+constexpr int kThreads = 640;       // 0 TMA, 1 MMA + TMEM, 2-3 and 12-15 queries, 4-7 and 8-11 softmax, 16-19 values
 constexpr int kLoaders = 6;
-constexpr float kLog2P = 4.f;       // probabilities are held times 2^4 ...
-constexpr float kRescale = 4.f;     // ... and their reference lags the maximum by up to 2^4: at most 2^8 < 448
-constexpr int kOffQ = 0;                        // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes], then the ring
-constexpr int kOffOut = 2 * kQBuf + kSlots * kSlotBytes;  // the output on its way, 16 KB
-constexpr int kOffScale = kOffOut + 16384;      // f32 [2 buffers][256 rows]: the queries' scales
-static_assert(2 * kQTile + kSlotsBoth * kSlotBytes == kOffOut, "both layouts end there");
+constexpr int kWideners = 4;
+constexpr int kRegisters = 96, kRegistersSoftmax = 128, kRegistersQueries = 88, kRegistersValues = 48;  // of a thread
+static_assert(2 * kRegistersSoftmax + 2 * kRegistersQueries + kRegistersValues <= kThreads / 128 * kRegisters,
+              "the warpgroups share what the block was launched with");
+constexpr float kLog2P = 11.f;      // probabilities are held times 2^11 ...
+constexpr float kRescale = 4.f;     // ... and their reference lags the maximum by up to 2^4: at most 2^15, fp16 ends at 2^16
+constexpr int kOffQ = 0;            // [2 buffers][2 tiles][hi, lo][128 rows][128 bytes], then the rings and the output
+constexpr int out_bytes(bool both) { return both ? 16384 : 8192; }  // on its way
+constexpr int off_keys(bool both) { return 2 * (both ? kQTile : kQBuf); }
+constexpr int off_raw(bool both) { return off_keys(both) + key_slots(both) * kKeyBytes; }
+constexpr int off_wide(bool both) { return off_raw(both) + raw_slots(both) * kRawBytes; }
+constexpr int off_out(bool both) { return off_wide(both) + wide_slots(both) * kWideBytes; }
+constexpr int kOffScale = off_out(true) + out_bytes(true);  // f32 [2 buffers][256 rows]: the queries' scales
+static_assert(off_out(false) + out_bytes(false) == kOffScale, "both layouts end there");
 constexpr int kSmem = kOffScale + 2 * 2 * kTile * 4 + 1024;
-// Tile t: scores at kColS + 128 t, over them the probabilities (of 32 tokens: hi
-// in the first 8 columns of their scores, lo in the next 8); output at kColO + 128 t.
+// Tile t: scores at kColS + 128 t, over them the probabilities (of 32 tokens: in the
+// first 16 columns of their scores); output at kColO + 128 t.
 constexpr uint32_t kColS = 0, kColO = 256;
-static_assert(kSmem + 1024 <= 232448, "shared memory budget");
+static_assert(kSmem + 4096 <= 232448, "shared memory budget");
 
 struct Maps {
   CUtensorMap k, v;
@@ -351,19 +368,12 @@ struct Walk {
   }
 };
 
-// A place in the ring of keys' and values' steps.  They lie there in the order in
-// which the products need them: where both tiles take every step K0 V0 K1 V1 ...,
-// where they take them in turn K0 K1 V0 K2 V1 K3 ...
+// A place in a ring and the parity of the phase that comes next there.
 struct Cursor {
   int at;
   uint32_t parity;
   __device__ __forceinline__ void next(int slots) {
     if (++at == slots) { at = 0; parity ^= 1u; }
-  }
-  __device__ __forceinline__ void skip(int n, int slots) {
-    const int to = at + n;
-    at = to % slots;
-    parity ^= uint32_t(to / slots) & 1u;
   }
 };
 
@@ -375,14 +385,8 @@ __device__ __forceinline__ void mma8_ss(uint32_t d, uint64_t a, uint64_t b, uint
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
       :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void mma8_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
-      :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool b_mn_major) {
+// The types' code is 0 for e4m3 under kind::f8f6f4 and for fp16 under kind::f16; fp32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_of(int M, int N, bool b_mn_major) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
@@ -419,9 +423,9 @@ __device__ __forceinline__ float scale_log2(const Args& a, float scale) {
   return float(int(v >> 23) - 127);
 }
 
-// 2^(x mul + shift) of 32 scores, as e4m3 terms hi + lo, and their sums.
-__device__ __forceinline__ void probabilities(const uint32_t (&s)[32], float mul_, float shift, uint32_t (&hi)[8],
-                                              uint32_t (&lo)[8], float2& sum0, float2& sum1) {
+// 2^(x mul + shift) of 32 scores in fp16, and their fp32 sums.
+__device__ __forceinline__ void probabilities(const uint32_t (&s)[32], float mul_, float shift, uint32_t (&p)[16],
+                                              float2& sum0, float2& sum1) {
   const float2 mul = make_float2(mul_, mul_), add = make_float2(shift, shift);
 #pragma unroll
   for (int e = 0; e < 32; e += 4) {
@@ -433,14 +437,8 @@ __device__ __forceinline__ void probabilities(const uint32_t (&s)[32], float mul
     sum0 = __fadd2_rn(sum0, x01);
     sum1 = __fadd2_rn(sum1, x23);
     const __half2 p01 = __floats2half2_rn(x01.x, x01.y), p23 = __floats2half2_rn(x23.x, x23.y);
-    const uint16_t h01 = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&p01));
-    const uint16_t h23 = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&p23));
-    const uint32_t b01 = e4m3x2_to_f16x2(h01), b23 = e4m3x2_to_f16x2(h23);
-    const __half2 l01 = __hsub2(p01, *reinterpret_cast<const __half2*>(&b01));
-    const __half2 l23 = __hsub2(p23, *reinterpret_cast<const __half2*>(&b23));
-    hi[e >> 2] = uint32_t(h01) | uint32_t(h23) << 16;
-    lo[e >> 2] = uint32_t(f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&l01))) |
-                 uint32_t(f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&l23))) << 16;
+    p[e >> 1] = *reinterpret_cast<const uint32_t*>(&p01);
+    p[(e >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&p23);
   }
 }
 
@@ -451,20 +449,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kSlotsBoth], empty[kSlotsBoth], q_full[2], q_empty[2], o_free[2];
+  __shared__ uint64_t key_full[kMaxSlots], key_empty[kMaxSlots], raw_full[kMaxSlots], raw_empty[kMaxSlots];
+  __shared__ uint64_t wide_full[kMaxSlots], wide_empty[kMaxSlots], q_full[2], q_empty[2], o_free[2];
   __shared__ uint64_t s_full[2], p_full[2][2], pv_done[2];  // of a tile; p_full: of a page of a step
   __shared__ uint32_t tmem_slot;
   __shared__ float2 step_scale[kScaleSteps][2];  // of a step's two pages: the keys' scale, log2 of the values'
+  __shared__ int raw_rows[kMaxSlots];            // tokens of a page of values; -1: the end
   __shared__ float2 copy_ml[2 * kTile];          // maximum and denominator of every copy of a row
   __shared__ uint64_t copies;
   __shared__ Piece work[2];                      // what a buffer of queries is for; no steps: the end
   float* q_scale = reinterpret_cast<float*>(sm + kOffScale);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int slots = both ? kSlotsBoth : kSlots;
-  constexpr int q_buf = both ? kQTile : kQBuf, ring = 2 * q_buf;  // bytes of a buffer of queries; the ring's place
+  constexpr int q_buf = both ? kQTile : kQBuf;  // bytes of a buffer of queries
+  constexpr int keys_at = off_keys(both), raw_at = off_raw(both), wide_at = off_wide(both), out_at = off_out(both);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlotsBoth; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kMaxSlots; ++s) {
+      mbar_init(&key_full[s], 1);
+      mbar_init(&key_empty[s], 1);
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], kWideners);
+      mbar_init(&wide_full[s], kWideners);
+      mbar_init(&wide_empty[s], 1);
+    }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], kLoaders);
       mbar_init(&q_empty[t], 1 + 8);  // the last product that reads it, and the softmax warps (its scales)
@@ -483,8 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp < 4 || warp >= 12) {
-    set_max_registers_down<96>();
+  if (warp < 4 || (warp >= 12 && warp < 16)) {
+    set_max_registers_down<kRegistersQueries>();
     if (warp == 0) {
       // ================= keys and values =================
       Walk walk(a, lane);
@@ -501,8 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       Piece p, after;
       bool more = next_steps(p), ok = true;
       int coming = more ? entry(p, 0) : 0;  // the entry for the next 16 steps of keys, read that much ahead
-      Cursor c{0, 1};
-      int issued = 0, step = 0;  // step: of step_scale
+      Cursor keys{0, 1}, raw{0, 1};
+      int issued_keys = 0, issued_raw = 0, step = 0;  // step: of step_scale
       for (bool more_after; more && ok; more = more_after, p = after) {
         more_after = next_steps(after);
         const int n = p.count, ahead = both ? 2 : 1;
@@ -530,61 +537,95 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             }
           }
           const int pages = values ? v_pages : k_pages, at = 2 * (j & 15);
-          const int z0 = __shfl_sync(0xffffffffu, pages, at) * a.heads + p.u.head;
-          const int z1 = __shfl_sync(0xffffffffu, pages, at + 1) * a.heads + p.u.head;
+          const int z[2] = {__shfl_sync(0xffffffffu, pages, at) * a.heads + p.u.head,
+                            __shfl_sync(0xffffffffu, pages, at + 1) * a.heads + p.u.head};
+          if (values) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&raw_empty[raw.at], raw.parity));
+              if (!ok) break;
+              if (elect_one()) {
+                const int rows = min(max(p.u.tokens - (p.first + j) * kStep - h * kPage, 0), kPage);
+                raw_rows[raw.at] = rows;
+                if (rows > 0) {
+                  mbar_arrive_expect_tx(&raw_full[raw.at], uint32_t(kPage * D));
+                  tma_load_3d(sm + raw_at + raw.at * kRawBytes, &maps.v, &raw_full[raw.at], 0, 0, z[h]);
+                } else {
+                  mbar_arrive(&raw_full[raw.at]);
+                }
+              }
+              __syncwarp();
+              ++issued_raw;
+              raw.next(raw_slots(both));
+            }
+            continue;
+          }
           const bool second = pages_left(p, j) > 1;
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[c.at], c.parity));
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&key_empty[keys.at], keys.parity));
           if (!ok) break;
           if (elect_one()) {
-            unsigned char* dst = sm + ring + c.at * kSlotBytes;
-            const CUtensorMap* map = values ? &maps.v : &maps.k;
-            tma_load_3d(dst, map, &full[c.at], 0, 0, z0);
-            if (second) tma_load_3d(dst + kSlotBytes / 2, map, &full[c.at], 0, 0, z1);
+            unsigned char* dst = sm + keys_at + keys.at * kKeyBytes;
+            tma_load_3d(dst, &maps.k, &key_full[keys.at], 0, 0, z[0]);
+            if (second) tma_load_3d(dst + kKeyBytes / 2, &maps.k, &key_full[keys.at], 0, 0, z[1]);
           }
           // the scales are on their way while the tiles are: what the barrier expects comes behind them
-          if (!values) {
-            if ((j & 15) == 0) scales.y = scale_log2(a, scales.y);
-            if ((lane >> 1) == (j & 15)) step_scale[step % kScaleSteps][lane & 1] = scales;
-            ++step;
+          if ((j & 15) == 0) scales.y = scale_log2(a, scales.y);
+          if ((lane >> 1) == (j & 15)) step_scale[step % kScaleSteps][lane & 1] = scales;
+          ++step;
+          __syncwarp();
+          if (elect_one())
+            mbar_arrive_expect_tx(&key_full[keys.at], second ? uint32_t(kKeyBytes) : uint32_t(kKeyBytes / 2));
+          __syncwarp();
+          ++issued_keys;
+          keys.next(key_slots(both));
+        }
+      }
+      if (ok) {  // the end of the values
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&raw_empty[raw.at], raw.parity));
+        if (ok) {
+          if (elect_one()) {
+            raw_rows[raw.at] = -1;
+            mbar_arrive(&raw_full[raw.at]);
           }
-          __syncwarp();
-          if (elect_one()) mbar_arrive_expect_tx(&full[c.at], second ? uint32_t(kSlotBytes) : uint32_t(kSlotBytes / 2));
-          __syncwarp();
-          ++issued;
-          c.next(slots);
+          ++issued_raw;
         }
       }
       if (!ok && lane == 0) report_operator_timeout(a.err);
       // the copies in flight land before the block can end
-      for (int l = issued > slots ? issued - slots : 0; l < issued; ++l)
-        mbar_wait_bounded(&full[l % slots], uint32_t((l / slots) & 1));
+      auto land = [&](uint64_t* full, int issued, int slots) {
+        for (int l = issued > slots ? issued - slots : 0; l < issued; ++l)
+          mbar_wait_bounded(&full[l % slots], uint32_t((l / slots) & 1));
+      };
+      land(key_full, issued_keys, key_slots(both));
+      land(raw_full, issued_raw, raw_slots(both));
     } else if (warp == 1) {
       // ================= products =================
       // One elected lane waits and issues: a wait by the whole warp, its vote and a new election around every product
       // took 1000 clocks a product.
-      constexpr uint32_t id_s = idesc_e4m3(128, kStep, false), id_o = idesc_e4m3(128, D, true);
-      Cursor start{0, 0};
+      constexpr uint32_t id_s = idesc_of(128, kStep, false), id_o = idesc_of(128, D, true);
+      Cursor keys{0, 0}, wide{0, 0};  // the elected lane's
       int buf = 0;
       uint32_t q_parity = 0, p_parity = 0, o_parity = 3;  // p_parity, o_parity: bit t
       bool ok = true;
       const uint64_t desc = umma_desc_sw128(smem_u32(sm), 16, 1024);  // of the start of shared memory
+      const uint64_t wide_desc = umma_desc_sw128(smem_u32(sm + wide_at), kPage * 128, 1024);
       for (;;) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(&q_full[buf], q_parity));
         if (!ok) break;
         const int n = work[buf].count;
         if (n == 0) break;
-        const int last_valid = work[buf].u.tokens - (work[buf].first + n - 1) * kStep;  // tokens of the last step
         const int tiles = both ? min(n, 2) : (work[buf].u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
         __syncwarp();
         auto wait = [&](uint64_t* bar, uint32_t parity) {
           if (ok) ok = mbar_wait_bounded(bar, parity);
         };
-        // scores of tile t with the keys in `slot`
-        auto scores = [&](int t, int slot, bool frees_keys, bool frees_queries) {
+        // scores of tile t with the keys at their ring's cursor
+        auto scores = [&](int t, bool frees_keys, bool frees_queries) {
+          wait(&key_full[keys.at], keys.parity);
           if (!ok) return;
           tc_fence_after();
           const uint64_t qd = desc + uint64_t((kOffQ + buf * q_buf + (both ? 0 : t) * kQTile) >> 4);
-          const uint64_t kd = desc + uint64_t((ring + slot * kSlotBytes) >> 4);
+          const uint64_t kd = desc + uint64_t((keys_at + keys.at * kKeyBytes) >> 4);
           const uint32_t d = tmem + kColS + uint32_t(128 * t);
 #pragma unroll
           for (int x = 0; x < 2; ++x)
@@ -593,91 +634,60 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               mma8_ss(d, qd + uint64_t((x * kTile * 128 + kk * 32) >> 4), kd + uint64_t((kk * 32) >> 4), id_s,
                       x > 0 || kk > 0 ? 1u : 0u);
           tc_commit(&s_full[t]);
-          if (frees_keys) tc_commit(&empty[slot]);
+          if (frees_keys) {
+            tc_commit(&key_empty[keys.at]);
+            keys.next(key_slots(both));
+          }
           if (frees_queries) tc_commit(&q_empty[buf]);
         };
-        // output of tile t += probabilities times the values in `slot`, a page as soon as its probabilities are there
-        auto output = [&](int t, int slot, bool first, bool frees_values) {
+        // output of tile t += probabilities times the values of the two pages at their ring's cursor, a page as soon as
+        // its probabilities are there
+        auto output = [&](int t, bool first, bool frees_values) {
           if (first) {
             wait(&o_free[t], (o_parity >> t) & 1u);
             o_parity ^= 1u << t;
           }
-          const uint64_t vd = desc + uint64_t((ring + slot * kSlotBytes) >> 4);
           const uint32_t d = tmem + kColO + uint32_t(128 * t), pt = tmem + kColS + uint32_t(128 * t);
+          Cursor c = wide;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            wait(&wide_full[c.at], c.parity);
             wait(&p_full[t][h], (p_parity >> t) & 1u);
             if (!ok) return;
             tc_fence_after();
+            const uint64_t vd = wide_desc + uint64_t((c.at * kWideBytes) >> 4);
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int kk = 0; kk < 2; ++kk)
-                mma8_ts(d, pt + uint32_t(h * 64 + kk * 32 + x * 8), vd + uint64_t((h * 8192 + kk * 4096) >> 4), id_o,
-                        !first || h > 0 || x > 0 || kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < kPage / 16; ++kk)
+              mma_ts(d, pt + uint32_t(h * 64 + (kk >> 1) * 32 + (kk & 1) * 8), vd + uint64_t((kk * 2048) >> 4), id_o,
+                     !first || h > 0 || kk > 0 ? 1u : 0u);
+            if (frees_values) tc_commit(&wide_empty[c.at]);
+            c.next(wide_slots(both));
           }
           p_parity ^= 1u << t;
           tc_commit(&pv_done[t]);
-          if (frees_values) tc_commit(&empty[slot]);
+          if (frees_values) wide = c;
         };
         if (elect_one()) {
-          Cursor c = start;
-          // all but the last step's output
           if (both) {
-            for (int j = 0; j < tiles; ++j, c.next(slots)) {
-              wait(&full[c.at], c.parity);
-              scores(j, c.at, true, j == n - 1);
-            }
-            for (int j = 0; j < n - 1 && ok; ++j) {
-              wait(&full[c.at], c.parity);
-              output(j & 1, c.at, j < 2, true);
-              c.next(slots);
-              if (j + 2 < n) {
-                wait(&full[c.at], c.parity);
-                scores(j & 1, c.at, true, j + 2 == n - 1);
-                c.next(slots);
-              }
+            for (int j = 0; j < tiles; ++j) scores(j, true, j == n - 1);
+            for (int j = 0; j < n && ok; ++j) {
+              output(j & 1, j < 2, true);
+              if (j + 2 < n) scores(j & 1, true, j + 2 == n - 1);
             }
           } else {
-            wait(&full[c.at], c.parity);
-            for (int t = 0; t < tiles; ++t) scores(t, c.at, t == tiles - 1, n == 1 && t == tiles - 1);
-            c.next(slots);
-            for (int j = 0; j < n - 1 && ok; ++j) {
-              const int values = c.at;
-              wait(&full[c.at], c.parity);
-              c.next(slots);
-              output(0, values, j == 0, tiles == 1);
-              wait(&full[c.at], c.parity);
-              scores(0, c.at, tiles == 1, tiles == 1 && j == n - 2);
+            for (int t = 0; t < tiles; ++t) scores(t, t == tiles - 1, n == 1 && t == tiles - 1);
+            for (int j = 0; j < n && ok; ++j) {
+              const bool more = j + 1 < n, last = j + 2 == n;
+              output(0, j == 0, tiles == 1);
+              if (more) scores(0, tiles == 1, tiles == 1 && last);
               if (tiles == 2) {
-                output(1, values, j == 0, true);
-                scores(1, c.at, true, j == n - 2);
+                output(1, j == 0, true);
+                if (more) scores(1, true, last);
               }
-              c.next(slots);
             }
-          }
-        }
-        __syncwarp();
-        start.skip(2 * n - 1, slots);
-        if (last_valid < kStep) {
-          // what lies behind the last token is no value: it may be a NaN's bits, and 0 * NaN is NaN
-          mbar_wait_bounded(&full[start.at], start.parity);
-          unsigned char* vs = sm + ring + start.at * kSlotBytes;
-          for (int i = lane; i < (kStep - last_valid) * 8; i += 32)
-            *reinterpret_cast<uint4*>(vs + last_valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async();
-          __syncwarp();
-        }
-        if (elect_one()) {
-          wait(&full[start.at], start.parity);
-          if (both) {
-            output((n - 1) & 1, start.at, n <= 2, true);
-          } else {
-            for (int t = 0; t < tiles; ++t) output(t, start.at, n == 1, t == tiles - 1);
           }
         }
         ok = __all_sync(0xffffffffu, ok);  // the elected lane's, the others' is true
-        start.skip(1, slots);
         if ((buf ^= 1) == 0) q_parity ^= 1u;
       }
       if (!ok && lane == 0) report_operator_timeout(a.err);
@@ -782,8 +792,65 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       }
       if (!ok && lane == 0) report_operator_timeout(a.err);
     }
+  } else if (warp >= 16) {
+    set_max_registers_down<kRegistersValues>();
+    // ================= values: from e4m3 to fp16, which is exact =================
+    // A warp 16 tokens of a page, a lane 16 dimensions of a token; what lies behind the last token is no value (it may
+    // be a NaN's bits, and 0 * NaN is NaN) and becomes zero.
+    constexpr int kRowLanes = D / 16, kRowsAtOnce = 32 / kRowLanes, kVecs = kPage / kWideners / kRowsAtOnce;
+    const int row0 = (warp - 16) * (kPage / kWideners) + lane / kRowLanes, c = lane % kRowLanes;
+    Cursor raw{0, 0}, wide{0, 1};
+    bool ok = true;
+    for (;;) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&wide_empty[wide.at], wide.parity) &&
+                                       mbar_wait_bounded(&raw_full[raw.at], raw.parity));
+      if (!ok) break;
+      const int rows = raw_rows[raw.at];
+      if (rows < 0) break;
+      const unsigned char* src = sm + raw_at + raw.at * kRawBytes + c * 16;
+      uint4 x[kVecs];
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int row = row0 + i * kRowsAtOnce;
+        x[i] = row < rows ? *reinterpret_cast<const uint4*>(src + row * D) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      unsigned char* dst = sm + wide_at + wide.at * kWideBytes + (c >> 2) * (kPage * 128);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int row = row0 + i * kRowsAtOnce;
+        const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[2 * e] = e4m3x2_to_f16x2(uint16_t(in[e]));
+          v[2 * e + 1] = e4m3x2_to_f16x2(uint16_t(in[e] >> 16));
+        }
+        // the row's 16-byte pieces are swizzled by the row; the lanes of the second 64 dimensions store their second
+        // piece first, so that eight lanes meet no bank twice
+        const bool swap = (c >> 2) != 0;
+        unsigned char* at = dst + row * 128;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int piece = (c & 3) * 2 + (k ^ int(swap));
+          const bool high = (k != 0) != swap;
+          *reinterpret_cast<uint4*>(at + ((piece ^ (row & 7)) << 4)) =
+              make_uint4(high ? v[4] : v[0], high ? v[5] : v[1], high ? v[6] : v[2], high ? v[7] : v[3]);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      // (the page's place is handed back when what was read of it has been used: an arrival does not wait for loads
+      // before it, which took 1500 clocks behind another warp's stores)
+      if (lane == 0) {
+        mbar_arrive(&wide_full[wide.at]);
+        mbar_arrive(&raw_empty[raw.at]);
+      }
+      raw.next(raw_slots(both));
+      wide.next(wide_slots(both));
+    }
+    if (!ok && lane == 0) report_operator_timeout(a.err);
   } else {
-    set_max_registers_up<160>();
+    set_max_registers_up<kRegistersSoftmax>();
     // ================= softmax of tile t: a thread a row =================
     const int t = (warp - 4) >> 2, w = warp & 3, row = w * 32 + lane;
     const uint32_t lanes = uint32_t(w * 32) << 16;
@@ -882,18 +949,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             follow(top, top + v_log2, j == begin);
             const float dv = value_shift(v_log2);
             float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-            uint32_t hi[8], lo[8];
-            probabilities(s, c, dv + kLog2P - (m == -INFINITY ? 0.f : m), hi, lo, sum0, sum1);
+            uint32_t pk[16];
+            probabilities(s, c, dv + kLog2P - (m == -INFINITY ? 0.f : m), pk, sum0, sum1);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {  // nothing for the tokens of the other quarters
-              uint32_t x[8], y[8];
+              uint32_t x[16];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                x[e] = g == w ? hi[e] : 0u;
-                y[e] = g == w ? lo[e] : 0u;
-              }
-              tmem_st8(s_tmem + uint32_t(32 * g), x);
-              tmem_st8(s_tmem + uint32_t(32 * g + 8), y);
+              for (int e = 0; e < 16; ++e) x[e] = g == w ? pk[e] : 0u;
+              tmem_st16(s_tmem + uint32_t(32 * g), x);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -934,10 +997,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             load(h, s);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-              uint32_t hi[8], lo[8];
-              probabilities(s[g], h ? c1 : c0, shift, hi, lo, sum0, sum1);
-              tmem_st8(s_tmem + uint32_t(64 * h + 32 * g), hi);
-              tmem_st8(s_tmem + uint32_t(64 * h + 32 * g + 8), lo);
+              uint32_t pk[16];
+              probabilities(s[g], h ? c1 : c0, shift, pk, sum0, sum1);
+              tmem_st16(s_tmem + uint32_t(64 * h + 32 * g), pk);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -955,7 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const int64_t part_row = (int64_t(blockIdx.x) * 2 + p.part) * 2 * kTile;  // the first of a part of the unit
       if (both) {
         // the copies of a row (2 tiles, or 8 warps) are added through shared memory, 16 columns at a time
-        float4* xch = reinterpret_cast<float4*>(sm + kOffOut);
+        float4* xch = reinterpret_cast<float4*>(sm + out_at);
         const int me = t * kTile + row, rows = quarters ? 32 : kTile, r_me = me & (rows - 1);
         copy_ml[me] = make_float2(m, l);
         all_copies();
@@ -1018,25 +1080,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           }
         }
       } else if (t < tiles) {
-        // through shared memory, 32 columns at a time: 4 lanes then write 64 bytes of a row
+        // through shared memory, 16 columns at a time: 2 lanes then write 32 bytes of a row
         const float f = to_true / l;
-        unsigned char* stage = sm + kOffOut + (warp - 4) * 2048;
-        int64_t at[4];
+        unsigned char* stage = sm + out_at + (warp - 4) * 1024;
+        int64_t at[2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int rr = r0 + w * 32 + x * 8 + (lane >> 2);
-          at[x] = rr < a.rows ? row_offset(a, a.os, rr) + (lane & 3) * 8 : -1;
+        for (int x = 0; x < 2; ++x) {
+          const int rr = r0 + w * 32 + x * 16 + (lane >> 1);
+          at[x] = rr < a.rows ? row_offset(a, a.os, rr) + (lane & 1) * 8 : -1;
         }
 #pragma unroll 1
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t o[16];
           __syncwarp();
-          tmem_ld32(o_tmem + 32u * uint32_t(i), o);
+          tmem_ld16(o_tmem + 16u * uint32_t(i), o);
           tmem_wait_ld();
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
+          for (int v = 0; v < 2; ++v) {
             const uint32_t* x = &o[8 * v];
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) =
+            *reinterpret_cast<uint4*>(stage + lane * 32 + ((v ^ ((lane >> 2) & 1)) << 4)) =
                 make_uint4(pack_bf16x2(__uint_as_float(x[0]) * f, __uint_as_float(x[1]) * f),
                            pack_bf16x2(__uint_as_float(x[2]) * f, __uint_as_float(x[3]) * f),
                            pack_bf16x2(__uint_as_float(x[4]) * f, __uint_as_float(x[5]) * f),
@@ -1044,10 +1106,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           }
           __syncwarp();
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int rr = x * 8 + (lane >> 2);
-            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
-            if (at[x] >= 0) *reinterpret_cast<uint4*>(out + at[x] + 32 * i) = y;
+          for (int x = 0; x < 2; ++x) {
+            const int rr = x * 16 + (lane >> 1);
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 32 + (((lane & 1) ^ ((rr >> 2) & 1)) << 4));
+            if (at[x] >= 0) *reinterpret_cast<uint4*>(out + at[x] + 16 * i) = y;
           }
         }
       }
@@ -1151,17 +1213,19 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-// e4m3 [pages * heads][64][dim]; a box is a page of one head, its rows 128 bytes
-// apart in shared memory (dim 64: the rest of a row is filled with zeros).
-bool make_page_map(CUtensorMap* m, const void* base, int64_t pages, int heads, int dim) {
+// e4m3 [pages * heads][64][dim]; a box is a page of one head.  Keys: its rows 128
+// bytes apart in shared memory (dim 64: the rest of a row is filled with zeros) and
+// swizzled for the products; values: as they lie in the cache.
+bool make_page_map(CUtensorMap* m, const void* base, int64_t pages, int heads, int dim, bool keys) {
   const auto fn = tensor_map_encoder();
   if (!fn) return false;
   const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(kPage), cuuint64_t(pages * heads)};
   const cuuint64_t strides[2] = {cuuint64_t(dim), cuuint64_t(dim) * kPage};
-  const cuuint32_t box[3] = {128u, cuuint32_t(kPage), 1u};
+  const cuuint32_t box[3] = {keys ? 128u : cuuint32_t(dim), cuuint32_t(kPage), 1u};
   const cuuint32_t step[3] = {1u, 1u, 1u};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, step,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, keys ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1196,11 +1260,19 @@ int device_sms(int* sms) {
 
 size_t part_bytes(int sms, int dim) { return size_t(sms) * 2 * 2 * kTile * (size_t(dim) * 4 + sizeof(float2)); }
 
+// The warpgroups share out the registers that the block is launched with: with fewer they would wait for good.
+int registers_of(void (*kernel)(Maps, Args)) {
+  cudaFuncAttributes at{};
+  return cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(kernel)) == cudaSuccess ? at.numRegs : 0;
+}
+
 template <int D>
 cudaError_t launch_attention(cudaStream_t st, const Maps& maps, const Args& a, int sms) {
   const auto kernel = a.rows <= kTile ? attention_kernel<D, true> : attention_kernel<D, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
+  static const int registers[2] = {registers_of(attention_kernel<D, false>), registers_of(attention_kernel<D, true>)};
+  if (registers[a.rows <= kTile] != kRegisters) return cudaErrorInvalidKernelImage;
   kernel<<<unsigned(sms), kThreads, kSmem, st>>>(maps, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int rows = a.rows < 2 * kTile ? a.rows : 2 * kTile;
@@ -1297,8 +1369,8 @@ int pasa_kv8_attention(void* stream, const void* q, const int64_t* q_stride, con
   if (!a.err) return PASA_ERR_CUDA;
   // (without pages no request has tokens: the maps are not used)
   const void* some = pages ? k_cache : workspace;
-  if (!make_page_map(&maps.k, some, pages ? pages : 1, int(heads), dim) ||
-      !make_page_map(&maps.v, pages ? v_cache : workspace, pages ? pages : 1, int(heads), dim))
+  if (!make_page_map(&maps.k, some, pages ? pages : 1, int(heads), dim, true) ||
+      !make_page_map(&maps.v, pages ? v_cache : workspace, pages ? pages : 1, int(heads), dim, false))
     return PASA_ERR_CUDA;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
