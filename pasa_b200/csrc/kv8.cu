@@ -883,6 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const bool live = r < a.rows, warp_live = quarters || r0 + w * 32 < a.rows;
       const int tiles = both ? min(n, 2) : (p.u.block * 2 + 1) * kTile < a.rows ? 2 : 1;
       const float q_row = q_scale[buf * 2 * kTile + (both ? 0 : t * kTile) + row] * a.scale_log2;
+      __threadfence_block();  // an arrival does not wait for loads before it
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[buf]);
       if ((buf ^= 1) == 0) q_parity ^= 1u;
