@@ -413,14 +413,16 @@ __device__ __forceinline__ int64_t row_offset(const Args& a, const int64_t (&s)[
   return (row - query * a.group) * s[1] + query * s[2];
 }
 
-// The exponent of a values' scale; NaN for NaN, and for what is no power of two (an error).
-__device__ __forceinline__ float scale_log2(const Args& a, float scale) {
+// A page's scale as it is; NaN for NaN, and for what is no power of two (an error).
+__device__ __forceinline__ float checked_scale(const Args& a, float scale) {
   const uint32_t v = __float_as_uint(scale);
-  if (v >= 0x7F800000u || (v & 0x7FFFFFu) || v == 0) {
-    if (v != 0x7FC00000u) atomicOr(a.err, PASA_DEVERR_BAD_SCALE);
-    return __uint_as_float(0x7FC00000u);
-  }
-  return float(int(v >> 23) - 127);
+  if (v < 0x7F800000u && !(v & 0x7FFFFFu) && v != 0) return scale;
+  if (v != 0x7FC00000u) atomicOr(a.err, PASA_DEVERR_BAD_SCALE);
+  return __uint_as_float(0x7FC00000u);
+}
+// The exponent of a checked scale.
+__device__ __forceinline__ float scale_log2(float scale) {
+  return scale == scale ? float(int(__float_as_uint(scale) >> 23) - 127) : scale;
 }
 
 // 2^(x mul + shift) of 32 scores in fp16, and their fp32 sums.
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             if (second) tma_load_3d(dst + kKeyBytes / 2, &maps.k, &key_full[keys.at], 0, 0, z[1]);
           }
           // the scales are on their way while the tiles are: what the barrier expects comes behind them
-          if ((j & 15) == 0) scales.y = scale_log2(a, scales.y);
+          if ((j & 15) == 0) scales = make_float2(checked_scale(a, scales.x), scale_log2(checked_scale(a, scales.y)));
           if ((lane >> 1) == (j & 15)) step_scale[step % kScaleSteps][lane & 1] = scales;
           ++step;
           __syncwarp();

@@ -1,0 +1,33 @@
+"""What the 8-bit cache's kernels report: pages that do not exist, scales that cannot be, and who gets to know."""
+import pytest
+import torch
+
+from pasa_b200 import ops
+from test_gpu_kv8 import Pages, i32, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("queries", [1, 40, 200])
+@pytest.mark.parametrize("bad", [0.3, 0.0, -1.0, -0.0, float("inf"), 2.0 ** -130])
+def test_scales_of_keys_that_are_no_power_of_two(cuda_device, bad, queries):
+    p = Pages([200, 100], 2, 64).fill()
+    q, n = randn(2, 4, queries, 64), i32([200, 100])
+    clean = ops.kv8_attention(q, p.cache, p.table, n)
+    scales = p.cache.k_scale.clone()
+    scales[p.rows[0][1], 1] = bad
+    out = ops.kv8_attention(q, p.cache._replace(k_scale=scales), p.table, n)
+    with pytest.raises(RuntimeError, match="power of two"):
+        ops.check_operator_errors()
+    assert out[0, 2:].isnan().all()
+    assert torch.equal(out[0, :2], clean[0, :2]) and torch.equal(out[1], clean[1])
+    out = ops.kv8_attention(q, p.cache._replace(k_scale=scales), p.table, i32([64, 100]))  # before that page
+    assert out.isfinite().all()
+    ops.check_operator_errors()
+
+
+def test_a_scale_of_nan_is_a_page_with_nan(cuda_device):
+    p = Pages([200], 1, 128).fill()
+    p.cache.k_scale[p.rows[0][2]] = float("nan")
+    assert ops.kv8_attention(randn(1, 2, 3, 128), p.cache, p.table, i32([200])).isnan().all()
+    ops.check_operator_errors()
