@@ -507,8 +507,8 @@ PASA_API int pasa_lora_update_backward(void* stream, const void* dy, int64_t ldd
  *                     i % 64 of page table[b][i / 64]
  * A table entry outside [0, pages) that is needed is an error
  * (PASA_DEVERR_BAD_PAGE in pasa_operator_errors): nothing is written to such a
- * page, and the attention of such a request is undefined, but reads no memory
- * outside of the cache.
+ * page, and the attention reads it as NaN.  So it reads a page with a scale that
+ * is no power of two (PASA_DEVERR_BAD_SCALE).
  *
  * pasa_kv8_write rounds new tokens (k, v: bf16 [batch, heads, tokens, dim], the
  * host arrays' strides of batch, head and token in elements, multiples of 8)

@@ -531,7 +531,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
               k_pages = bad ? 0 : coming;
               // (a page behind the last token is masked: scores are -infinity whatever the scale, the values' is below any)
               scales = make_float2(1.f, __uint_as_float(0x00800000u));
-              if (mine) {
+              if (bad && mine) {  // (what is read in its place is another request's)
+                scales.x = scales.y = __uint_as_float(0x7FC00000u);
+              } else if (mine) {
                 const int64_t z = int64_t(k_pages) * a.heads + p.u.head;
                 scales = make_float2(a.k_scale[z], a.v_scale[z]);
               }

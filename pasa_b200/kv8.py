@@ -127,6 +127,8 @@ def kv8_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], table: torch.T
     ``scale`` is positive, D**-0.5 by default.  Returns a new tensor with q's strides, or ``out`` (its last stride 1,
     the others multiples of 8).  Queries enter the products to 8 significant bits (or 2^-17 of the row's largest
     element), probabilities to 11 (or 2^-36 of the largest), sums are fp32.  Has no gradient.
+    A needed table entry that is no page, or a scale that is no power of two, makes the rows that need it NaN and is
+    reported by ``check_operator_errors``.
     """
     args, store = _check_cache(cache, table)
     device = store.device

@@ -31,3 +31,20 @@ def test_a_scale_of_nan_is_a_page_with_nan(cuda_device):
     p.cache.k_scale[p.rows[0][2]] = float("nan")
     assert ops.kv8_attention(randn(1, 2, 3, 128), p.cache, p.table, i32([200])).isnan().all()
     ops.check_operator_errors()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("queries", [1, 40, 200])
+@pytest.mark.parametrize("at", [0, 3, 40])
+def test_a_page_that_does_not_exist_reads_as_nan(cuda_device, dim, queries, at):
+    """And not as what another request has in some page."""
+    p = Pages([2700, 500], 2, dim).fill()
+    q, n = randn(2, 2, queries, dim), i32([2700, 500])
+    clean = ops.kv8_attention(q, p.cache, p.table, n)
+    for bad in (-1, p.pages, 1 << 30, -(1 << 31)):
+        table = p.table.clone()
+        table[0, at] = bad
+        out = ops.kv8_attention(q, p.cache, table, n)
+        with pytest.raises(RuntimeError, match="page that does not exist"):
+            ops.check_operator_errors()
+        assert out[0].isnan().all() and torch.equal(out[1], clean[1])
