@@ -449,8 +449,10 @@ PASA_API int pasa_rope_axes(void* stream, const pasa_rope_tensor* tensors, int n
 
 /*
  * Errors of the operators below on the current device: the bits that their
- * kernels' bounded waits have set since the last call (PASA_DEVERR_*), written
- * to the host word `flags` and cleared.  Synchronises the stream.
+ * kernels have set since the last call (PASA_DEVERR_*), from whatever stream,
+ * written to the host word `flags` and cleared, both at once.  There is one word
+ * a device: a caller also gets what the kernels of others have set.
+ * Synchronises the stream.
  */
 PASA_API int pasa_operator_errors(void* stream, uint32_t* flags);
 

@@ -1,12 +1,20 @@
 // Host helpers of the operators with kernels of their own: the driver's tensor
 // map encoder and the error word that their bounded waits report to.
 #include <atomic>
+#include <mutex>
 
 #include "umma.cuh"
 
 namespace pasa {
 
-__device__ uint32_t g_operator_errors;  // one a device; kernels only set bits
+// Of each device: the word in which kernels set bits, and what was last taken out of it.
+__device__ uint32_t g_operator_errors[2];
+
+namespace {
+// Read and cleared at once: a bit that a kernel on another stream sets is in this report or in the next.
+__global__ void take_errors(uint32_t* words) { words[1] = atomicExch(&words[0], 0u); }
+std::mutex g_taking;  // from taking the bits to their arrival: there is one place for them
+}  // namespace
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
@@ -39,10 +47,14 @@ uint32_t* operator_error_word() {
 
 extern "C" int pasa_operator_errors(void* stream, uint32_t* flags) {
   if (!flags) return PASA_ERR_NULL;
-  uint32_t* word = pasa::operator_error_word();
+  uint32_t* words = pasa::operator_error_word();
+  if (!words) return PASA_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!word || cudaMemcpyAsync(flags, word, sizeof(uint32_t), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
-      cudaMemsetAsync(word, 0, sizeof(uint32_t), st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess)
+  const std::lock_guard<std::mutex> hold(pasa::g_taking);
+  pasa::take_errors<<<1, 1, 0, st>>>(words);
+  if (cudaGetLastError() != cudaSuccess ||
+      cudaMemcpyAsync(flags, words + 1, sizeof(uint32_t), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      cudaStreamSynchronize(st) != cudaSuccess)
     return PASA_ERR_CUDA;
   return PASA_OK;
 }

@@ -48,3 +48,31 @@ def test_a_page_that_does_not_exist_reads_as_nan(cuda_device, dim, queries, at):
         with pytest.raises(RuntimeError, match="page that does not exist"):
             ops.check_operator_errors()
         assert out[0].isnan().all() and torch.equal(out[1], clean[1])
+
+
+def test_reports_of_another_stream_are_not_lost(cuda_device):
+    """A kernel on one stream reports while another stream asks, over and over: somebody gets to know of each."""
+    p = Pages([300], 1, 64).fill()
+    table = p.table.clone()
+    table[0, 4] = -1
+    q, n = randn(1, 1, 3, 64), i32([300])
+    torch.cuda.synchronize()
+    ops.check_operator_errors()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(100):
+        told = 0
+        with torch.cuda.stream(one):
+            ops.kv8_attention(q, p.cache, table, n)
+            done = torch.cuda.Event()
+            done.record()
+        last = False
+        with torch.cuda.stream(two):
+            while not last:
+                last = done.query()
+                try:
+                    ops.check_operator_errors()
+                except RuntimeError:
+                    told += 1
+        assert told == 1
+    with torch.cuda.stream(two):
+        ops.check_operator_errors()
