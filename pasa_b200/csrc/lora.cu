@@ -754,8 +754,9 @@ __global__ void __launch_bounds__(kFewCols) up_few_kernel(const __grid_constant_
 // different numbers of rows keep all SMs busy.  A block owns 512 columns (256
 // above rank 64) of x or of dy and one share; where its share passes from one
 // adapter to the next it puts down what it has summed.  An adapter that lies in
-// one share is written at once; the others' sums go to the workspace and a
-// second kernel adds them in the order of the shares.
+// one share is written at once; the others' sums, two a share at most (of the
+// adapter that it begins in and of the one that it ends in), go to the workspace
+// and a second kernel adds them in the order of the shares.
 //
 // A stage's rows behind the request's last are zeroed in shared memory: they
 // hold another request's values, which may be NaN.  hi and lo sit side by side
@@ -777,7 +778,7 @@ struct GradArgs {
   int problem0;                // the first problem computed (0: dA, 1: dB)
   int64_t cols[2], blocks[2];  // columns and column blocks
   int shares;
-  float* partial;         // [shares + adapters][rank * cols] for each problem
+  float* partial;         // [shares][2][rank * cols] for each problem
   __nv_bfloat16* out[2];  // [adapters][rank][cols], [adapters][cols][rank]
   uint32_t* err;
 };
@@ -810,6 +811,12 @@ struct Piece {
   int base;    // stages of the adapters before
   bool whole;  // all of the adapter's
 };
+
+// The place of the sums that share `share`, which begins at stage g0, has of an adapter with `base` stages before it and
+// more in other shares: such an adapter is the one that the share begins in, or else the one that it ends in.
+__device__ __forceinline__ int64_t partial_index(int share, int base, int g0) {
+  return int64_t(share) * 2 + (base > g0 ? 1 : 0);
+}
 
 // The piece of the share [g0, g1) behind `after` (slot -1, base 0: the first); count 0: there is none.  All lanes.
 __device__ __forceinline__ Piece next_piece(const int* stages, int adapters, int g0, int g1, const Piece& after,
@@ -985,10 +992,8 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
       }
       acc_parity ^= 1u;
       tc_fence_after();
-      // a piece's place is its share and its adapter together: either grows from one piece to the next
-      float* partial = a.partial +
-                       (problem == 1 && a.problem0 == 0 ? int64_t(a.shares + a.rows.adapters) * a.rank * a.cols[0] : 0) +
-                       int64_t(share + p.slot) * size;
+      float* partial = a.partial + (problem == 1 && a.problem0 == 0 ? int64_t(a.shares) * 2 * a.rank * a.cols[0] : 0) +
+                       partial_index(share, p.base, g0) * size;
       __nv_bfloat16* out = a.out[problem] + int64_t(p.slot) * size;
       for (int x = 0; x < width / 128; ++x) {
         const int64_t col = col0 + x * 128 + q * 32 + lane;
@@ -1080,15 +1085,16 @@ __global__ void __launch_bounds__(256) grad_sum_kernel(const __grid_constant__ S
   int problem = 0;
   if (i >= a.size[0]) {
     i -= a.size[0];
-    partial += int64_t(a.shares + a.rows.adapters) * a.size[0];
+    partial += int64_t(a.shares) * 2 * a.size[0];
     problem = 1;
     if (i >= a.size[1]) return;
   }
   float v[8] = {};
   for (int share = first; share <= last; ++share) {
     // (a share without stages of its own, when there are fewer stages than shares, wrote nothing)
-    if (share_begin(total, share, a.shares) == share_begin(total, share + 1, a.shares)) continue;
-    const float4* src = reinterpret_cast<const float4*>(partial + int64_t(share + adapter) * a.size[problem] + i);
+    const int g0 = share_begin(total, share, a.shares);
+    if (g0 == share_begin(total, share + 1, a.shares)) continue;
+    const float4* src = reinterpret_cast<const float4*>(partial + partial_index(share, before, g0) * a.size[problem] + i);
     const float4 x = src[0], y = src[1];
     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
     v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
@@ -1306,7 +1312,7 @@ int grad_shares(int64_t m, int64_t blocks, int rank, int64_t adapters, int64_t r
 
 size_t grad_partial_bytes(int64_t m, int64_t k, int64_t n, int rank, int64_t adapters, int64_t requests, int sms) {
   const int64_t shares = grad_shares(m, grad_blocks(k, rank) + grad_blocks(n, rank), rank, adapters, requests, sms);
-  return shares > 1 ? size_t(shares + adapters) * size_t(rank) * size_t(k + n) * 4 : 0;
+  return shares > 1 ? size_t(shares) * 2 * size_t(rank) * size_t(k + n) * 4 : 0;
 }
 
 cudaError_t grad(cudaStream_t st, const Rows& r, int rank, Matrix x, int64_t k, Matrix dy, int64_t n,

@@ -1,0 +1,60 @@
+"""The adapters' operators where there are many adapters, infinities, memory that overlaps or row offsets that go back."""
+import ctypes
+
+import pytest
+import torch
+
+from pasa_b200 import _lib, ops
+from test_gpu_lora import Problem
+
+pytestmark = pytest.mark.gpu
+
+
+def workspace(m, k, n, rank, adapters, requests):
+    size = ctypes.c_size_t()
+    assert _lib.load().pasa_lora_backward_workspace_size(m, k, n, rank, adapters, requests, ctypes.byref(size)) == _lib.OK
+    return size.value
+
+
+@pytest.mark.parametrize("m,k,n,rank,requests", [(4096, 5120, 5120, 16, 64), (32760, 5120, 5120, 128, 64),
+                                                 (8000, 64, 72, 128, 4096)])
+def test_workspace_does_not_grow_with_the_adapters(cuda_device, m, k, n, rank, requests):
+    """Two sums a share at most, over all its blocks: 3 waves of blocks of 256 columns and more, 128 ranks."""
+    most = 2 * m * 128 * 2 + 256 + 2 * 3 * 160 * 512 * 128 * 4
+    assert workspace(m, k, n, rank, 4096, requests) <= most
+
+
+@pytest.mark.parametrize("lengths,adapters,slots", [
+    ([64] * 90, 90, None), ([40, 7, 300, 1, 33] * 30, 60, [(7 * i) % 61 - 1 for i in range(150)]),
+    ([5000, 3, 3, 3, 6000], 4000, [3999, 1, 2, 1, 0]), ([31, 33] * 200, 400, None)])
+def test_gradients_of_many_adapters(cuda_device, lengths, adapters, slots):
+    """Shares that begin and end in the middle of an adapter, on its first row, and hold many whole ones."""
+    for k, n, rank in ((72, 328, 24), (264, 64, 120)):
+        p = Problem(lengths, k, n, rank, adapters, slots)
+        grads = ops.lora_update_backward(p.dy, *p.args)
+        p.check_grads(*grads)
+        assert all(torch.equal(u, v) for u, v in zip(grads, ops.lora_update_backward(p.dy, *p.args)))
+    ops.check_operator_errors()
+
+
+def test_gradients_of_a_alone_without_h(cuda_device):
+    """The C entry needs h for the gradients of B only."""
+    p = Problem([200, 30], 72, 64, 16, 2)
+    dx, da, _ = ops.lora_update_backward(p.dy, *p.args)
+    size = workspace(p.m, p.k, p.n, p.rank, 2, 2)
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    got, db = torch.empty_like(p.a), torch.empty_like(p.b)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+
+    def call(h, dx, da, db):
+        return _lib.load().pasa_lora_update_backward(
+            torch.cuda.current_stream().cuda_stream, ptr(p.dy), p.n, ptr(p.x), p.k, ptr(p.a), ptr(p.b), ptr(p.scale), p.m,
+            p.k, p.n, p.rank, 2, ptr(p.rows), ptr(p.slots), 2, ptr(h), 0, None, 0, ptr(dx), p.k, ptr(da), ptr(db),
+            space.data_ptr(), size)
+
+    assert call(None, None, got, None) == _lib.OK
+    assert torch.equal(got, da)
+    other = torch.empty_like(p.x)
+    assert call(None, other, None, None) == _lib.OK
+    assert torch.equal(other, dx)
+    assert call(None, None, None, db) == _lib.ERR_NULL
