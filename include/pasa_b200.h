@@ -467,8 +467,9 @@ PASA_API int pasa_operator_errors(void* stream, uint32_t* flags);
  *   y    [m, n] bf16, row stride ldy      b  [adapters, n, rank] bf16
  *   out  [m, n] bf16, row stride ldo; may be y (in place), no other overlap
  *   rows, slots  device int32 [requests + 1], [requests]; rows must not
- *        decrease (then some rows of out are not written; nothing outside of
- *        the tensors is read or written in any case)
+ *        decrease (then some rows of out are not written, and gradients are
+ *        some sums or zero; the kernels end, and nothing outside of the
+ *        tensors is read or written, in any case)
  *   scale device fp32 [adapters], or NULL for 1
  *   h    scratch of pasa_lora_h_size bytes; what pasa_lora_update_backward
  *        takes as h

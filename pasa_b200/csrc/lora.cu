@@ -309,6 +309,7 @@ struct UpArgs {
   int rp;
   int64_t chunks;  // of C
   int split;       // units of a span
+  int64_t units;   // at most (spans without end, where the rows decrease, end there)
   int64_t cols, ldo;
   const __nv_bfloat16* h;  // [2][m][rp]
   __nv_bfloat16* out;
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
     Cursor c{0, 1};
     int64_t issued = 0;
     bool ok = true;
-    for (int64_t id = blockIdx.x; ok; id += gridDim.x) {
+    for (int64_t id = blockIdx.x; ok && id < a.units; id += gridDim.x) {
       const Unit u = find_unit(a, id, lane);
       if (u.span.count == 0) break;
       if (weights ? !u.adapts : !a.has_base) continue;
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
     Cursor w{0, 0}, c{0, 1};
     uint32_t h_parity = 0;
     bool ok = true;
-    for (int64_t id = blockIdx.x; ok; id += gridDim.x) {
+    for (int64_t id = blockIdx.x; ok && id < a.units; id += gridDim.x) {
       const Unit u = find_unit(a, id, lane);
       if (u.span.count == 0) break;
       if (!u.adapts) continue;
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
     bool ok = true;
     Cursor y{0, 0};
     int before = -1;  // the slot whose stores may still read it
-    for (int64_t id = blockIdx.x; ok; id += gridDim.x) {
+    for (int64_t id = blockIdx.x; ok && id < a.units; id += gridDim.x) {
       const Unit u = find_unit(a, id, lane);
       if (u.span.count == 0) break;
       if (elect_one()) {
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
     bool ok = true;
     Cursor y{0, a.has_base ? 0u : 1u}, c{0, 0};  // of the base's arrivals, or of the slots that are free
     uint64_t* ready = a.has_base ? y_full : y_empty;
-    for (int64_t id = blockIdx.x;; id += gridDim.x) {
+    for (int64_t id = blockIdx.x; id < a.units; id += gridDim.x) {
       const Unit u = find_unit(a, id, lane);
       if (u.span.count == 0) break;
       const int live = min(max(u.span.count - q * kBox, 0), kBox);  // this warp's rows of the span
@@ -800,6 +801,11 @@ __device__ __forceinline__ int request_stages(const Rows& a, int q, int stage_ro
   return int((end - begin + stage_rows - 1) / stage_rows);
 }
 
+// All stages, from their sum over the requests; none where the rows decrease and there are more than there can be.
+__device__ __forceinline__ int total_stages(const Rows& a, int stage_rows, unsigned long long sum) {
+  return sum <= (unsigned long long)((a.m + stage_rows - 1) / stage_rows + a.requests) ? int(sum) : 0;
+}
+
 // First stage of a share, of `total`.
 __device__ __forceinline__ int share_begin(int total, int share, int shares) {
   return int(int64_t(total) * share / shares);
@@ -857,7 +863,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full, acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ int valid[kMaxStages];  // rows of a stage that are the request's
-  __shared__ int total;
+  __shared__ unsigned long long sum;  // of the requests' stages
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int width = grad_cols(a.atoms), stage_rows = grad_rows(a.atoms), box = stage_rows * 128;
   int64_t id = blockIdx.x;
@@ -873,7 +879,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
     mbar_init(&acc_full, 1);
     mbar_init(&acc_empty, 4);
     fence_barrier_init();
-    total = 0;
+    sum = 0;
   }
   for (int s = int(threadIdx.x); s < a.rows.adapters; s += kThreads) stages[s] = 0;
   if (warp == 1) { tmem_alloc(&tmem_slot, cols); tmem_relinquish(); }
@@ -884,10 +890,11 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ 
     int slot;
     int64_t begin, end;
     const int own = request_stages(a.rows, q, stage_rows, slot, begin, end);
-    if (own > 0) { atomicAdd(&stages[slot], own); atomicAdd(&total, own); }
+    if (own > 0) { atomicAdd(&stages[slot], own); atomicAdd(&sum, (unsigned long long)own); }
   }
   __syncthreads();
   const uint32_t tmem = tmem_slot;
+  const int total = total_stages(a.rows, stage_rows, sum);
   const int g0 = share_begin(total, share, a.shares), g1 = share_begin(total, share + 1, a.shares);
   const Piece none{-1, 0, 0, 0, false};
 
@@ -1056,25 +1063,28 @@ struct SumArgs {
 };
 
 __global__ void __launch_bounds__(256) grad_sum_kernel(const __grid_constant__ SumArgs a) {
-  __shared__ int before, mine, total;
+  __shared__ int before, mine;
+  __shared__ unsigned long long all;
   const int adapter = int(blockIdx.y);
-  if (threadIdx.x == 0) before = mine = total = 0;
+  if (threadIdx.x == 0) { before = mine = 0; all = 0; }
   __syncthreads();
-  int sum[3] = {0, 0, 0};
+  int sum[2] = {0, 0};
+  unsigned long long own_all = 0;
   for (int q = int(threadIdx.x); q < a.rows.requests; q += 256) {
     int slot;
     int64_t begin, end;
     const int own = request_stages(a.rows, q, a.stage_rows, slot, begin, end);
     if (own > 0) {
-      sum[2] += own;
+      own_all += own;
       if (slot < adapter) sum[0] += own;
       if (slot == adapter) sum[1] += own;
     }
   }
-  if (sum[2] > 0) { atomicAdd(&before, sum[0]); atomicAdd(&mine, sum[1]); atomicAdd(&total, sum[2]); }
+  if (own_all > 0) { atomicAdd(&before, sum[0]); atomicAdd(&mine, sum[1]); atomicAdd(&all, own_all); }
   __syncthreads();
+  const int total = total_stages(a.rows, a.stage_rows, all);
   int first = 0, last = -1;  // the shares of the adapter's first and last stage
-  if (mine > 0) {
+  if (total > 0 && mine > 0) {
     while (share_begin(total, first + 1, a.shares) <= before) ++first;
     last = first;
     while (share_begin(total, last + 1, a.shares) < before + mine) ++last;
@@ -1218,12 +1228,12 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
         (double(cdiv(busy_spans(r) * split, 2 * sms)) + 0.5) * (double(cdiv(a.chunks, split)) + 2.0);
     if (split == 1 || time < best * 0.98) { best = time; a.split = int(split); }
   }
-  const int64_t units = span_count(r) * a.split;
+  a.units = span_count(r) * a.split;
   const int smem = a.room + 1024;
   cudaError_t e = allow_smem<up_kernel<MN>>(smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(units < 2 * sms ? units : 2 * sms));
+  cfg.gridDim = dim3(unsigned(a.units < 2 * sms ? a.units : 2 * sms));
   cfg.blockDim = dim3(kUpThreads);
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = st;

@@ -58,3 +58,19 @@ def test_gradients_of_a_alone_without_h(cuda_device):
     assert call(None, other, None, None) == _lib.OK
     assert torch.equal(other, dx)
     assert call(None, None, None, db) == _lib.ERR_NULL
+
+
+def test_row_offsets_that_go_back_end(cuda_device):
+    """Offsets must not decrease.  Where they do, the calls end all the same, here with 2^31 stages to sum by the
+    requests' sizes, and what lies behind the tensors stays as it is."""
+    m, half = 1 << 20, 1 << 16
+    rows = torch.tensor([0, m] * half + [0], dtype=torch.int32, device="cuda")
+    slots = torch.arange(2 * half, dtype=torch.int32, device="cuda") // 2 % 2
+    x, dy = (torch.zeros(m, 8, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    a, b = torch.zeros(2, 8, 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 8, 8, dtype=torch.bfloat16, device="cuda")
+    h = torch.zeros(2, m, 16, dtype=torch.bfloat16, device="cuda")
+    dx, da, db = ops.lora_update_backward(dy, x, a, b, rows, slots, h=h)
+    torch.cuda.synchronize()
+    assert dx.shape == x.shape and da.shape == a.shape and db.shape == b.shape
+    p = Problem([100, 200], 64, 64, 8, 2)
+    p.check_grads(*ops.lora_update_backward(p.dy, *p.args))
