@@ -129,7 +129,7 @@ struct DownMaps {
 struct DownArgs {
   Rows rows;
   int room;        // bytes of shared memory for the ring
-  int rp;          // R rounded up to 16
+  int rank, rp;    // R, and rounded up to 16: h is zero behind R, whatever x holds (infinity times the zeros of w is NaN)
   int64_t steps;   // 64-wide steps of C
   int split;       // CTAs of a cluster, each a share of the steps
   __nv_bfloat16* h;  // [2][m][rp]
@@ -239,8 +239,10 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
       } else if (live) {
         uint32_t h[8], l[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i) {
           split2(scale * __uint_as_float(v[2 * i]), scale * __uint_as_float(v[2 * i + 1]), h[i], l[i]);
+          if (c + 2 * i >= a.rank) h[i] = l[i] = 0u;  // (R is a multiple of 8)
+        }
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
           *reinterpret_cast<uint4*>(hi + c + 2 * i) = make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]);
@@ -271,6 +273,7 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const __grid_constant__ 
     uint32_t h[2], l[2];
     split2(scale * sum.x, scale * sum.y, h[0], l[0]);
     split2(scale * sum.z, scale * sum.w, h[1], l[1]);
+    if (c >= a.rank) h[0] = h[1] = l[0] = l[1] = 0u;
     __nv_bfloat16* hi = a.h + (span.begin + row) * a.rp + c;
     *reinterpret_cast<uint2*>(hi) = make_uint2(h[0], h[1]);
     *reinterpret_cast<uint2*>(hi + a.rows.m * a.rp) = make_uint2(l[0], l[1]);
@@ -1167,6 +1170,7 @@ cudaError_t down(cudaStream_t st, const Rows& r, Matrix u, int64_t c, const void
                  int sms, uint32_t* err) {
   DownMaps maps;
   DownArgs a{};
+  a.rank = rank;
   a.rp = int(cdiv(rank, 16)) * 16;
   if (!make_map(&maps.u, u.p, c, r.m, 1, u.ld, kBox)) return cudaErrorInvalidValue;
   if (!(MN ? make_map(&maps.w, w, rank, c, r.adapters, rank, 64)

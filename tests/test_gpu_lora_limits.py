@@ -37,6 +37,27 @@ def test_gradients_of_many_adapters(cuda_device, lengths, adapters, slots):
     ops.check_operator_errors()
 
 
+@pytest.mark.parametrize("rows", [3, 100, 300])
+@pytest.mark.parametrize("rank", [8, 24, 16])
+def test_an_infinity_stays_one(cuda_device, rank, rows):
+    """An infinite x or dy of one row with positive weights makes that row's results +infinity, and no other row's."""
+    p = Problem([rows], 64, 72, rank, 1)
+    p.a.abs_()
+    p.b.abs_()
+    clean = ops.lora_update(p.y, *p.args)
+    grads = ops.lora_update_backward(p.dy, *p.args)
+    p.x[2, 5] = float("inf")
+    out = ops.lora_update(p.y, *p.args)
+    keep = torch.arange(rows, device="cuda") != 2
+    assert (out[2] == float("inf")).all() and torch.equal(out[keep], clean[keep])
+    p.x[2, 5] = 0.5
+    p.dy[2, 5] = float("inf")
+    dx, da, db = ops.lora_update_backward(p.dy, *p.args)
+    assert (dx[2] == float("inf")).all() and torch.equal(dx[keep], grads[0][keep])
+    assert torch.equal(da[0].double(), float("inf") * p.x[2].double().sign().expand(rank, -1))
+    assert not db[0, 5].isfinite().any() and db[0, 6:].isfinite().all()
+
+
 def test_gradients_of_a_alone_without_h(cuda_device):
     """The C entry needs h for the gradients of B only."""
     p = Problem([200, 30], 72, 64, 16, 2)
