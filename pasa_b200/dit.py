@@ -254,8 +254,8 @@ def _text_keys(text: torch.Tensor, w: dict, cfg: DiTConfig, fused: bool) -> torc
 def text_cache(text_embed: torch.Tensor, embed: dict, blocks: List[dict], cfg: DiTConfig,
                lengths: Optional[torch.Tensor] = None) -> TextCache:
     """The cache of a batch of texts for ``step``'s ``text_kv`` (bf16 weights on a GPU; heads of 64 or 128
-    dimensions).  ``text_embed`` [B, Lt, text_dim]; ``lengths`` int32 [B]: the texts' tokens (all Lt by default), which
-    are all that is attended to."""
+    dimensions).  ``text_embed`` [B, Lt, text_dim]; ``lengths`` int32 [B]: the texts' tokens (all Lt by default, and at
+    most), which are all that is attended to."""
     text = project_text(embed, text_embed)
     batch, tokens = text.shape[:2]
     width = -(-tokens // 64)
@@ -263,6 +263,7 @@ def text_cache(text_embed: torch.Tensor, embed: dict, blocks: List[dict], cfg: D
     starts = torch.zeros(batch, dtype=torch.int32, device=text.device)
     if lengths is None:
         lengths = torch.full_like(starts, tokens)
+    lengths = lengths.clamp(0, tokens)  # the rest of the last page has no tokens
     caches = []
     for w in blocks:
         cache = ops.kv8_cache(batch * width, cfg.heads, cfg.head_dim, device=text.device)
