@@ -6,6 +6,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -54,9 +55,19 @@ def check_operator_errors(device=None) -> None:
         raise RuntimeError(f"pasa_b200: {', '.join(reasons)} (error word {flags.value:#x})")
 
 
+def refuse_tangents(fn: str, *tensors) -> None:
+    """A tensor with a forward-mode tangent is refused: the kernels would return a result without one."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{fn} has no forward-mode derivative")
+
+
 def wants_grad(fn: str, *tensors) -> bool:
-    """Whether autograd has to see this call.  While a stream is captured that is refused: the engine may run leaves'
+    """Whether autograd has to see this call.  Forward-mode tangents are refused.  While a stream is captured that is refused: the engine may run leaves'
     accumulation on the stream of an eager graph of the same leaves, which a capture cannot contain."""
+    refuse_tangents(fn, *tensors)
     if not torch.is_grad_enabled():
         return False
     for t in tensors:

@@ -9,7 +9,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, overlaps_itself
+from ._launch import check_cuda, launch, overlaps_itself, refuse_tangents
 
 PAGE = 64
 _BF16 = (torch.bfloat16,)
@@ -70,6 +70,7 @@ def _strides(t: torch.Tensor):
 
 
 def _no_grad(fn: str, *tensors: torch.Tensor) -> None:
+    refuse_tangents(fn, *tensors)
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{fn} has no gradient; call it under torch.no_grad() or on detached tensors")
 

@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, wants_grad
+from ._launch import check_cuda, launch, refuse_tangents, wants_grad
 
 _BF16 = (torch.bfloat16,)
 _I32 = (torch.int32,)
@@ -188,11 +188,12 @@ def lora_update(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     K, N and R are multiples of 8, R at most 128 (other ranks: pad with zeros), S at most 4096.
 
     Returns a new tensor like y, or ``out`` (``out=y`` updates in place); with ``return_h`` also the scaled x A^T that
-    ``lora_update_backward`` takes.  Sums are fp32 and the result is rounded once.  Differentiable in y, x, a and b,
-    except under stream capture (capture ``lora_update_backward``).
+    ``lora_update_backward`` takes.  Sums are fp32 and the result is rounded once.  Differentiable in y, x, a and b
+    (in reverse mode), except under stream capture (capture ``lora_update_backward``).
     """
     if scale is not None and isinstance(scale, torch.Tensor) and scale.requires_grad:
         raise ValueError("lora_update has no gradient for scale")
+    refuse_tangents("lora_update", scale)
     if wants_grad("lora_update", y, x, a, b):
         if out is not None:
             raise ValueError("out is not differentiable")
@@ -214,5 +215,6 @@ def lora_update_backward(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: 
     without it a new one.  ``h``: the second result of ``lora_update(..., return_h=True)``; without it it is computed
     again.  y's gradient is dy itself.  No autograd: for explicit training steps, captured ones among them.
     """
+    refuse_tangents("lora_update_backward", dy, x, a, b, scale, h, dx)
     call = _Call(x, a, b, rows, slots, scale)
     return _backward(call, dy, x.shape, h, dx, True, True, True)
