@@ -81,6 +81,11 @@ def wants_grad(fn: str, *tensors) -> bool:
     return True
 
 
+def written(*tensors: torch.Tensor) -> None:
+    """Tells autograd that they were written in place: what an operation before has saved of them is no longer valid."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def overlaps_itself(t: torch.Tensor) -> bool:
     """Whether two elements share memory, for the strides that views have (a broadcast dimension)."""
     return any(size > 1 and stride == 0 for size, stride in zip(t.shape, t.stride()))

@@ -9,7 +9,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, overlaps_itself, refuse_tangents
+from ._launch import check_cuda, launch, overlaps_itself, refuse_tangents, written
 
 PAGE = 64
 _BF16 = (torch.bfloat16,)
@@ -108,6 +108,7 @@ def kv8_write(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, t
     k, v, table, starts = _rows(k), _rows(v), table.contiguous(), starts.contiguous()
     launch("pasa_kv8_write", device, k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), *args, table.data_ptr(),
            table.shape[1], starts.data_ptr(), None if counts is None else counts.data_ptr(), batch, tokens)
+    written(*cache)
 
 
 @functools.lru_cache(maxsize=None)
@@ -145,8 +146,8 @@ def kv8_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], table: torch.T
     if not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive")
     _no_grad("kv8_attention", q)
-    q = _rows(q)
-    if out is None:
+    q, given = _rows(q), out is not None
+    if not given:
         out = torch.empty_like(q)
         if out.stride(3) != 1 or (out.stride(0) | out.stride(1) | out.stride(2)) & 7:
             out = torch.empty(q.shape, dtype=q.dtype, device=device)
@@ -164,4 +165,6 @@ def kv8_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], table: torch.T
     launch("pasa_kv8_attention", device, q.data_ptr(), _strides(q), *args, table.data_ptr(), table.shape[1],
            lengths.data_ptr(), batch, queries, q_heads // heads, scale, out.data_ptr(), _strides(out),
            workspace.data_ptr(), size)
+    if given:
+        written(out)
     return out

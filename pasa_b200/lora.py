@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, refuse_tangents, wants_grad
+from ._launch import check_cuda, launch, refuse_tangents, wants_grad, written
 
 _BF16 = (torch.bfloat16,)
 _I32 = (torch.int32,)
@@ -109,7 +109,8 @@ def _forward(call: _Call, y, out):
     base, ldy = _matrix(y, "y", call.device)
     if base.shape != (call.m, call.n):
         raise ValueError(f"y must have {call.m} rows of {call.n} columns, got shape {tuple(y.shape)}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
         target, ldo = out, call.n
     else:
@@ -121,6 +122,8 @@ def _forward(call: _Call, y, out):
     h = call.h()
     launch("pasa_lora_update", call.device, call.x.data_ptr(), call.ldx, base.data_ptr(), ldy, *call.weights,
            *call.sizes, h.data_ptr(), target.data_ptr(), ldo)
+    if given:
+        written(out)
     return out, h
 
 
@@ -128,8 +131,8 @@ def _backward(call: _Call, dy, x_shape, h, dx, need_x, need_a, need_b):
     grad, lddy = _matrix(dy, "dy", call.device)
     if grad.shape != (call.m, call.n):
         raise ValueError(f"dy must have {call.m} rows of {call.n} columns, got shape {tuple(dy.shape)}")
-    base = ldbase = 0
-    if dx is not None:
+    base, ldbase, adds = 0, 0, dx is not None
+    if adds:
         target, lddx = _target(dx, "dx", x_shape, call.device)
         if target.data_ptr() in (call.x.data_ptr(), grad.data_ptr()) and dx.numel():
             raise ValueError("dx is x or dy")
@@ -152,6 +155,8 @@ def _backward(call: _Call, dy, x_shape, h, dx, need_x, need_a, need_b):
     launch("pasa_lora_update_backward", call.device, grad.data_ptr(), lddy, call.x.data_ptr(), call.ldx, *call.weights,
            *call.sizes, h.data_ptr(), int(given), base or None, ldbase, target.data_ptr() if dx is not None else None,
            lddx if dx is not None else 0, ptr(da), ptr(db), workspace.data_ptr(), size)
+    if adds:
+        written(dx)
     return dx, da, db
 
 

@@ -10,7 +10,7 @@ from typing import NamedTuple, Optional, Sequence, Union
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, overlaps_itself, wants_grad
+from ._launch import check_cuda, launch, overlaps_itself, wants_grad, written
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 _POS_TYPES = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32,
@@ -157,6 +157,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, axes: Sequen
         if k is not None and k.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("q and k are the same memory: it would be turned twice")
         _apply(tensors, tensors, positions, plan, inverse)
+        written(*tensors)
     else:
         tensors = _turn(tensors, positions, plan, inverse)
     return tensors[0] if k is None else tensors

@@ -10,6 +10,34 @@ from test_gpu_lora import Problem
 pytestmark = pytest.mark.gpu
 
 
+def changed_after_it_was_saved(t, change):
+    """Whether autograd notices that ``change`` writes t, which an operation before it has saved."""
+    w = torch.ones_like(t, requires_grad=True)
+    product = (w * t).sum()
+    with torch.no_grad():
+        change(t)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+
+
+def test_writes_in_place_are_noticed(cuda_device):
+    p = Problem([100], 64, 64, 8, 1)
+    changed_after_it_was_saved(p.y, lambda t: ops.lora_update(t, *p.args, out=t))
+    changed_after_it_was_saved(torch.zeros_like(p.y), lambda t: ops.lora_update(p.y, *p.args, out=t))
+    changed_after_it_was_saved(torch.zeros_like(p.x), lambda t: ops.lora_update_backward(p.dy, *p.args, dx=t))
+    rope = dict(axes=(8, 8), grid=(4, 5), inplace=True)
+    changed_after_it_was_saved(randn(1, 2, 20, 32), lambda t: ops.rope_axes(t, **rope))
+    changed_after_it_was_saved(randn(1, 2, 20, 32), lambda t: ops.rope_axes(randn(1, 2, 20, 32), t, **rope))
+    c = Pages([100], 2, 64).fill()
+    changed_after_it_was_saved(randn(1, 2, 7, 64), lambda t: ops.kv8_attention(t, c.cache, c.table, i32([100]), out=t))
+    before = [t._version for t in c.cache]
+    ops.kv8_write(c.cache, randn(1, 2, 3, 64), randn(1, 2, 3, 64), c.table, i32([97]))
+    assert all(t._version > v for t, v in zip(c.cache, before))
+    with torch.inference_mode():  # tensors without a counter
+        q = randn(1, 2, 20, 32)
+        assert ops.rope_axes(q, **rope) is q
+
+
 def test_forward_mode_is_refused(cuda_device):
     p = Problem([100], 64, 64, 8, 1)
     c = Pages([100], 2, 64).fill()
