@@ -81,6 +81,12 @@ def wants_grad(fn: str, *tensors) -> bool:
     return True
 
 
+def check_target(name: str, t: torch.Tensor) -> None:
+    """A tensor that is written in place has no history that autograd would have to know of."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} is written in place and must not require a gradient")
+
+
 def written(*tensors: torch.Tensor) -> None:
     """Tells autograd that they were written in place: what an operation before has saved of them is no longer valid."""
     torch.autograd.graph.increment_version(tensors)

@@ -9,7 +9,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, overlaps_itself, refuse_tangents, written
+from ._launch import check_cuda, check_target, launch, overlaps_itself, refuse_tangents, written
 
 PAGE = 64
 _BF16 = (torch.bfloat16,)
@@ -153,6 +153,7 @@ def kv8_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], table: torch.T
             out = torch.empty(q.shape, dtype=q.dtype, device=device)
     else:
         check_cuda("out", out, 4, _BF16, device)
+        check_target("out", out)
         if out.shape != q.shape:
             raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
         if out.numel() and (out.stride(3) != 1 or (out.stride(0) | out.stride(1) | out.stride(2)) & 7

@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._launch import check_cuda, launch, refuse_tangents, wants_grad, written
+from ._launch import check_cuda, check_target, launch, refuse_tangents, wants_grad, written
 
 _BF16 = (torch.bfloat16,)
 _I32 = (torch.int32,)
@@ -34,6 +34,7 @@ def _matrix(t: torch.Tensor, name: str, device=None):
 def _target(t: torch.Tensor, name: str, shape, device):
     """A tensor that is written in place, as rows of one stride."""
     check_cuda(name, t, None, _BF16, device)
+    check_target(name, t)
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     try:

@@ -38,6 +38,22 @@ def test_writes_in_place_are_noticed(cuda_device):
         assert ops.rope_axes(q, **rope) is q
 
 
+def test_targets_that_require_a_gradient(cuda_device):
+    p = Problem([100], 64, 64, 8, 1)
+    c = Pages([100], 2, 64).fill()
+    q = randn(1, 2, 7, 64)
+    for call, like in ((lambda t: ops.lora_update(p.y, *p.args, out=t), p.y),
+                       (lambda t: ops.lora_update_backward(p.dy, *p.args, dx=t), p.x),
+                       (lambda t: ops.kv8_attention(q, c.cache, c.table, i32([100]), out=t), q)):
+        with pytest.raises(ValueError, match="require"):
+            call(torch.zeros_like(like, requires_grad=True))
+        leaf = torch.zeros_like(like, requires_grad=True)
+        with pytest.raises(ValueError, match="require"):
+            call(leaf * 1)
+        with torch.no_grad():
+            call(leaf)
+
+
 def test_forward_mode_is_refused(cuda_device):
     p = Problem([100], 64, 64, 8, 1)
     c = Pages([100], 2, 64).fill()
