@@ -49,6 +49,21 @@ def _target(t: torch.Tensor, name: str, shape, device):
     return m, cols if rows <= 1 else step
 
 
+def _overlap(a: torch.Tensor, lda: int, b: torch.Tensor, ldb: int) -> bool:
+    """Whether two bf16 matrices (rows lda and ldb values apart) share memory.  Columns of the same rows beside one
+    another do not; of rows that lie differently among one another that is not found out."""
+    if not a.numel() or not b.numel():
+        return False
+    at = (a.data_ptr() - b.data_ptr()) // 2
+    if at >= (b.shape[0] - 1) * ldb + b.shape[1] or -at >= (a.shape[0] - 1) * lda + a.shape[1]:
+        return False
+    steps = {ld for m, ld in ((a, lda), (b, ldb)) if m.shape[0] > 1}
+    if len(steps) != 1:
+        return True
+    step = steps.pop()
+    return at % step < b.shape[1] or at % step + a.shape[1] > step
+
+
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(m, k, n, rank, adapters, requests, index: int) -> int:
     size = ctypes.c_size_t()
@@ -116,9 +131,9 @@ def _forward(call: _Call, y, out):
         target, ldo = out, call.n
     else:
         target, ldo = _target(out, "out", y.shape, call.device)
-        if target.data_ptr() == call.x.data_ptr() and out.numel():
-            raise ValueError("out is x")
-        if target.data_ptr() == base.data_ptr() and ldo != ldy:
+        if _overlap(target, ldo, call.x, call.ldx):
+            raise ValueError("out is x or overlaps it")
+        if (target.data_ptr() != base.data_ptr() or ldo != ldy) and _overlap(target, ldo, base, ldy):
             raise ValueError("out overlaps y: it may be y itself")
     h = call.h()
     launch("pasa_lora_update", call.device, call.x.data_ptr(), call.ldx, base.data_ptr(), ldy, *call.weights,
@@ -135,8 +150,8 @@ def _backward(call: _Call, dy, x_shape, h, dx, need_x, need_a, need_b):
     base, ldbase, adds = 0, 0, dx is not None
     if adds:
         target, lddx = _target(dx, "dx", x_shape, call.device)
-        if target.data_ptr() in (call.x.data_ptr(), grad.data_ptr()) and dx.numel():
-            raise ValueError("dx is x or dy")
+        if _overlap(target, lddx, call.x, call.ldx) or _overlap(target, lddx, grad, lddy):
+            raise ValueError("dx is x or dy, or overlaps one of them")
         base, ldbase = target.data_ptr(), lddx
     elif need_x:
         dx = torch.empty(x_shape, dtype=torch.bfloat16, device=call.device)

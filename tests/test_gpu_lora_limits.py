@@ -81,6 +81,36 @@ def test_gradients_of_a_alone_without_h(cuda_device):
     assert call(None, None, None, db) == _lib.ERR_NULL
 
 
+def test_targets_that_overlap_what_is_read(cuda_device):
+    p = Problem([100], 64, 64, 8, 1)
+    want = ops.lora_update(p.y, *p.args)
+    wide = torch.zeros(101, 200, device="cuda", dtype=torch.bfloat16)
+    x, rest = wide[:100, :64], p.args[1:]
+    x.copy_(p.x)
+    for out in (wide[:100, 32:96], wide[1:, :64], wide[:100, 56:120], wide[:100, 192:193].expand(-1, 64)):
+        with pytest.raises(ValueError):
+            ops.lora_update(p.y, x, *rest, out=out)
+        with pytest.raises(ValueError):
+            ops.lora_update_backward(p.dy, x, *rest, dx=out)
+    assert torch.equal(ops.lora_update(p.y, x, *rest, out=wide[:100, 64:128]), want)  # beside x in the same rows
+    assert torch.equal(x, p.x)
+    tall = torch.zeros(205, 64, device="cuda", dtype=torch.bfloat16)
+    y = tall[:100]
+    y.copy_(p.y)
+    for out in (tall[1:101], tall[99:199]):
+        with pytest.raises(ValueError):
+            ops.lora_update(y, *p.args, out=out)
+        with pytest.raises(ValueError):
+            ops.lora_update_backward(y, *p.args, dx=out)
+    assert torch.equal(ops.lora_update(y, *p.args, out=tall[100:200]), want)
+    assert torch.equal(ops.lora_update(y, *p.args, out=y), want)
+    one = Problem([1], 64, 64, 8, 1)
+    line = torch.zeros(64 + 32, device="cuda", dtype=torch.bfloat16)
+    line[:64] = one.x[0]
+    with pytest.raises(ValueError):
+        ops.lora_update(one.y, line[None, :64], *one.args[1:], out=line[None, 32:])
+
+
 def test_row_offsets_that_go_back_end(cuda_device):
     """Offsets must not decrease.  Where they do, the calls end all the same, here with 2^31 stages to sum by the
     requests' sizes, and what lies behind the tensors stays as it is."""
