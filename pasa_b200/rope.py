@@ -29,8 +29,7 @@ class _Plan(NamedTuple):
 
 @functools.lru_cache(maxsize=256)
 def _plan(axes, theta, pairs, grid, origin) -> _Plan:
-    axes = tuple(int(d) for d in axes)
-    theta = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(axes)
+    theta = theta if isinstance(theta, tuple) else (theta,) * len(axes)
     if not 1 <= len(axes) <= 4 or any(d < 0 or d % 2 for d in axes) or not 2 <= sum(axes) <= 256:
         raise ValueError(f"axes are 1 to 4 even numbers of dimensions, 2 to 256 together, got {axes}")
     if len(theta) != len(axes) or any(not 0 < t < math.inf for t in theta):
@@ -40,8 +39,7 @@ def _plan(axes, theta, pairs, grid, origin) -> _Plan:
     freqs = [t ** (-2 * i / d) for d, t in zip(axes, theta) for i in range(d // 2)]
     where = points = None
     if grid is not None:
-        grid = tuple(int(n) for n in grid)
-        origin = (0,) * len(axes) if origin is None else tuple(int(n) for n in origin)
+        origin = (0,) * len(axes) if origin is None else origin
         if len(grid) != len(axes) or len(origin) != len(axes) or min(grid) < 0:
             raise ValueError(f"grid {grid} and origin {origin} need one number for each of {len(axes)} axes")
         points = math.prod(grid)
@@ -134,8 +132,10 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, axes: Sequen
         tensors = (q, k)
     if (positions is None) == (grid is None):
         raise ValueError("give either positions or grid")
-    plan = _plan(tuple(axes), tuple(theta) if isinstance(theta, (tuple, list)) else theta, pairs,
-                 None if grid is None else tuple(grid), None if origin is None else tuple(origin))
+    # (numbers, not objects that hold them: plans are found again by their values)
+    plan = _plan(tuple(map(int, axes)), tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta),
+                 pairs, None if grid is None else tuple(map(int, grid)),
+                 None if origin is None else tuple(map(int, origin)))
     if plan.turned > dim:
         raise ValueError(f"axes {plan.axes} take more than the {dim} dimensions of a head")
     if grid is not None and plan.points != tokens:
