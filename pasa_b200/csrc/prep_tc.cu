@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) prep_umma_kernel(
       for (int n = kBlock; n > 1; n >>= 1)
 #pragma unroll
         for (int r = 0; r < n / 2; ++r) x[r] = prep_tc::add_bf16x2(x[r], x[r + n / 2]);
+      __threadfence_block();  // an arrival does not wait for loads before it
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);  // this warp's reads of the stage are done
       const uint32_t sum2 = x[0];
