@@ -604,8 +604,10 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
 // rows' epilogue, 1500 clocks for 8 KB of weights; here 24 single rows of
 // 5120 -> 30720 at rank 64 (76 MB) take 34 us where they took 57 us.
 // ---------------------------------------------------------------------------
-constexpr int kFewRows = 4;         // rows of a span
-constexpr int kFewMost = 64;        // rows of a call that takes this way
+// Rows of a span; 5120 -> 30720 at rank 64 with 2, 4 and 8: one request of 16 rows 14.3, 14.3 and 17.8 us, 64 requests of
+// one row 63, 72 and 80; 1536 -> 8960 at rank 128, one request of 32 rows: 17.3, 15.1 and 18.3.
+constexpr int kFewRows = 4;
+constexpr int kFewMost = 64;        // rows of a call that may take this way: few_rows
 constexpr int kFewRanks = 8;        // ranks of a down block
 constexpr int kFewWarps = 8;
 constexpr int kFewCols = 128;       // columns of an up block, one a thread
@@ -1249,7 +1251,20 @@ cudaError_t up(cudaStream_t st, const Rows& r, const __nv_bfloat16* h, const voi
   return cudaLaunchKernelEx(&cfg, up_kernel<MN>, maps, a);
 }
 
-// The kernels for at most kFewMost rows.
+// Whether a call takes the kernels for few rows.  They read an adapter's weights for every four rows of a request, the
+// others for every 128, and take 6 us less to begin with; what a read costs beside is fitted to the times of 1 to 128
+// rows.  (us, here / there.  5120 -> 30720, rank 64: one request of 16, 24 and 64 rows 14.3 / 16.2, 17.2 / 16.8 and
+// 28.8 / 17.1, 16 and 64 requests of one row 21 / 41 and 72 / 120.  1536 -> 8960, rank 128: 24, 32 and 64 rows 14.8 /
+// 14.9, 15.1 / 15.5 and 26 / 16.7; 64 and 128 requests 50 / 48 and 98 / 90.  5120 -> 5120, rank 16: one request of 64
+// rows 9.2 / 13.5, 64 requests 13 / 35.)  The requests' lengths are not known here: they are taken to be equal.
+bool few_rows(const Rows& r, int64_t k, int64_t n, int rank) {
+  if (r.m > kFewMost) return false;
+  const double mb = double(rank) * double(k + n) * 2e-6;
+  const int64_t requests = r.requests < 1 ? 1 : r.requests < r.m ? r.requests : r.m;
+  const int64_t reads = requests * cdiv(cdiv(r.m, requests), kFewRows);
+  return 0.35 * mb * double(reads) <= 6.0 + double(requests) * (0.3 + 0.3 * mb);
+}
+
 unsigned few_spans(const Rows& r) {
   const int64_t spans = cdiv(r.m, kFewRows) + r.requests + 1;
   return unsigned(spans < r.m ? spans : r.m);  // every span has a row
@@ -1297,9 +1312,9 @@ cudaError_t up_few(cudaStream_t st, const Rows& r, __nv_bfloat16* h, const void*
 }
 
 // h of x, the same wherever it is computed.
-cudaError_t down_a(cudaStream_t st, const Rows& r, Matrix x, int64_t k, const void* a, int rank, __nv_bfloat16* h,
-                   int sms, uint32_t* err) {
-  return r.m <= kFewMost ? down_few(st, r, x, k, a, rank, h) : down<false>(st, r, x, k, a, rank, h, sms, err);
+cudaError_t down_a(cudaStream_t st, const Rows& r, Matrix x, int64_t k, int64_t n, const void* a, int rank,
+                   __nv_bfloat16* h, int sms, uint32_t* err) {
+  return few_rows(r, k, n, rank) ? down_few(st, r, x, k, a, rank, h) : down<false>(st, r, x, k, a, rank, h, sms, err);
 }
 
 int64_t grad_blocks(int64_t c, int rank) { return cdiv(c, grad_cols(rank <= 64 ? 1 : 2)); }
@@ -1424,10 +1439,10 @@ int pasa_lora_update(void* stream, const void* x, int64_t ldx, const void* y, in
   const Rows r{rows, slots, scale, int(requests), int(adapters), m};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   __nv_bfloat16* hh = static_cast<__nv_bfloat16*>(h);
-  cudaError_t e = down_a(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
+  cudaError_t e = down_a(s, r, Matrix{x, ldx}, k, n, a, rank, hh, sms, err);
   if (e == cudaSuccess)
-    e = m <= kFewMost ? up_few(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo})
-                      : up<false>(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo}, sms, err);
+    e = few_rows(r, k, n, rank) ? up_few(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo})
+                                : up<false>(s, r, hh, b, rank, n, Matrix{y, ldy}, Matrix{out, ldo}, sms, err);
   return e == cudaSuccess ? PASA_OK : PASA_ERR_CUDA;
 }
 
@@ -1480,7 +1495,7 @@ int pasa_lora_update_backward(void* stream, const void* dy, int64_t lddy, const 
   size_t h_bytes = 0;
   pasa_lora_h_size(m, rank, &h_bytes);
   cudaError_t e = cudaSuccess;
-  if (db && !h_given && requests) e = down_a(s, r, Matrix{x, ldx}, k, a, rank, hh, sms, err);
+  if (db && !h_given && requests) e = down_a(s, r, Matrix{x, ldx}, k, n, a, rank, hh, sms, err);
   if (e == cudaSuccess && (dx || da)) e = down<true>(s, r, Matrix{dy, lddy}, n, b, rank, g, sms, err);
   if (e == cudaSuccess && dx)
     e = up<true>(s, r, g, a, rank, k, Matrix{dx_base, ldbase}, Matrix{dx, lddx}, sms, err);
