@@ -212,7 +212,7 @@ def lora_update(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     ``lora_update_backward`` takes.  Sums are fp32 and the result is rounded once.  Differentiable in y, x, a and b
     (in reverse mode), except under stream capture (capture ``lora_update_backward``).
     """
-    if scale is not None and isinstance(scale, torch.Tensor) and scale.requires_grad:
+    if torch.is_grad_enabled() and isinstance(scale, torch.Tensor) and scale.requires_grad:
         raise ValueError("lora_update has no gradient for scale")
     refuse_tangents("lora_update", scale)
     if wants_grad("lora_update", y, x, a, b):

@@ -75,3 +75,14 @@ def test_forward_mode_is_refused(cuda_device):
         ops.rope_axes(q, axes=(8, 8), grid=(4, 5))
         ops.lora_update(p.y, *p.args)
         ops.kv8_attention(q, c.cache, c.table, i32([100]))
+
+
+def test_a_scale_that_requires_a_gradient(cuda_device):
+    """It has none; without gradients it is a scale like any other."""
+    p = Problem([100], 64, 64, 8, 1)
+    want = ops.lora_update(p.y, *p.args)
+    p.scale.requires_grad_()
+    with pytest.raises(ValueError, match="scale"):
+        ops.lora_update(p.y, *p.args)
+    with torch.no_grad():
+        assert torch.equal(ops.lora_update(p.y, *p.args), want)
