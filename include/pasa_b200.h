@@ -532,7 +532,8 @@ PASA_API int pasa_kv8_write(void* stream, const void* k, const int64_t* k_stride
  * out = softmax(scale q k^T) v over each request's first lengths[b] tokens
  * (device int32; cut at width * 64); zero for a request without tokens.
  *   q, out  bf16 [batch, heads * group, queries, dim]; query head h reads
- *           key/value head h / group.  Strides as above, 16-byte aligned.
+ *           key/value head h / group.  Strides as above, 16-byte aligned.  out
+ *           may be q itself, no other overlap.
  *   scale   positive
  *   workspace  pasa_kv8_attention_workspace_size bytes, not shared by two calls
  *           that may run at the same time

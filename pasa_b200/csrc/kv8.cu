@@ -11,8 +11,10 @@
 //
 //   write      rounds new tokens into pages.  Where a page has earlier tokens its
 //              scale is the larger of theirs and the new ones', and they are
-//              rounded again to it.  Bound: HBM, 2 bytes read and 1 written a value
-//              (4680 tokens, 12 heads of 128, 43 MB: 12 us, 3.6 TB/s).
+//              rounded again to it.  Reads 2 bytes and writes 1 a value; a block has
+//              a page and head and waits for its maximum before it writes, which is
+//              what bounds it (4680 tokens, 12 heads of 128, 43 MB: 12 us, 3.6 TB/s;
+//              one token of 8 requests, 8 heads: 4.2 us).
 //   attention  out = softmax(q k^T scale) v over a request's first `length`
 //              tokens.  Bound: the tensor cores for many queries, HBM (one byte a
 //              value) for single tokens.

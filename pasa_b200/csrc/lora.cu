@@ -15,8 +15,8 @@
 // traffic and lets each kernel split its own long axis: down splits K over a
 // cluster of up to 8 CTAs when there are few rows (the partial sums meet in
 // distributed shared memory, in rank order), up splits N.  Measured: 75600 rows,
-// 5120 -> 5120, R = 32: down 133 us (5.8 TB/s), up 328 us (4.7 TB/s); 32760 rows,
-// R = 64: grad 137 us (4.9 TB/s).
+// 5120 -> 5120, R = 32: down 133 us (5.8 TB/s), up 332 us (4.7 TB/s); 32760 rows,
+// R = 64: grad 131 us (5.1 TB/s).
 //
 // Rounding: h and g are products' operands again, and are kept as two bf16
 // terms, v = hi + lo to 2^-17 of v, each multiplied and accumulated in fp32:
@@ -101,7 +101,8 @@ __device__ __forceinline__ Span find_span(const Rows& a, int64_t t, int lane) {
   return s;
 }
 
-// v = hi + lo in two bf16 terms; an infinity or NaN is hi alone.
+// v = hi + lo in two bf16 terms; an infinity or NaN is hi alone.  (Times an infinite element of the other operand the
+// two terms may differ in sign: such a sum is infinite or NaN.)
 __device__ __forceinline__ void split2(float v0, float v1, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(v0, v1);
   const float h0 = __uint_as_float(hi << 16), h1 = __uint_as_float(hi & 0xFFFF0000u);
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(kUpThreads, 2) up_kernel(const __grid_constant
 // weights once and do next to nothing with them, so what counts is how many
 // loads are in flight.  On the tensor cores a span of one row still takes 128
 // rows' epilogue, 1500 clocks for 8 KB of weights; here 24 single rows of
-// 5120 -> 30720 at rank 64 (76 MB) take 34 us where they took 57 us.
+// 5120 -> 30720 at rank 64 (76 MB) take 33 us where they took 57 us.
 // ---------------------------------------------------------------------------
 // Rows of a span; 5120 -> 30720 at rank 64 with 2, 4 and 8: one request of 16 rows 14.3, 14.3 and 17.8 us, 64 requests of
 // one row 63, 72 and 80; 1536 -> 8960 at rank 128, one request of 32 rows: 17.3, 15.1 and 18.3.

@@ -188,7 +188,8 @@ def head_to_tokens(t: torch.Tensor, group) -> torch.Tensor:
 class Adapters(NamedTuple):
     """Low-rank adapters of a step's requests.  ``slots`` int32 [B]: the adapter of each batch entry, -1 for none;
     ``scale`` fp32 [adapters] or None for 1; ``blocks``: for each block the adapted projections (of "q", "k", "v",
-    "o", "cq", "co", "ffn1", "ffn2") with their a [adapters, rank, in] and b [adapters, out, rank]."""
+    "o", "cq", "co", "ffn1", "ffn2") with their a [adapters, rank, in] and b [adapters, out, rank].  The fused step has
+    no gradients: adapters that require one are refused where they are recorded."""
     slots: torch.Tensor
     scale: Optional[torch.Tensor]
     blocks: Sequence[Dict[str, Tuple[torch.Tensor, torch.Tensor]]]

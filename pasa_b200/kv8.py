@@ -127,7 +127,7 @@ def kv8_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], table: torch.T
     q: bf16 [B, Hq, L, D] (any strides), Hq a multiple of the cache's heads H: query head h reads head h * H // Hq.
     ``table`` int32 [B, W] as for ``kv8_write``, ``lengths`` int32 [B] (cut at 64 W), both on the GPU and read there.
     ``scale`` is positive, D**-0.5 by default.  Returns a new tensor with q's strides, or ``out`` (its last stride 1,
-    the others multiples of 8).  Queries enter the products to 8 significant bits (or 2^-17 of the row's largest
+    the others multiples of 8; it may be q, and must not overlap it otherwise).  Queries enter the products to 8 significant bits (or 2^-17 of the row's largest
     element), probabilities to 11 (or 2^-36 of the largest), sums are fp32.  Has no gradient.
     A needed table entry that is no page, or a scale that is no power of two, makes the rows that need it NaN and is
     reported by ``check_operator_errors``.

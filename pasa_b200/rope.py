@@ -118,7 +118,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, axes: Sequen
 
     ``inverse`` turns back, which is also the gradient: d(rope)/dx applied to dy is ``rope_axes(dy, inverse=True)``.
     Angles are formed in fp64, the rotation in fp32, and rounded once.  Returns new tensors like q and k (one tensor
-    without k), or q and k themselves with ``inplace``.  Differentiable in q and k (in
+    without k), or q and k themselves with ``inplace`` (they must not overlap).  Differentiable in q and k (in
     reverse mode), except under stream capture.
     """
     check_cuda("q", q, 4, _DTYPES)
